@@ -272,6 +272,62 @@ int tf_rmsnorm_fp8_w4a16_linear(const uint16_t* x, int64_t ldx, const uint16_t* 
                                 int64_t k, int32_t group_size, const tf_gemm_config* cfg,
                                 int32_t epilogue, void* stream);
 
+/* --------------------------------------------------------------- FP8 with a scale per block of 128 */
+
+/* 16-bit element types of the entry points below. */
+#define TF_DTYPE_FP16 0
+#define TF_DTYPE_BF16 1
+
+/* Longest row the quantizers reduce as a whole (the norm; every producer with group_size 0). */
+#define TF_FP8_MAX_ROW 32768
+
+/* Three producers of e4m3 codes with scales, no counterpart in the reference (its one quantizer is
+ * rmsnorm_fp8_quant, one scale per row). For each row of y [t, k], in fp32 without a 16-bit
+ * rounding on the way:
+ *   scale = max(amax|y| / 448, 1/(448*512)) over each 128 elements of the row (the last block may
+ *           be shorter; group_size 128, scale fp32 [t, ceil(k/128)]) or over the row (group_size
+ *           0, scale fp32 [t], the form tf_w4a8_linear_ex reads)
+ *   q     = e4m3fn(RNE(y / scale)), uint8 [t, k]
+ * q and scale are contiguous. A NaN or infinity in a block (row) reaches that block (row) alone.
+ *
+ * tf_fp8_quant: y = x [t, k], row stride ldx.
+ * tf_silu_mul_fp8_quant: y = silu(x[:, :k]) * x[:, k:], x [t, 2k], silu(v) = v / (1 + exp(-v)).
+ * tf_add_rmsnorm_fp8_quant: hidden = x + residual in the 16-bit type, written [t, k] contiguous
+ *   (residual NULL: hidden = x, not written, and may be NULL); y = hidden / sqrt(mean(hidden^2) +
+ *   eps) * weight, weight [k]. */
+int tf_fp8_quant(const uint16_t* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale, int64_t t,
+                 int64_t k, int32_t group_size, void* stream);
+int tf_silu_mul_fp8_quant(const uint16_t* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale,
+                          int64_t t, int64_t k, int32_t group_size, void* stream);
+int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr,
+                             const uint16_t* weight, int32_t dtype, uint8_t* q, float* scale,
+                             uint16_t* hidden, int64_t t, int64_t k, float eps, int32_t group_size,
+                             void* stream);
+
+/* Kernel families of tf_fp8_block_linear (the `kernel` field of its tf_gemm_config; they are not
+ * in the variant table above, which lists the int4 kernels). */
+#define TF_KERNEL_FP8_BLOCK_GEMV 4 /* weights from memory to the MFMA; block_m rows x 16 columns per
+                                      workgroup, num_warps waves share K                            */
+
+/* The linear on e4m3 codes and e4m3 weights, a scale per 128 of K on both sides. No counterpart in
+ * the reference (its weights are int4); for FP8 checkpoints with 128 x 128 weight scales.
+ *   out[m][n] = round16( sum_b xscale[m][b] * wscale[n/128][b]
+ *                              * sum_{k in 128b..128b+127} e4m3(x8[m][k]) * e4m3(weight[n][k])
+ *                        + bias[n] + residual[m][n] )
+ * x8 [m, k] and weight [n, k]: e4m3fn codes, 16-byte aligned rows (strides ldx8, ldw in bytes);
+ * xscale fp32 [m, ceil(k/128)] and wscale fp32 [ceil(n/128), ceil(k/128)] (strides in elements);
+ * bias [n], residual [m, n] (stride ldr) or NULL and out [m, n] (stride ldo) of type `dtype`. k a
+ * multiple of 16; n and m any. A block's products are summed by the MFMA, the blocks in fp32, and
+ * bias and residual are added in fp32 before the one rounding. cfg: one of the compiled configs
+ * (else TF_EINVAL); workspace: fp32, >= tf_fp8_block_workspace_bytes (-1 for an unknown config). */
+int64_t tf_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k, const tf_gemm_config* cfg);
+int tf_fp8_block_linear(const uint8_t* x8, int64_t ldx8, const float* xscale, int64_t ldxs,
+                        const uint8_t* weight, int64_t ldw, const float* wscale, int64_t ldws,
+                        const uint16_t* bias, const uint16_t* residual, int64_t ldr, uint16_t* out,
+                        int64_t ldo, int32_t dtype, int64_t m, int64_t n, int64_t k,
+                        const tf_gemm_config* cfg, float* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 /* Test hook for the e4m3fn encoding used by tf_rmsnorm_fp8_quant
  * (rmsnorm_fp8.py:29-41 _round_to_e4m3_grid + cast): fp32 [count] -> uint8 [count], through
  * the same hardware conversion (v_cvt_pk_fp8_f32) and NaN handling as that kernel.

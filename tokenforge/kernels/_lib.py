@@ -24,6 +24,10 @@ TF_ELAUNCH = 2
 TF_ERANGE = 3
 
 KERNEL_IDS = {"gemv_dot": 0, "gemv_mfma": 1, "gemm_mfma": 2, "gemm_fp8": 3}
+BLOCK_KERNEL_IDS = {"gemv_block": 4}
+"""Kernel families of ``tf_fp8_block_linear`` (TF_KERNEL_FP8_BLOCK_*)."""
+FP8_MAX_ROW = 32768
+"""TF_FP8_MAX_ROW: longest row the FP8 quantizers reduce as a whole."""
 EPILOGUE_NONE = 0
 EPILOGUE_RESIDUAL = 1
 EPILOGUE_SILU_MUL = 2
@@ -104,6 +108,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_p, _i64, _p, _f32, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32,
          ctypes.POINTER(TfGemmConfig), _i32, _p]),
+    "tf_fp8_quant": (ctypes.c_int, [_p, _i64, _i32, _p, _p, _i64, _i64, _i32, _p]),
+    "tf_silu_mul_fp8_quant": (ctypes.c_int, [_p, _i64, _i32, _p, _p, _i64, _i64, _i32, _p]),
+    "tf_add_rmsnorm_fp8_quant": (
+        ctypes.c_int, [_p, _i64, _p, _i64, _p, _i32, _p, _p, _p, _i64, _i64, _f32, _i32, _p]),
+    "tf_fp8_block_workspace_bytes": (_i64, [_i64, _i64, _i64, ctypes.POINTER(TfGemmConfig)]),
+    "tf_fp8_block_linear": (
+        ctypes.c_int,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64,
+         ctypes.POINTER(TfGemmConfig), _p, _i64, _p]),
     "tf_e4m3_encode": (ctypes.c_int, [_p, _p, _i64, _p]),
 }
 

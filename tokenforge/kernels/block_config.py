@@ -1,0 +1,38 @@
+"""Launch configurations of the block-scaled e4m3 linear (``fp8_block_linear``).
+
+A call's config follows from its M, N and K alone, by the rule of :func:`block_config`; there is no
+table of tuned layers. ``BLOCK_TILES`` lists what the library compiles.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+BLOCK = 128
+"""K and N of a weight's scale block, and K of an activation's."""
+
+
+@dataclass(frozen=True)
+class BlockConfig:
+    """One launch: ``gemv_block`` (block_m rows x 16 columns per workgroup, ``num_warps`` waves share
+    K)."""
+
+    kernel: str
+    block_m: int
+    block_n: int
+    split_k: int
+    num_warps: int
+    num_stages: int
+
+
+BLOCK_TILES: tuple[tuple[str, int, int, int, int], ...] = (
+    ("gemv_block", 16, 16, 8, 1), ("gemv_block", 64, 16, 4, 1),
+)
+"""(kernel, block_m, block_n, num_warps, num_stages) of every compiled kernel."""
+
+
+def block_config(m: int, n: int, k: int) -> BlockConfig:
+    """The launch of an M x N x K call."""
+    if m <= 16:
+        return BlockConfig("gemv_block", 16, 16, 1, 8, 1)
+    return BlockConfig("gemv_block", 64, 16, 1, 4, 1)

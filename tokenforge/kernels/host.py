@@ -224,3 +224,51 @@ def rmsnorm_fp8_quant_dequant(x: torch.Tensor, weight: torch.Tensor, eps: float,
     """:func:`rmsnorm_fp8_quant` plus ``(q.to(float32) * scale).to(float16)``."""
     q, s = rmsnorm_fp8_quant(x, weight, eps, scale)
     return q, s, (q.to(torch.float32) * s).to(torch.float16)
+
+
+# ----------------------------------------------------------------------------- FP8 with a scale per 128
+
+BLOCK = 128
+
+
+def block_quant(y: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 codes and scales of fp32 ``y [T, K]``: ``scale = max(amax / 448, 1 / (448 * 512))`` over each
+    128 of a row (``group_size`` 128, the last block shorter where 128 does not divide K) or over the
+    row (0)."""
+    t, k = y.shape
+    g = group_size or k
+    nb = -(-k // g)
+    parts = torch.nn.functional.pad(y, (0, nb * g - k)).reshape(t, nb, g)
+    s = (parts.abs().amax(dim=-1) / FP8_E4M3_MAX).clamp(min=MIN_SCALE)
+    q = (parts / s[..., None]).clamp(-FP8_E4M3_MAX, FP8_E4M3_MAX).reshape(t, nb * g)[:, :k]
+    return q.to(torch.float8_e4m3fn).contiguous(), s
+
+
+def silu_mul_block_quant(x: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`block_quant` of ``silu(x[:, :K]) * x[:, K:]`` in fp32."""
+    xf = x.to(torch.float32)
+    gate, up = xf.chunk(2, dim=-1)
+    return block_quant(torch.nn.functional.silu(gate) * up, group_size)
+
+
+def add_rmsnorm_block_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float,
+                            group_size: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``hidden = x + residual`` in x's type and :func:`block_quant` of its RMSNorm in fp32; ``hidden`` is
+    empty without a residual."""
+    hidden = x if residual is None else x + residual
+    h = hidden.to(torch.float32)
+    y = h * torch.rsqrt(h.pow(2).mean(dim=-1, keepdim=True) + eps) * weight.to(torch.float32)
+    q, s = block_quant(y, group_size)
+    return q, s, x.new_empty((0,)) if residual is None else hidden
+
+
+def block_linear(x8: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_scale: torch.Tensor,
+                 bias: torch.Tensor | None, out_dtype: torch.dtype, residual: torch.Tensor | None) -> torch.Tensor:
+    """The dequantized product in fp32, bias and residual added in fp32, one rounding to ``out_dtype``."""
+    n, k = weight.shape
+    xs = x_scale.repeat_interleave(BLOCK, dim=1)[:, :k]
+    ws = w_scale.repeat_interleave(BLOCK, dim=0)[:n].repeat_interleave(BLOCK, dim=1)[:, :k]
+    y = (x8.to(torch.float32) * xs) @ (weight.to(torch.float32) * ws).t()
+    for extra in (bias, residual):
+        y = y if extra is None else y + extra.to(torch.float32)
+    return y.to(out_dtype)

@@ -45,6 +45,18 @@ and the decode norm-then-linear in one launch (no counterpart either):
   from ``rmsnorm_fp8_quant_dequant(x, norm_weight, eps, None)``; one kernel where the bucket's
   config is the GEMV stream form (M <= 4), the two kernels otherwise; same bits either way.
 
+and FP8 with a scale per 128 (no counterparts): codes and scales of three producers, and the linear on
+such codes with e4m3 weights that have a scale per 128 x 128 block, as FP8 checkpoints hold them
+(``group_size`` 128, or 0 for the scale per row that ``w4a8_linear`` reads):
+
+* ``tokenforge::fp8_quant(x, group_size)`` = ``(q, scale)``
+* ``tokenforge::silu_mul_fp8_quant(x, group_size)`` = ``fp8_quant`` of ``silu(x[..., :K]) * x[..., K:]``
+* ``tokenforge::add_rmsnorm_fp8_quant(x, residual, weight, eps, group_size)`` = ``(q, scale, hidden)``,
+  ``fp8_quant`` of the RMSNorm of ``hidden = x + residual`` (``residual`` None: of x, ``hidden`` empty)
+* ``tokenforge::fp8_block_linear(x8, x_scale, weight, w_scale, bias, out_dtype, backend, epilogue,
+  residual)`` = ``x8 @ weight^T`` with the scales applied, plus bias, plus the residual (epilogue
+  ``"residual"``), in fp32 with one rounding to fp16 or bf16
+
 On GPU tensors every op runs the hand-written HIP kernels, and a missing kernel library (or
 a GPU other than gfx950) raises instead of falling back. Host (CPU) tensors take the
 reference's ``torch_reference`` route (ops.py:79-81): the torch expressions of
@@ -60,6 +72,7 @@ import functools
 import torch
 
 from tokenforge.kernels import _lib, autotune, dispatch, host
+from tokenforge.kernels.block_config import BLOCK, BlockConfig, block_config
 from tokenforge.kernels.config import (
     M_BUCKETS,
     MAX_BUCKET_M,
@@ -77,6 +90,7 @@ from tokenforge.kernels.config import (
     w4a8_gemv_config,
 )
 from tokenforge.kernels.device import SUPPORTED_ARCHS, device_arch, gpu_identity
+from tokenforge.kernels.hip import fp8_block as _block
 from tokenforge.kernels.hip import rmsnorm_fp8 as _rms
 from tokenforge.kernels.hip import w4a16 as _w4a16
 from tokenforge.kernels.metrics import KERNEL_CALLS
@@ -178,9 +192,21 @@ def _w4a8_config(cfg: GemmConfig, m: int, n: int, k: int, group_size: int) -> Ge
     return cfg
 
 
+def _block_family(cfg: BlockConfig) -> dispatch.Kernel:
+    return "hip_gemv" if cfg.kernel == "gemv_block" else "hip_gemm"
+
+
+def _block_decision(device: torch.device, m: int, n: int, k: int) -> BlockConfig:
+    """The launch config of a block-scaled linear (after the device check, as :func:`_gpu_config`)."""
+    runnable = device_arch(device) in SUPPORTED_ARCHS and _lib.available()
+    decision = dispatch.select(m, backend="hip", on_gpu=True, triton_ok=runnable, cuda_ext_available=_lib.available())
+    dispatch.require_gpu_decision(decision, on_gpu=True)
+    return block_config(m, n, k)
+
+
 # ----------------------------------------------------------------------------- the C++ side's hooks
 
-KIND_LINEAR, KIND_W4A8, KIND_NORM_LINEAR = 0, 1, 2
+KIND_LINEAR, KIND_W4A8, KIND_NORM_LINEAR, KIND_BLOCK = 0, 1, 2, 3
 _EPILOGUE_NAMES = {_lib.EPILOGUE_NONE: "none", _lib.EPILOGUE_RESIDUAL: "residual", _lib.EPILOGUE_SILU_MUL: "silu_mul"}
 _FAMILIES: tuple[dispatch.Kernel, ...] = ("hip_gemv", "hip_gemm")
 _BUCKET_LABELS = tuple(str(b) for b in M_BUCKETS) + (f">{MAX_BUCKET_M}",)
@@ -192,6 +218,12 @@ def _resolve_launch(kind: int, epilogue: int, m: int, n: int, k: int, group_size
     the config fields, the counter's family and bucket indices, the workspace bytes and, for
     the norm + linear, whether the GEMV's prologue runs the norm."""
     dev = torch.device("cuda", device)
+    if kind == KIND_BLOCK:
+        bcfg = _block_decision(dev, m, n, k)
+        c = _block.to_c_config(bcfg)
+        return [c.kernel, c.block_m, c.block_n, c.block_k, c.split_k, c.num_warps, c.num_stages,
+                _FAMILIES.index(_block_family(bcfg)), _BUCKET_LABELS.index(dispatch.bucket_label(m)),
+                _block.workspace_bytes(m, n, k, bcfg), 0]
     cfg = _gpu_config(dev, m, n, k, group_size)
     fused = 0
     h = _lib.lib()
@@ -453,6 +485,101 @@ def _rmsnorm_fp8_w4a16_linear_fake(x, norm_weight, eps, qweight_t, scales, qzero
     return x.new_empty((*x.shape[:-1], n // 2 if epilogue == "silu_mul" else n))
 
 
+# ----------------------------------------------------------------------------- FP8 with a scale per 128
+
+
+def _scale_shape(lead: torch.Size, k: int, group_size: int) -> tuple[int, ...]:
+    # (k + 127) // 128: with a symbolic k the fake traces this form
+    return (*lead, (k + BLOCK - 1) // BLOCK if group_size else 1)
+
+
+def _fp8_quant(x, group_size):  # type: ignore[no-untyped-def]
+    x2 = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.numel(), 0)
+    _, k = _block.check_quant_input(x2, group_size)
+    if _on_host("fp8_quant", x2):
+        q, s = host.block_quant(x2.to(torch.float32), group_size)
+    else:
+        q, s = _block.fp8_quant(x2, group_size)
+    return q.reshape(x.shape), s.reshape(_scale_shape(x.shape[:-1], k, group_size))
+
+
+def _silu_mul_fp8_quant(x, group_size):  # type: ignore[no-untyped-def]
+    x2 = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.numel(), 0)
+    _, k = _block.check_quant_input(x2, group_size, halves=2)
+    q, s = (host.silu_mul_block_quant if _on_host("silu_mul_fp8_quant", x2) else _block.silu_mul_fp8_quant)(
+        x2, group_size)
+    return q.reshape((*x.shape[:-1], k)), s.reshape(_scale_shape(x.shape[:-1], k, group_size))
+
+
+def _add_rmsnorm_fp8_quant(x, residual, weight, eps, group_size):  # type: ignore[no-untyped-def]
+    x2 = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.numel(), 0)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual shape {tuple(residual.shape)} != {tuple(x.shape)}")
+    r2 = None if residual is None else residual.reshape(x2.shape)
+    _, h = _block.check_norm_args(x2, r2, weight, group_size)
+    on_host = _on_host("add_rmsnorm_fp8_quant", x2, r2, weight)
+    q, s, hidden = (host.add_rmsnorm_block_quant if on_host else _block.add_rmsnorm_fp8_quant)(
+        x2, r2, weight, eps, group_size)
+    return (q.reshape(x.shape), s.reshape(_scale_shape(x.shape[:-1], h, group_size)),
+            hidden if residual is None else hidden.reshape(x.shape))
+
+
+def _fp8_block_linear(x8, x_scale, weight, w_scale, bias, out_dtype, backend, epilogue="none", residual=None):  # type: ignore[no-untyped-def]
+    """The block-scaled e4m3 linear with an optional epilogue ("none", "residual"); ``x8``/``x_scale`` as
+    the quantizers above return them with ``group_size`` 128."""
+    _check_backend(backend)
+    if epilogue not in ("none", "residual"):
+        raise ValueError(f"epilogue must be 'none' or 'residual', got {epilogue!r}")
+    if (epilogue == "residual") != (residual is not None):
+        raise ValueError("a residual goes with epilogue 'residual', and only with it")
+    if x8.dim() < 1 or weight.dim() != 2:
+        raise ValueError(f"x8 must be [..., K] and weight [N, K], got {tuple(x8.shape)} and {tuple(weight.shape)}")
+    k, n = x8.shape[-1], weight.shape[0]
+    out_shape = (*x8.shape[:-1], n)
+    if residual is not None and tuple(residual.shape) != out_shape:
+        raise ValueError(f"residual shape {tuple(residual.shape)} != {out_shape}")
+    if x_scale.shape[:-1] != x8.shape[:-1]:
+        raise ValueError(f"x_scale shape {tuple(x_scale.shape)} does not match x8 {tuple(x8.shape)}")
+    m = x8.numel() // k if k else 0
+    x2, s2 = x8.reshape(m, k), x_scale.reshape(m, x_scale.shape[-1])
+    r2 = None if residual is None else residual.reshape(m, n)
+    _block.check_block_linear(x2, s2, weight, w_scale, bias, out_dtype, r2)
+    on_host = _on_host("fp8_block_linear", x2, s2, weight, w_scale, bias, r2)
+    if m == 0 or n == 0:
+        return x8.new_empty(out_shape, dtype=out_dtype)
+    if on_host:
+        _record_host(m, backend)
+        return host.block_linear(x2, s2, weight, w_scale, bias, out_dtype, r2).reshape(out_shape)
+    cfg = _block_decision(x2.device, m, n, k)
+    dispatch.record(dispatch.Decision(_block_family(cfg), dispatch.bucket_label(m)))
+    return _block.fp8_block_gemm(x2, s2, weight, w_scale, cfg, bias, out_dtype, r2).reshape(out_shape)
+
+
+@torch.library.register_fake("tokenforge::fp8_quant")
+def _fp8_quant_fake(x, group_size):  # type: ignore[no-untyped-def]
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty(_scale_shape(x.shape[:-1], x.shape[-1], group_size), dtype=torch.float32))
+
+
+@torch.library.register_fake("tokenforge::silu_mul_fp8_quant")
+def _silu_mul_fp8_quant_fake(x, group_size):  # type: ignore[no-untyped-def]
+    k = x.shape[-1] // 2
+    return (x.new_empty((*x.shape[:-1], k), dtype=torch.float8_e4m3fn),
+            x.new_empty(_scale_shape(x.shape[:-1], k, group_size), dtype=torch.float32))
+
+
+@torch.library.register_fake("tokenforge::add_rmsnorm_fp8_quant")
+def _add_rmsnorm_fp8_quant_fake(x, residual, weight, eps, group_size):  # type: ignore[no-untyped-def]
+    q, s = _fp8_quant_fake(x, group_size)
+    return q, s, x.new_empty((0,) if residual is None else x.shape)
+
+
+@torch.library.register_fake("tokenforge::fp8_block_linear")
+def _fp8_block_linear_fake(x8, x_scale, weight, w_scale, bias, out_dtype, backend, epilogue="none",  # type: ignore[no-untyped-def]
+                           residual=None):
+    return x8.new_empty((*x8.shape[:-1], weight.shape[0]), dtype=out_dtype)
+
+
 # ----------------------------------------------------------------------------- registrations
 
 # Each operator's Python body: the CPU kernel (the torch route) and tokenforge::_py_<op>, which
@@ -466,6 +593,10 @@ _BODIES = {
     "rmsnorm_fp8_quant": _rmsnorm_fp8_quant,
     "rmsnorm_fp8_quant_dequant": _rmsnorm_fp8_quant_dequant,
     "rmsnorm_fp8_w4a16_linear": _rmsnorm_fp8_w4a16_linear,
+    "fp8_quant": _fp8_quant,
+    "silu_mul_fp8_quant": _silu_mul_fp8_quant,
+    "add_rmsnorm_fp8_quant": _add_rmsnorm_fp8_quant,
+    "fp8_block_linear": _fp8_block_linear,
 }
 for _name, _body in _BODIES.items():
     _schema = str(getattr(torch.ops.tokenforge, _name).default._schema)

@@ -46,6 +46,10 @@ struct Api {
   decltype(&tf_w4a8_linear_ex) w4a8 = nullptr;
   decltype(&tf_rmsnorm_fp8_quant_ex) norm = nullptr;
   decltype(&tf_rmsnorm_fp8_w4a16_linear) norm_linear = nullptr;
+  decltype(&tf_fp8_quant) quant = nullptr;
+  decltype(&tf_silu_mul_fp8_quant) silu_quant = nullptr;
+  decltype(&tf_add_rmsnorm_fp8_quant) add_norm = nullptr;
+  decltype(&tf_fp8_block_linear) block_linear = nullptr;
   decltype(&tf_last_error) last_error = nullptr;
 };
 
@@ -70,6 +74,10 @@ void bind_library(c10::string_view path) {
   bind_symbol(handle, "tf_w4a8_linear_ex", api.w4a8);
   bind_symbol(handle, "tf_rmsnorm_fp8_quant_ex", api.norm);
   bind_symbol(handle, "tf_rmsnorm_fp8_w4a16_linear", api.norm_linear);
+  bind_symbol(handle, "tf_fp8_quant", api.quant);
+  bind_symbol(handle, "tf_silu_mul_fp8_quant", api.silu_quant);
+  bind_symbol(handle, "tf_add_rmsnorm_fp8_quant", api.add_norm);
+  bind_symbol(handle, "tf_fp8_block_linear", api.block_linear);
   bind_symbol(handle, "tf_last_error", api.last_error);
   g_api = api;
   g_bound.store(true, std::memory_order_release);
@@ -92,7 +100,7 @@ void check(int rc, const char* what) {
 
 // ----------------------------------------------------------------------------- launch configs
 
-enum Kind : int64_t { kLinear = 0, kW4A8 = 1, kNormLinear = 2 };
+enum Kind : int64_t { kLinear = 0, kW4A8 = 1, kNormLinear = 2, kBlockLinear = 3 };
 
 struct Key {
   int64_t kind, epilogue, m, n, k, group, device;
@@ -246,6 +254,13 @@ using NormDqFn = std::tuple<at::Tensor, at::Tensor, at::Tensor>(const at::Tensor
 using NormLinearFn = at::Tensor(const at::Tensor&, const at::Tensor&, double, const at::Tensor&, const at::Tensor&,
                                 const at::Tensor&, const std::optional<at::Tensor>&, c10::SymInt, c10::string_view,
                                 c10::string_view);
+
+using QuantFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, c10::SymInt);
+using AddNormFn = std::tuple<at::Tensor, at::Tensor, at::Tensor>(const at::Tensor&, const std::optional<at::Tensor>&,
+                                                                 const at::Tensor&, double, c10::SymInt);
+using BlockLinearFn = at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                 const std::optional<at::Tensor>&, at::ScalarType, c10::string_view,
+                                 c10::string_view, const std::optional<at::Tensor>&);
 
 // ----------------------------------------------------------------------------- W4A16 linear
 
@@ -495,6 +510,167 @@ at::Tensor rmsnorm_fp8_w4a16_linear(const at::Tensor& x, const at::Tensor& nw, d
                                    group_size, backend, epilogue);
 }
 
+// ----------------------------------------------------------------------------- FP8 with a scale per 128
+
+constexpr int64_t kBlock = 128;
+
+// TF_DTYPE_* of a 16-bit tensor, -1 for another type.
+int32_t dtype_code(at::ScalarType t) {
+  return t == at::kHalf ? TF_DTYPE_FP16 : t == at::kBFloat16 ? TF_DTYPE_BF16 : -1;
+}
+
+// t as [rows, last] with contiguous rows that do not overlap; undefined where that needs a copy.
+at::Tensor plain_rows(const at::Tensor& t) {
+  const int64_t w = t.size(-1);
+  if (t.dim() < 1 || t.numel() == 0) return {};
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, w});
+  if (r.stride(1) != 1 || (r.size(0) > 1 && r.stride(0) < w)) return {};
+  return r;
+}
+
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// The outputs' options and [..., blocks] (or [..., 1]) shape of a quantizer's codes and scales.
+at::Tensor empty_codes(const at::Tensor& x, int64_t k) {
+  return at::empty(with_last(x.sizes().slice(0, x.dim() - 1), k), x.options().dtype(at::kFloat8_e4m3fn));
+}
+at::Tensor empty_scales(const at::Tensor& x, int64_t k, int64_t g) {
+  return at::empty(with_last(x.sizes().slice(0, x.dim() - 1), g ? (k + kBlock - 1) / kBlock : 1),
+                   x.options().dtype(at::kFloat));
+}
+
+// Whether a quantizer's input takes the fast path; rows out.
+bool quant_ok(const at::Tensor& x, int64_t g, bool whole_row, int64_t halves, at::Tensor& rows) {
+  if (x.dim() < 1 || !x.is_cuda() || dtype_code(x.scalar_type()) < 0 || (g != 0 && g != kBlock)) return false;
+  if (x.size(-1) % halves != 0 || ((whole_row || g == 0) && x.size(-1) / halves > TF_FP8_MAX_ROW)) return false;
+  rows = plain_rows(x);
+  return rows.defined();
+}
+
+std::tuple<at::Tensor, at::Tensor> quant_fast(decltype(&tf_fp8_quant) fn, const char* what, const at::Tensor& x,
+                                              int64_t g, int64_t halves) {
+  at::Tensor x2;
+  if (!quant_ok(x, g, false, halves, x2)) return {};
+  const int64_t k = x.size(-1) / halves;
+  const c10::Device dev = x.device();
+  c10::OptionalDeviceGuard guard(dev);
+  at::Tensor q = empty_codes(x, k), s = empty_scales(x, k, g);
+  check(fn(data<const uint16_t>(x2), row_stride(x2), dtype_code(x.scalar_type()), data<uint8_t>(q), data<float>(s),
+           x2.size(0), k, static_cast<int32_t>(g), c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        what);
+  return {q, s};
+}
+
+std::tuple<at::Tensor, at::Tensor> fp8_quant(const at::Tensor& x, c10::SymInt group_size) {
+  auto r = quant_fast(api().quant, "tf_fp8_quant", x, group_size.guard_int(__FILE__, __LINE__), 1);
+  if (std::get<0>(r).defined()) return r;
+  return python_body<QuantFn>("tokenforge::_py_fp8_quant", x, group_size);
+}
+
+std::tuple<at::Tensor, at::Tensor> silu_mul_fp8_quant(const at::Tensor& x, c10::SymInt group_size) {
+  auto r = quant_fast(api().silu_quant, "tf_silu_mul_fp8_quant", x, group_size.guard_int(__FILE__, __LINE__), 2);
+  if (std::get<0>(r).defined()) return r;
+  return python_body<QuantFn>("tokenforge::_py_silu_mul_fp8_quant", x, group_size);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_norm_fast(const at::Tensor& x,
+                                                             const std::optional<at::Tensor>& residual,
+                                                             const at::Tensor& w, double eps, int64_t g) {
+  at::Tensor x2, r2;
+  if (!quant_ok(x, g, true, 1, x2)) return {};
+  const c10::Device dev = x.device();
+  const int64_t h = x.size(-1);
+  if (w.dim() != 1 || w.size(0) != h || w.scalar_type() != x.scalar_type() || !w.is_contiguous() || !on(w, dev))
+    return {};
+  if (residual.has_value()) {
+    if (residual->scalar_type() != x.scalar_type() || !on(*residual, dev) || residual->sizes() != x.sizes()) return {};
+    r2 = plain_rows(*residual);
+    if (!r2.defined()) return {};
+  }
+  c10::OptionalDeviceGuard guard(dev);
+  at::Tensor q = empty_codes(x, h), s = empty_scales(x, h, g);
+  at::Tensor hidden = r2.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  check(api().add_norm(data<const uint16_t>(x2), row_stride(x2), r2.defined() ? data<const uint16_t>(r2) : nullptr,
+                       r2.defined() ? row_stride(r2) : 0, data<const uint16_t>(w), dtype_code(x.scalar_type()),
+                       data<uint8_t>(q), data<float>(s), r2.defined() ? data<uint16_t>(hidden) : nullptr, x2.size(0),
+                       h, static_cast<float>(eps), static_cast<int32_t>(g),
+                       c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        "tf_add_rmsnorm_fp8_quant");
+  return {q, s, hidden};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_fp8_quant(const at::Tensor& x,
+                                                                     const std::optional<at::Tensor>& residual,
+                                                                     const at::Tensor& w, double eps,
+                                                                     c10::SymInt group_size) {
+  auto r = add_norm_fast(x, residual, w, eps, group_size.guard_int(__FILE__, __LINE__));
+  if (std::get<0>(r).defined()) return r;
+  return python_body<AddNormFn>("tokenforge::_py_add_rmsnorm_fp8_quant", x, residual, w, eps, group_size);
+}
+
+// Code rows as the kernels read them: 16-byte aligned.
+bool code_rows_ok(const at::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_stride(t) % 16 == 0;
+}
+
+at::Tensor block_linear_fast(const at::Tensor& x8, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
+                             const std::optional<at::Tensor>& bias, at::ScalarType out_dtype,
+                             c10::string_view backend, c10::string_view epilogue,
+                             const std::optional<at::Tensor>& residual) {
+  const int32_t dtype = dtype_code(out_dtype);
+  if (dtype < 0 || !backend_ok(backend) || x8.dim() < 1 || w.dim() != 2 || ws.dim() != 2 || !x8.is_cuda()) return {};
+  if (epilogue != (residual.has_value() ? "residual" : "none")) return {};
+  const c10::Device dev = x8.device();
+  const int64_t k = x8.size(-1), n = w.size(0), nkb = (k + kBlock - 1) / kBlock;
+  if (x8.scalar_type() != at::kFloat8_e4m3fn || w.scalar_type() != at::kFloat8_e4m3fn || w.size(1) != k || k % 16 != 0)
+    return {};
+  if (xs.scalar_type() != at::kFloat || ws.scalar_type() != at::kFloat || !on(xs, dev) || !on(w, dev) || !on(ws, dev))
+    return {};
+  const auto lead = x8.sizes().slice(0, x8.dim() - 1);
+  if (xs.sizes() != at::IntArrayRef(with_last(lead, nkb)) || ws.size(0) != (n + kBlock - 1) / kBlock ||
+      ws.size(1) != nkb)
+    return {};
+  const at::Tensor x2 = plain_rows(x8), s2 = plain_rows(xs), w2 = plain_rows(w), ws2 = plain_rows(ws);
+  if (!x2.defined() || !s2.defined() || !w2.defined() || !ws2.defined() || !code_rows_ok(x2) || !code_rows_ok(w2))
+    return {};
+  if (bias.has_value() && (bias->dim() != 1 || bias->size(0) != n || bias->scalar_type() != out_dtype ||
+                           !bias->is_contiguous() || !on(*bias, dev)))
+    return {};
+  const std::vector<int64_t> out_shape = with_last(lead, n);
+  at::Tensor r2;
+  if (residual.has_value()) {
+    if (residual->scalar_type() != out_dtype || !on(*residual, dev) || residual->sizes() != at::IntArrayRef(out_shape))
+      return {};
+    r2 = plain_rows(*residual);
+    if (!r2.defined()) return {};
+  }
+  const int64_t m = x2.size(0);
+  const Launch l = resolve(Key{kBlockLinear, TF_EPILOGUE_NONE, m, n, k, kBlock, dev.index()});
+  count(l);
+  c10::OptionalDeviceGuard guard(dev);
+  at::Tensor out = at::empty(out_shape, x8.options().dtype(out_dtype));
+  at::Tensor work;
+  if (l.need > 0) work = at::empty({(l.need + 3) / 4}, x8.options().dtype(at::kFloat));
+  check(api().block_linear(data<const uint8_t>(x2), row_stride(x2), data<const float>(s2), row_stride(s2),
+                           data<const uint8_t>(w2), row_stride(w2), data<const float>(ws2), row_stride(ws2),
+                           static_cast<const uint16_t*>(ptr_or_null(bias)),
+                           r2.defined() ? data<const uint16_t>(r2) : nullptr, r2.defined() ? row_stride(r2) : 0,
+                           data<uint16_t>(out), n, dtype, m, n, k, &l.cfg, work.defined() ? data<float>(work) : nullptr,
+                           l.need, c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        "tf_fp8_block_linear");
+  return out;
+}
+
+at::Tensor fp8_block_linear(const at::Tensor& x8, const at::Tensor& x_scale, const at::Tensor& weight,
+                            const at::Tensor& w_scale, const std::optional<at::Tensor>& bias,
+                            at::ScalarType out_dtype, c10::string_view backend, c10::string_view epilogue,
+                            const std::optional<at::Tensor>& residual) {
+  at::Tensor y = block_linear_fast(x8, x_scale, weight, w_scale, bias, out_dtype, backend, epilogue, residual);
+  if (y.defined()) return y;
+  return python_body<BlockLinearFn>("tokenforge::_py_fp8_block_linear", x8, x_scale, weight, w_scale, bias, out_dtype,
+                                    backend, epilogue, residual);
+}
+
 }  // namespace
 
 // Schemas: the reference's three ops (ops.py:48-156) and this build's fused forms, with the
@@ -514,6 +690,12 @@ TORCH_LIBRARY(tokenforge, m) {
   m.def("rmsnorm_fp8_quant_dequant(Tensor x, Tensor weight, float eps, Tensor? scale) -> (Tensor, Tensor, Tensor)");
   m.def("rmsnorm_fp8_w4a16_linear(Tensor x, Tensor norm_weight, float eps, Tensor qweight_t, Tensor scales, "
         "Tensor qzeros, Tensor? bias, SymInt group_size, str backend, str epilogue) -> Tensor");
+  m.def("fp8_quant(Tensor x, SymInt group_size) -> (Tensor, Tensor)");
+  m.def("silu_mul_fp8_quant(Tensor x, SymInt group_size) -> (Tensor, Tensor)");
+  m.def("add_rmsnorm_fp8_quant(Tensor x, Tensor? residual, Tensor weight, float eps, SymInt group_size) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("fp8_block_linear(Tensor x8, Tensor x_scale, Tensor weight, Tensor w_scale, Tensor? bias, "
+        "ScalarType out_dtype, str backend, str epilogue=\"none\", Tensor? residual=None) -> Tensor");
   m.def("_bind_library(str path) -> ()");
   m.def("_native_calls() -> int[]");
   m.def("_clear_launch_cache() -> ()");
@@ -528,6 +710,10 @@ TORCH_LIBRARY_IMPL(tokenforge, CUDA, m) {
   m.impl("rmsnorm_fp8_quant", &rmsnorm_fp8_quant);
   m.impl("rmsnorm_fp8_quant_dequant", &rmsnorm_fp8_quant_dequant);
   m.impl("rmsnorm_fp8_w4a16_linear", &rmsnorm_fp8_w4a16_linear);
+  m.impl("fp8_quant", &fp8_quant);
+  m.impl("silu_mul_fp8_quant", &silu_mul_fp8_quant);
+  m.impl("add_rmsnorm_fp8_quant", &add_rmsnorm_fp8_quant);
+  m.impl("fp8_block_linear", &fp8_block_linear);
 }
 
 TORCH_LIBRARY_IMPL(tokenforge, CompositeExplicitAutograd, m) {
