@@ -24,7 +24,7 @@ TF_ELAUNCH = 2
 TF_ERANGE = 3
 
 KERNEL_IDS = {"gemv_dot": 0, "gemv_mfma": 1, "gemm_mfma": 2, "gemm_fp8": 3}
-BLOCK_KERNEL_IDS = {"gemv_block": 4}
+BLOCK_KERNEL_IDS = {"gemv_block": 4, "gemm_block": 5}
 """Kernel families of ``tf_fp8_block_linear`` (TF_KERNEL_FP8_BLOCK_*)."""
 FP8_MAX_ROW = 32768
 """TF_FP8_MAX_ROW: longest row the FP8 quantizers reduce as a whole."""

@@ -15,7 +15,8 @@ BLOCK = 128
 @dataclass(frozen=True)
 class BlockConfig:
     """One launch: ``gemv_block`` (block_m rows x 16 columns per workgroup, ``num_warps`` waves share
-    K)."""
+    K), or ``gemm_block`` (block_m x block_n tiles, ``num_stages`` LDS stages, K in ``split_k`` slices that a
+    second kernel adds)."""
 
     kernel: str
     block_m: int
@@ -27,6 +28,9 @@ class BlockConfig:
 
 BLOCK_TILES: tuple[tuple[str, int, int, int, int], ...] = (
     ("gemv_block", 16, 16, 8, 1), ("gemv_block", 64, 16, 4, 1),
+    ("gemm_block", 256, 256, 8, 2), ("gemm_block", 256, 128, 8, 3), ("gemm_block", 128, 256, 8, 3),
+    ("gemm_block", 128, 128, 4, 2), ("gemm_block", 128, 128, 8, 4), ("gemm_block", 64, 128, 8, 3),
+    ("gemm_block", 64, 64, 4, 4),
 )
 """(kernel, block_m, block_n, num_warps, num_stages) of every compiled kernel."""
 
@@ -35,4 +39,8 @@ def block_config(m: int, n: int, k: int) -> BlockConfig:
     """The launch of an M x N x K call."""
     if m <= 16:
         return BlockConfig("gemv_block", 16, 16, 1, 8, 1)
-    return BlockConfig("gemv_block", 64, 16, 1, 4, 1)
+    nkb = -(-k // BLOCK)
+    bm, bn, warps, stages = (64, 128, 8, 3) if m <= 64 else (128, 128, 8, 4) if m <= 512 else (256, 256, 8, 2)
+    tiles = -(-m // bm) * -(-n // bn)
+    split = max(1, min(256 // tiles, nkb // 4, 8))
+    return BlockConfig("gemm_block", bm, bn, split, warps, stages)

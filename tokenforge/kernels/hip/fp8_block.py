@@ -18,6 +18,8 @@ from tokenforge.kernels.hip._common import on_device, ptr, require_gpu, stream_o
 
 DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # TF_DTYPE_* of the C header
 GROUP_SIZES = (BLOCK, 0)
+MAX_CODE_STRIDE = 1 << 22  # rows of codes start less than 4 MiB apart, rows of x_scale less than 2^20 elements:
+MAX_SCALE_STRIDE = 1 << 20  # a tile's offsets stay in 31 bits (rows further apart are copied)
 
 
 def blocks(size: int) -> int:
@@ -68,9 +70,12 @@ def _outputs(t: int, k: int, group_size: int, dev: torch.device) -> tuple[torch.
     return q, torch.empty((t, blocks(k) if group_size else 1), dtype=torch.float32, device=dev)
 
 
-def rows(x: torch.Tensor) -> torch.Tensor:
-    """A 2-D tensor whose rows are contiguous and do not overlap; a copy only when needed."""
-    return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+def rows(x: torch.Tensor, limit: int = 1 << 62) -> torch.Tensor:
+    """A 2-D tensor whose rows are contiguous, do not overlap and start less than ``limit`` elements apart;
+    a copy only when needed."""
+    if x.stride(1) == 1 and (x.shape[0] <= 1 or x.shape[1] <= x.stride(0) < limit):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _row_stride(x: torch.Tensor) -> int:
@@ -152,8 +157,8 @@ def check_block_linear(
     n = weight.shape[0]
     if weight.shape[1] != k:
         raise ValueError(f"weight shape {tuple(weight.shape)} does not match K={k}")
-    if k == 0 or k % 16:
-        raise ValueError(f"K must be a multiple of 16, got {k}")
+    if k == 0 or k % 16 or k >= MAX_CODE_STRIDE:
+        raise ValueError(f"K must be a multiple of 16 below {MAX_CODE_STRIDE}, got {k}")
     if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
         raise TypeError(f"x_scale and w_scale must be fp32, got {x_scale.dtype} and {w_scale.dtype}")
     if tuple(x_scale.shape) != (m, blocks(k)):
@@ -175,7 +180,7 @@ def check_block_linear(
 
 def _code_rows(t: torch.Tensor) -> torch.Tensor:
     """:func:`rows` that start on 16 bytes (the kernels use 128-bit loads)."""
-    t = rows(t)
+    t = rows(t, MAX_CODE_STRIDE)
     if t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) % 16 == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -211,7 +216,7 @@ def fp8_block_gemm(
     if m == 0 or n == 0:
         return out
     x8, weight = _code_rows(x8), _code_rows(weight)
-    x_scale, w_scale = rows(x_scale), rows(w_scale)
+    x_scale, w_scale = rows(x_scale, MAX_SCALE_STRIDE), rows(w_scale)
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else rows(residual)
     c = to_c_config(config)

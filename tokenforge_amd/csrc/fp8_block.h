@@ -81,6 +81,15 @@ __device__ __forceinline__ void store_block4(const BlockArgs& a, int m, int n, c
   }
 }
 
+// Row strides (bytes of codes, elements of scales) below which a tile's offsets stay in 31 bits.
+constexpr int64_t kMaxCodeStride = 1 << 22;
+constexpr int64_t kMaxScaleStride = 1 << 20;
+
+bool block_gemv_known(const tf_gemm_config& cfg);
 int launch_block_gemv(const BlockArgs& a, const tf_gemm_config& cfg, hipStream_t stream);
+
+bool block_gemm_known(const tf_gemm_config& cfg);
+int block_split(const tf_gemm_config& cfg, int64_t nkb);  // K slices that hold a block
+int launch_block_gemm(const BlockArgs& a, const tf_gemm_config& cfg, float* part, hipStream_t stream);
 
 }  // namespace tf

@@ -13,8 +13,10 @@ using namespace tf;
 
 extern "C" int64_t tf_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k, const tf_gemm_config* cfg) {
   if (!cfg || m < 0 || n < 0 || k < 0) return -1;
-  if (cfg->kernel == TF_KERNEL_FP8_BLOCK_GEMV) return 0;
-  return -1;
+  if (cfg->kernel == TF_KERNEL_FP8_BLOCK_GEMV) return block_gemv_known(*cfg) ? 0 : -1;
+  if (cfg->kernel != TF_KERNEL_FP8_BLOCK_GEMM || !block_gemm_known(*cfg)) return -1;
+  const int split = block_split(*cfg, cdiv(k, kBlockK));
+  return split > 1 ? split * m * n * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int tf_fp8_block_linear(const uint8_t* x8, int64_t ldx8, const float* xscale, int64_t ldxs,
@@ -33,15 +35,19 @@ extern "C" int tf_fp8_block_linear(const uint8_t* x8, int64_t ldx8, const float*
     return bad("row stride smaller than the row");
   if (ldx8 % 16 || ldw % 16 || !multiple(x8, 16) || !multiple(weight, 16))
     return bad("rows of x8 and weight must be 16-byte aligned");
+  if (ldx8 >= kMaxCodeStride || ldw >= kMaxCodeStride || ldxs >= kMaxScaleStride)
+    return bad("rows further apart than 4 MiB (codes) or 2^20 elements (scales)");
   const int64_t need = tf_fp8_block_workspace_bytes(m, n, k, cfg);
   if (need < 0) return bad("not a compiled config");
   if (need > 0 && (!workspace || workspace_bytes < need))
     return bad("workspace too small (" + std::to_string(workspace_bytes) + " < " + std::to_string(need) + ")");
+  if (need > 0 && !multiple(workspace, 16)) return bad("workspace not 16-byte aligned");
   if (m == 0 || n == 0) return TF_OK;
   BlockArgs a{};
   a.x8 = x8, a.ldx = ldx8, a.xs = xscale, a.ldxs = ldxs;
   a.w = weight, a.ldw = ldw, a.ws = wscale, a.ldws = ldws;
   a.bias = bias, a.residual = residual, a.ldr = ldr, a.out = out, a.ldo = ldo;
   a.m = (int)m, a.n = (int)n, a.k = (int)k, a.nkb = (int)nkb, a.bf16 = dtype == TF_DTYPE_BF16;
-  return launch_block_gemv(a, *cfg, (hipStream_t)stream);
+  if (cfg->kernel == TF_KERNEL_FP8_BLOCK_GEMV) return launch_block_gemv(a, *cfg, (hipStream_t)stream);
+  return launch_block_gemm(a, *cfg, workspace, (hipStream_t)stream);
 }

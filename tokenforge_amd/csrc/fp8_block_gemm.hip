@@ -1,0 +1,302 @@
+// Block-scaled e4m3 linear, many rows: BM x BN tiles through LDS.
+//
+// A workgroup of WM x WN waves streams 128-wide K blocks of x and the weight, and the rows' scales of
+// the block, into S LDS stages by buffer->LDS loads issued S - 1 blocks ahead, one barrier a block.
+// A wave computes a (16 TM) x (16 TN) sub-tile: per block one v_mfma_scale_f32_16x16x128_f8f6f4
+// (unit MFMA scales) per 16 x 16 from a zero accumulator, then acc += (xs[m] * ws) * that in fp32.
+// The weight fragment is the first operand: lane l holds row l % 16 and columns 4 (l / 16) + q, so a
+// lane's four results share one scale, and the wave's columns lie in one 128-wide scale block.
+//
+// LDS rows are 128 bytes, 16-byte chunk c of row r in slot c ^ s(r), s(r) = 2 (r % 4) ^ ((r / 4) % 2):
+// with lane l at row l % 16 and chunks 2 (l / 16) + {0, 1} the reads are free of bank conflicts.
+#include "fp8_block.h"
+
+namespace tf {
+namespace {
+
+__device__ __forceinline__ int slot_xor(int row) { return ((row & 3) << 1) ^ ((row >> 2) & 1); }
+
+template <int BM, int BN, int WM, int WN, int S>
+struct Tile {
+  static constexpr int kWaves = WM * WN;
+  static constexpr int TM = BM / WM / 16;
+  static constexpr int TN = BN / WN / 16;
+  static constexpr int kXBytes = BM * kBlockK;
+  static constexpr int kWBytes = BN * kBlockK;
+  static constexpr int kScales = BM < 64 * WM * WN ? BM : 64 * WM * WN;
+  static constexpr int kStage = kXBytes + kWBytes;
+  static constexpr int kLds = S * (kStage + BM * 4);
+  static constexpr int kXLoads = BM / 8 / kWaves;  // 1 KB loads per wave and stage
+  static constexpr int kWLoads = BN / 8 / kWaves;
+  static constexpr int kLoads = kXLoads + kWLoads + 1;
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "a stage splits evenly over the waves");
+  static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "wave tile");
+  static_assert(128 % (16 * TN) == 0, "a wave's columns lie in one scale block");
+  static_assert(BM % 64 == 0 && BM <= 64 * kWaves, "one row-scale load per wave");
+  static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0x0 << 8) | ((N >> 4) << 14));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// 64 lanes x 16 bytes to the 1 KB at base + 1024 j, lane l's at 16 l.
+__device__ __forceinline__ void load16(__amdgpu_buffer_rsrc_t r, uint8_t* base, int j, uint32_t off, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(base + j * 1024), 16, off, soff, 0, 0);
+}
+
+template <int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, float* __restrict__ part, int split_k,
+                                                                  int tiles_m, int tiles_n) {
+  using C = Tile<BM, BN, WM, WN, S>;
+  constexpr int TM = C::TM, TN = C::TN;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  float* const s_lds = reinterpret_cast<float*>(smem + S * C::kStage);
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // Tiles in bands of 8 tile rows, the rows of a band innermost: the 32 tiles an XCD has in flight
+  // then read about 8 + 4 panels.
+  const int t = xcd_tile(blockIdx.x, gridDim.x);
+  const int plane = tiles_m * tiles_n;
+  const int z = t / plane;
+  const int r0 = t - z * plane;
+  const int band = r0 / (8 * tiles_n);
+  const int in_band = r0 - band * 8 * tiles_n;
+  const int rows = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+  const int m0 = (band * 8 + in_band % rows) * BM;
+  const int n0 = (in_band / rows) * BN;
+
+  const int kb0 = (int)(((int64_t)z * a.nkb) / split_k);
+  const int kb1 = (int)(((int64_t)(z + 1) * a.nkb) / split_k);
+
+  const int mrows = a.m - m0 < BM ? a.m - m0 : BM;
+  const int ncols = a.n - n0 < BN ? a.n - n0 : BN;
+  const uint8_t* const xp = a.x8 + (int64_t)m0 * a.ldx;
+  const uint8_t* const wp = a.w + (int64_t)n0 * a.ldw;
+  const float* const sp = a.xs + (int64_t)m0 * a.ldxs;
+  const uint32_t x_bytes = (uint32_t)((mrows - 1) * (int)a.ldx + a.k);
+  const uint32_t w_bytes = (uint32_t)((ncols - 1) * (int)a.ldw + a.k);
+  const uint32_t s_bytes = (uint32_t)((mrows - 1) * (int)a.ldxs + a.nkb) * 4u;
+
+  // Load i of a wave fills 64 consecutive 16-byte slots: slot 64 j + lane of a stage's x (then w).
+  uint32_t x_off[C::kXLoads], w_off[C::kWLoads];
+  int x_c[C::kXLoads], w_c[C::kWLoads];
+#pragma unroll
+  for (int i = 0; i < C::kXLoads; ++i) {
+    const int p = (wave + C::kWaves * i) * 64 + lane, row = p >> 3;
+    x_c[i] = ((p & 7) ^ slot_xor(row)) * 16;
+    x_off[i] = row < mrows ? (uint32_t)(row * (int)a.ldx + x_c[i]) : kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < C::kWLoads; ++i) {
+    const int p = (wave + C::kWaves * i) * 64 + lane, row = p >> 3;
+    w_c[i] = ((p & 7) ^ slot_xor(row)) * 16;
+    w_off[i] = row < ncols ? (uint32_t)(row * (int)a.ldw + w_c[i]) : kOutOfRange;
+  }
+  const int s_row0 = (wave % (BM / 64)) * 64;  // waves past BM / 64 load the same rows again
+  const uint32_t s_off = s_row0 + lane < mrows ? (uint32_t)((s_row0 + lane) * (int)a.ldxs) * 4u : kOutOfRange;
+
+  auto issue = [&](int kb, int st) __attribute__((always_inline)) {
+    // A block past the slice is loaded through empty resources: zeros, without touching memory.
+    const bool ok = kb < kb1;
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(xp, ok ? x_bytes : 0u);
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, ok ? w_bytes : 0u);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(sp, ok ? s_bytes : 0u);
+    const int sk = ok ? kb : 0;
+    const int left = a.k - sk * kBlockK;
+    uint8_t* const base = smem + st * C::kStage;
+    if (left >= kBlockK) {
+#pragma unroll
+      for (int i = 0; i < C::kXLoads; ++i) load16(rx, base, wave + C::kWaves * i, x_off[i], sk * kBlockK);
+#pragma unroll
+      for (int i = 0; i < C::kWLoads; ++i) load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_off[i], sk * kBlockK);
+    } else {  // the last block ends inside its 128: chunks past K are zeros on both sides
+#pragma unroll
+      for (int i = 0; i < C::kXLoads; ++i)
+        load16(rx, base, wave + C::kWaves * i, x_c[i] < left ? x_off[i] : kOutOfRange, sk * kBlockK);
+#pragma unroll
+      for (int i = 0; i < C::kWLoads; ++i)
+        load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_c[i] < left ? w_off[i] : kOutOfRange, sk * kBlockK);
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(s_lds + st * BM + s_row0), 4, s_off, sk * 4, 0, 0);
+  };
+
+  f4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int c16 = lane & 15;
+  const int kc = 2 * (lane >> 4);
+  const int x_row = wm * TM * 16 + c16, w_row = wn * TN * 16 + c16;
+  auto frag = [&](const uint8_t* base, int row) {
+    const uint32_t at = (uint32_t)(row * 8 + (kc ^ slot_xor(row))) * 16u;
+    const u4 lo = *reinterpret_cast<const u4*>(base + at), hi = *reinterpret_cast<const u4*>(base + (at ^ 16u));
+    return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+  // The wave's columns share one scale per block; columns past N are never stored.
+  int nb = (n0 + wn * TN * 16) >> 7;
+  nb = nb <= ((a.n - 1) >> 7) ? nb : (a.n - 1) >> 7;
+  const float* const wsp = a.ws + (int64_t)nb * a.ldws;
+
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue(kb0 + i, i);
+  float ws_next = kb0 < kb1 ? wsp[kb0] : 0.0f;
+
+  int st = 0;
+  for (int kb = kb0; kb < kb1; ++kb) {
+    stage_barrier<(S - 2) * C::kLoads>();
+    issue(kb + S - 1, st == 0 ? S - 1 : st - 1);
+    const float ws = ws_next;
+    ws_next = wsp[kb + 1 < kb1 ? kb + 1 : kb];
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* const X = smem + st * C::kStage;
+    const uint8_t* const W = X + C::kXBytes;
+    const float* const xs = s_lds + st * BM;
+    v8i bf[TN], af[2];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) bf[j] = frag(W, w_row + 16 * j);
+    af[0] = frag(X, x_row);
+    float sc[2];
+    sc[0] = xs[x_row] * ws;
+    f4 d[2][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      if (i + 1 < TM) af[(i + 1) & 1] = frag(X, x_row + 16 * (i + 1));
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af[i & 1], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0,
+                                                                       0, 0, kUnitScale, 0, kUnitScale);
+      __builtin_amdgcn_s_setprio(0);
+      if (i > 0) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            acc[i - 1][j][q] = __builtin_fmaf(sc[(i - 1) & 1], d[(i - 1) & 1][j][q], acc[i - 1][j][q]);
+      }
+      if (i + 1 < TM) sc[(i + 1) & 1] = xs[x_row + 16 * (i + 1)] * ws;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        acc[TM - 1][j][q] = __builtin_fmaf(sc[(TM - 1) & 1], d[(TM - 1) & 1][j][q], acc[TM - 1][j][q]);
+    st = st + 1 == S ? 0 : st + 1;
+  }
+
+  __builtin_amdgcn_s_waitcnt((0 & 0xF) | (0x7 << 4) | (0xF << 8));  // the last (empty) loads into LDS have ended
+  const int g4 = 4 * (lane >> 4);
+  const bool vec = split_k > 1 ? (a.n & 3) == 0 : runs_aligned(a);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int m = m0 + x_row + 16 * i;
+    if (m >= a.m) continue;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + wn * TN * 16 + 16 * j + g4;
+      if (n >= a.n) continue;
+      if (split_k > 1) {
+        float* const p = part + ((int64_t)z * a.m + m) * a.n + n;
+        if (vec) {
+          *reinterpret_cast<f4*>(p) = acc[i][j];
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (n + q < a.n) p[q] = acc[i][j][q];
+        }
+      } else {
+        store_block4(a, m, n, acc[i][j], vec);
+      }
+    }
+  }
+}
+
+// Sum of the K slices in slice order, then the epilogue; four columns a thread.
+__global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs a, const float* __restrict__ part, int split_k,
+                                                           int runs) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = i / runs;
+  if (m >= a.m) return;
+  const int n = (int)(i - m * runs) * 4;
+  const int64_t plane = (int64_t)a.m * a.n;
+  const float* const p = part + m * a.n + n;
+  f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  if ((a.n & 3) == 0) {
+    for (int z = 0; z < split_k; ++z) {
+      const f4 v = *reinterpret_cast<const f4*>(p + z * plane);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum[q] += v[q];
+    }
+  } else {
+    for (int z = 0; z < split_k; ++z)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < a.n) sum[q] += p[z * plane + q];
+  }
+  store_block4(a, (int)m, n, sum, runs_aligned(a));
+}
+
+template <int BM, int BN, int WM, int WN, int S>
+int launch(const BlockArgs& a, int split, float* part, hipStream_t stream) {
+  using C = Tile<BM, BN, WM, WN, S>;
+  const int tiles_m = (int)cdiv(a.m, BM), tiles_n = (int)cdiv(a.n, BN);
+  const int64_t grid = (int64_t)tiles_m * tiles_n * split;
+  if (grid > 0x7FFFFFFF) return fail(TF_EINVAL, "tf_fp8_block_linear: too many tiles");
+  auto kernel = block_gemm_kernel<BM, BN, WM, WN, S>;
+  if (C::kLds > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          C::kLds) != hipSuccess)
+    return fail(TF_ELAUNCH, "tf_fp8_block_linear: cannot reserve LDS");
+  kernel<<<(unsigned)grid, 64 * C::kWaves, C::kLds, stream>>>(a, part, split, tiles_m, tiles_n);
+  if (int rc = check_launch("tf_fp8_block_linear(gemm)")) return rc;
+  if (split == 1) return TF_OK;
+  const int runs = (int)cdiv(a.n, 4);
+  const int64_t groups = cdiv((int64_t)a.m * runs, 256);
+  block_reduce_kernel<<<(unsigned)groups, 256, 0, stream>>>(a, part, split, runs);
+  return check_launch("tf_fp8_block_linear(reduce)");
+}
+
+struct Entry {
+  int bm, bn, warps, stages;
+  int (*run)(const BlockArgs&, int, float*, hipStream_t);
+};
+
+#define TF_BLOCK(BM, BN, WM, WN, S) {BM, BN, WM * WN, S, launch<BM, BN, WM, WN, S>}
+const Entry kEntries[] = {
+    TF_BLOCK(256, 256, 2, 4, 2), TF_BLOCK(256, 128, 4, 2, 3), TF_BLOCK(128, 256, 2, 4, 3), TF_BLOCK(128, 128, 2, 2, 2),
+    TF_BLOCK(128, 128, 2, 4, 4), TF_BLOCK(64, 128, 2, 4, 3),  TF_BLOCK(64, 64, 2, 2, 4),
+};
+
+const Entry* find(const tf_gemm_config& cfg) {
+  for (const Entry& e : kEntries)
+    if (e.bm == cfg.block_m && e.bn == cfg.block_n && e.warps == cfg.num_warps && e.stages == cfg.num_stages) return &e;
+  return nullptr;
+}
+
+}  // namespace
+
+bool block_gemm_known(const tf_gemm_config& cfg) { return cfg.split_k >= 1 && find(cfg) != nullptr; }
+
+int block_split(const tf_gemm_config& cfg, int64_t nkb) {
+  return (int)(cfg.split_k < nkb ? cfg.split_k : (nkb > 0 ? nkb : 1));
+}
+
+int launch_block_gemm(const BlockArgs& a, const tf_gemm_config& cfg, float* part, hipStream_t stream) {
+  return find(cfg)->run(a, block_split(cfg, a.nkb), part, stream);
+}
+
+}  // namespace tf

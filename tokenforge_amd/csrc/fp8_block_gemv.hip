@@ -77,10 +77,12 @@ int launch(const BlockArgs& a, hipStream_t stream) {
 
 }  // namespace
 
+bool block_gemv_known(const tf_gemm_config& cfg) {
+  return (cfg.block_m == 16 && cfg.num_warps == 8) || (cfg.block_m == 64 && cfg.num_warps == 4);
+}
+
 int launch_block_gemv(const BlockArgs& a, const tf_gemm_config& cfg, hipStream_t stream) {
-  if (cfg.block_m == 16 && cfg.num_warps == 8) return launch<1, 8>(a, stream);
-  if (cfg.block_m == 64 && cfg.num_warps == 4) return launch<4, 4>(a, stream);
-  return fail(TF_EINVAL, "tf_fp8_block_linear: not a compiled gemv config");
+  return cfg.block_m == 16 ? launch<1, 8>(a, stream) : launch<4, 4>(a, stream);
 }
 
 }  // namespace tf

@@ -608,9 +608,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_fp8_quant(const at::T
   return python_body<AddNormFn>("tokenforge::_py_add_rmsnorm_fp8_quant", x, residual, w, eps, group_size);
 }
 
-// Code rows as the kernels read them: 16-byte aligned.
+// Code rows as the kernels read them: 16-byte aligned, less than 4 MiB apart.
 bool code_rows_ok(const at::Tensor& t) {
-  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_stride(t) % 16 == 0;
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_stride(t) % 16 == 0 && row_stride(t) < (1 << 22);
 }
 
 at::Tensor block_linear_fast(const at::Tensor& x8, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
@@ -631,7 +631,8 @@ at::Tensor block_linear_fast(const at::Tensor& x8, const at::Tensor& xs, const a
       ws.size(1) != nkb)
     return {};
   const at::Tensor x2 = plain_rows(x8), s2 = plain_rows(xs), w2 = plain_rows(w), ws2 = plain_rows(ws);
-  if (!x2.defined() || !s2.defined() || !w2.defined() || !ws2.defined() || !code_rows_ok(x2) || !code_rows_ok(w2))
+  if (!x2.defined() || !s2.defined() || !w2.defined() || !ws2.defined() || !code_rows_ok(x2) || !code_rows_ok(w2) ||
+      row_stride(s2) >= (1 << 20))
     return {};
   if (bias.has_value() && (bias->dim() != 1 || bias->size(0) != n || bias->scalar_type() != out_dtype ||
                            !bias->is_contiguous() || !on(*bias, dev)))
