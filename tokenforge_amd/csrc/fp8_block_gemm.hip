@@ -32,6 +32,7 @@ struct Tile {
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "a stage splits evenly over the waves");
   static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "wave tile");
   static_assert(128 % (16 * TN) == 0, "a wave's columns lie in one scale block");
+  static_assert(TM % 2 == 0, "the pipeline's two register sets alternate over whole blocks");
   static_assert(BM % 64 == 0 && BM <= 64 * kWaves, "one row-scale load per wave");
   static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -88,20 +89,19 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   const uint32_t w_bytes = (uint32_t)((ncols - 1) * (int)a.ldw + a.k);
   const uint32_t s_bytes = (uint32_t)((mrows - 1) * (int)a.ldxs + a.nkb) * 4u;
 
-  // Load i of a wave fills 64 consecutive 16-byte slots: slot 64 j + lane of a stage's x (then w).
+  // Load i of a wave fills 64 consecutive 16-byte slots: slot 64 (wave + waves i) + lane of a stage's x
+  // (then w), row (8 (wave + waves i) + lane / 8). A lane's chunk is the same in all of them.
   uint32_t x_off[C::kXLoads], w_off[C::kWLoads];
-  int x_c[C::kXLoads], w_c[C::kWLoads];
+  const int chunk = ((lane & 7) ^ slot_xor(lane >> 3)) * 16;
 #pragma unroll
   for (int i = 0; i < C::kXLoads; ++i) {
-    const int p = (wave + C::kWaves * i) * 64 + lane, row = p >> 3;
-    x_c[i] = ((p & 7) ^ slot_xor(row)) * 16;
-    x_off[i] = row < mrows ? (uint32_t)(row * (int)a.ldx + x_c[i]) : kOutOfRange;
+    const int row = (wave + C::kWaves * i) * 8 + (lane >> 3);
+    x_off[i] = row < mrows ? (uint32_t)(row * (int)a.ldx + chunk) : kOutOfRange;
   }
 #pragma unroll
   for (int i = 0; i < C::kWLoads; ++i) {
-    const int p = (wave + C::kWaves * i) * 64 + lane, row = p >> 3;
-    w_c[i] = ((p & 7) ^ slot_xor(row)) * 16;
-    w_off[i] = row < ncols ? (uint32_t)(row * (int)a.ldw + w_c[i]) : kOutOfRange;
+    const int row = (wave + C::kWaves * i) * 8 + (lane >> 3);
+    w_off[i] = row < ncols ? (uint32_t)(row * (int)a.ldw + chunk) : kOutOfRange;
   }
   const int s_row0 = (wave % (BM / 64)) * 64;  // waves past BM / 64 load the same rows again
   const uint32_t s_off = s_row0 + lane < mrows ? (uint32_t)((s_row0 + lane) * (int)a.ldxs) * 4u : kOutOfRange;
@@ -113,21 +113,19 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, ok ? w_bytes : 0u);
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(sp, ok ? s_bytes : 0u);
     const int sk = ok ? kb : 0;
-    const int left = a.k - sk * kBlockK;
     uint8_t* const base = smem + st * C::kStage;
-    if (left >= kBlockK) {
+    if (ok && a.k - kb * kBlockK <= chunk) {
+      // K ends inside this block, the last one: chunks past it are zeros on both sides, from here on
+      // (only empty blocks follow).
 #pragma unroll
-      for (int i = 0; i < C::kXLoads; ++i) load16(rx, base, wave + C::kWaves * i, x_off[i], sk * kBlockK);
+      for (int i = 0; i < C::kXLoads; ++i) x_off[i] = kOutOfRange;
 #pragma unroll
-      for (int i = 0; i < C::kWLoads; ++i) load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_off[i], sk * kBlockK);
-    } else {  // the last block ends inside its 128: chunks past K are zeros on both sides
-#pragma unroll
-      for (int i = 0; i < C::kXLoads; ++i)
-        load16(rx, base, wave + C::kWaves * i, x_c[i] < left ? x_off[i] : kOutOfRange, sk * kBlockK);
-#pragma unroll
-      for (int i = 0; i < C::kWLoads; ++i)
-        load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_c[i] < left ? w_off[i] : kOutOfRange, sk * kBlockK);
+      for (int i = 0; i < C::kWLoads; ++i) w_off[i] = kOutOfRange;
     }
+#pragma unroll
+    for (int i = 0; i < C::kXLoads; ++i) load16(rx, base, wave + C::kWaves * i, x_off[i], sk * kBlockK);
+#pragma unroll
+    for (int i = 0; i < C::kWLoads; ++i) load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_off[i], sk * kBlockK);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(s_lds + st * BM + s_row0), 4, s_off, sk * 4, 0, 0);
   };
 
@@ -137,66 +135,91 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // Fragment reads: rows 16 apart keep their slots, so a fragment is two chunks at a constant offset.
   const int c16 = lane & 15;
-  const int kc = 2 * (lane >> 4);
-  const int x_row = wm * TM * 16 + c16, w_row = wn * TN * 16 + c16;
-  auto frag = [&](const uint8_t* base, int row) {
-    const uint32_t at = (uint32_t)(row * 8 + (kc ^ slot_xor(row))) * 16u;
-    const u4 lo = *reinterpret_cast<const u4*>(base + at), hi = *reinterpret_cast<const u4*>(base + (at ^ 16u));
+  const int slot = (2 * (lane >> 4)) ^ slot_xor(c16);
+  const int x_row = wm * TM * 16 + c16;
+  const uint32_t x_at = (uint32_t)(x_row * 8 + slot) * 16u;
+  const uint32_t w_at = C::kXBytes + (uint32_t)((wn * TN * 16 + c16) * 8 + slot) * 16u;
+  auto frag = [&](const uint8_t* stage, uint32_t at, int i) {
+    const u4 lo = *reinterpret_cast<const u4*>(stage + at + i * 16 * kBlockK);
+    const u4 hi = *reinterpret_cast<const u4*>(stage + (at ^ 16u) + i * 16 * kBlockK);
     return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   };
-  // The wave's columns share one scale per block; columns past N are never stored.
+  // The wave's columns share one scale per block; lane l holds that of block kb0 + l of the current 64, read
+  // by lane number, as neither a scalar load (it shares the LDS reads' counter, and waiting for it
+  // waits for all of them) nor a vector load (it would wait for the stage loads) then stands in the loop.
+  // Columns past N are never stored.
   int nb = (n0 + wn * TN * 16) >> 7;
   nb = nb <= ((a.n - 1) >> 7) ? nb : (a.n - 1) >> 7;
   const float* const wsp = a.ws + (int64_t)nb * a.ldws;
+  auto load_ws = [&](int kb) { return wsp[kb + lane < kb1 ? kb + lane : kb1 - 1]; };
+  float ws64 = load_ws(kb0);
 
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i) issue(kb0 + i, i);
-  float ws_next = kb0 < kb1 ? wsp[kb0] : 0.0f;
-
+  for (int i = 0; i < S; ++i) issue(kb0 + i, i);
+  stage_barrier<(S - 1) * C::kLoads>();
+  // Software pipeline: the fragments of a step are read one step ahead, its results are scaled one
+  // step after its MFMAs, and the barrier to the next block stands before a block's last step: by
+  // then a wave has read all of its stage, so the stage is refilled and the next block's first
+  // fragments are read beside that step's MFMAs.
+  v8i bf[TN], af[2];
+  float xs[2], sc[2] = {0.0f, 0.0f};
+  f4 d[2][TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    bf[j] = frag(smem, w_at, j);
+    d[(TM - 1) & 1][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  af[0] = frag(smem, x_at, 0);
+  xs[0] = s_lds[x_row];
   int st = 0;
   for (int kb = kb0; kb < kb1; ++kb) {
-    stage_barrier<(S - 2) * C::kLoads>();
-    issue(kb + S - 1, st == 0 ? S - 1 : st - 1);
-    const float ws = ws_next;
-    ws_next = wsp[kb + 1 < kb1 ? kb + 1 : kb];
-    __builtin_amdgcn_sched_barrier(0);
-    const uint8_t* const X = smem + st * C::kStage;
-    const uint8_t* const W = X + C::kXBytes;
-    const float* const xs = s_lds + st * BM;
-    v8i bf[TN], af[2];
-#pragma unroll
-    for (int j = 0; j < TN; ++j) bf[j] = frag(W, w_row + 16 * j);
-    af[0] = frag(X, x_row);
-    float sc[2];
-    sc[0] = xs[x_row] * ws;
-    f4 d[2][TN];
+    const uint8_t* const stage = smem + st * C::kStage;
+    const float* const scales = s_lds + st * BM + x_row;
+    const int next = st + 1 == S ? 0 : st + 1;
+    const uint8_t* const stage2 = smem + next * C::kStage;
+    const int at = (kb - kb0) & 63;
+    if (at == 0 && kb > kb0) {
+      ws64 = load_ws(kb);
+      __asm__ volatile("" : "+v"(ws64));  // waits for it here, not at its uses
+    }
+    const float ws = as_f32((uint32_t)__builtin_amdgcn_readlane((int)as_u32(ws64), at));
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      if (i + 1 < TM) af[(i + 1) & 1] = frag(X, x_row + 16 * (i + 1));
-      __builtin_amdgcn_s_setprio(1);
+      if (i + 1 < TM) {
+        af[(i + 1) & 1] = frag(stage, x_at, i + 1);
+        xs[(i + 1) & 1] = scales[16 * (i + 1)];
+      } else {
+        stage_barrier<(S - 2) * C::kLoads>();
+        issue(kb + S, st);
+        __builtin_amdgcn_sched_barrier(0);
+        af[(i + 1) & 1] = frag(stage2, x_at, 0);
+        xs[(i + 1) & 1] = s_lds[next * BM + x_row];
+      }
+      sc[i & 1] = xs[i & 1] * ws;
+      constexpr int kLast = TM - 1;
+      const int p = i == 0 ? kLast : i - 1;  // the step whose results are scaled here
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < TN; ++j) {
         d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af[i & 1], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0,
                                                                        0, 0, kUnitScale, 0, kUnitScale);
-      __builtin_amdgcn_s_setprio(0);
-      if (i > 0) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            acc[i - 1][j][q] = __builtin_fmaf(sc[(i - 1) & 1], d[(i - 1) & 1][j][q], acc[i - 1][j][q]);
+        for (int q = 0; q < 4; ++q)
+          acc[p][j][q] = __builtin_fmaf(sc[(i + 1) & 1], d[(i + 1) & 1][j][q], acc[p][j][q]);
+        // Holds the MFMA and the scaling here: without a use in order they are moved to their results' uses.
+        __asm__ volatile("" : "+v"(d[i & 1][j]), "+v"(acc[p][j]));
+        if (i + 1 == TM) bf[j] = frag(stage2, w_at, j);  // in place, its last MFMA issued
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (i + 1 < TM) sc[(i + 1) & 1] = xs[x_row + 16 * (i + 1)] * ws;
-      __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        acc[TM - 1][j][q] = __builtin_fmaf(sc[(TM - 1) & 1], d[(TM - 1) & 1][j][q], acc[TM - 1][j][q]);
-    st = st + 1 == S ? 0 : st + 1;
+    st = next;
   }
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      acc[TM - 1][j][q] = __builtin_fmaf(sc[(TM - 1) & 1], d[(TM - 1) & 1][j][q], acc[TM - 1][j][q]);
 
   __builtin_amdgcn_s_waitcnt((0 & 0xF) | (0x7 << 4) | (0xF << 8));  // the last (empty) loads into LDS have ended
   const int g4 = 4 * (lane >> 4);
