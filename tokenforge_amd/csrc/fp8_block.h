@@ -81,6 +81,32 @@ __device__ __forceinline__ void store_block4(const BlockArgs& a, int m, int n, c
   }
 }
 
+// Whether runs of eight columns (8-aligned) of out (and residual) are one 16-byte access.
+__device__ __forceinline__ bool wide_rows(const BlockArgs& a) {
+  return (a.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
+         (a.residual == nullptr || ((a.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0));
+}
+
+// Columns n .. n + 7 of row m, as store_block4 (n % 8 == 0, N % 8 == 0 and wide_rows hold).
+__device__ __forceinline__ void store_block8(const BlockArgs& a, int m, int n, const f4& lo, const f4& hi) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < 4 ? lo[j & 3] : hi[j & 3];
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += from_16(a, a.bias[n + j]);
+  }
+  if (a.residual) {
+    const u4 r = *reinterpret_cast<const u4*>(a.residual + (int64_t)m * a.ldr + n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += from_16(a, (uint16_t)(r[j >> 1] >> (16 * (j & 1))));
+  }
+  u4 h;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = (uint32_t)to_16(a, v[2 * j]) | ((uint32_t)to_16(a, v[2 * j + 1]) << 16);
+  *reinterpret_cast<u4*>(a.out + (int64_t)m * a.ldo + n) = h;
+}
+
 // Row strides (bytes of codes, elements of scales) below which a tile's offsets stay in 31 bits.
 constexpr int64_t kMaxCodeStride = 1 << 22;
 constexpr int64_t kMaxScaleStride = 1 << 20;

@@ -23,17 +23,25 @@ struct Tile {
   static constexpr int TN = BN / WN / 16;
   static constexpr int kXBytes = BM * kBlockK;
   static constexpr int kWBytes = BN * kBlockK;
-  static constexpr int kScales = BM < 64 * WM * WN ? BM : 64 * WM * WN;
   static constexpr int kStage = kXBytes + kWBytes;
-  static constexpr int kLds = S * (kStage + BM * 4);
+  // Row scales: four K blocks of every row at a time, [BM][4] fp32, in a ring of its own. A wave's
+  // load brings 16 rows x 4 blocks, so a row's line is read once for four blocks.
+  static constexpr int kScaleRows = 16 * kWaves < BM ? 16 * kWaves : BM;  // rows the waves bring in one step
+  static constexpr int kScaleSteps = BM / kScaleRows;
+  static constexpr int kScaleRing = S <= 3 ? 2 : 4;
+  static constexpr int kScaleBuf = BM * 16;
+  static constexpr int kLoop = S * kStage + kScaleRing * kScaleBuf + 256;
+  static constexpr int kOut = kWaves * 16 * (16 * TN * 4 + 16);  // the epilogue's transposition
+  static constexpr int kLds = kLoop > kOut ? kLoop : kOut;
   static constexpr int kXLoads = BM / 8 / kWaves;  // 1 KB loads per wave and stage
   static constexpr int kWLoads = BN / 8 / kWaves;
   static constexpr int kLoads = kXLoads + kWLoads + 1;
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "a stage splits evenly over the waves");
   static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "wave tile");
   static_assert(128 % (16 * TN) == 0, "a wave's columns lie in one scale block");
+  static_assert(TN == 2 || TN == 4, "the epilogue's rows take whole waves");
   static_assert(TM % 2 == 0, "the pipeline's two register sets alternate over whole blocks");
-  static_assert(BM % 64 == 0 && BM <= 64 * kWaves, "one row-scale load per wave");
+  static_assert(kScaleSteps == 1 || kScaleSteps == 2, "a group's scales come with two stages at most");
   static_assert(kLds <= 160 * 1024, "LDS");
 };
 
@@ -59,7 +67,7 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   using C = Tile<BM, BN, WM, WN, S>;
   constexpr int TM = C::TM, TN = C::TN;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  float* const s_lds = reinterpret_cast<float*>(smem + S * C::kStage);
+  uint8_t* const s_lds = smem + S * C::kStage;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -103,15 +111,24 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     const int row = (wave + C::kWaves * i) * 8 + (lane >> 3);
     w_off[i] = row < ncols ? (uint32_t)(row * (int)a.ldw + chunk) : kOutOfRange;
   }
-  const int s_row0 = (wave % (BM / 64)) * 64;  // waves past BM / 64 load the same rows again
-  const uint32_t s_off = s_row0 + lane < mrows ? (uint32_t)((s_row0 + lane) * (int)a.ldxs) * 4u : kOutOfRange;
+  // Scales of K blocks kb0 + 4 G .. + 3 (group G): lane l brings row l / 4, block l % 4. Group G + 1
+  // comes with the last stages of group G (the second of them where kScaleSteps is 1), after
+  // every wave has read the group whose buffer it takes, and before its own first block.
+  const int s_row = (wave * 16) % C::kScaleRows;
+  auto issue_scales = [&](int g, int part, bool real) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(sp, real ? s_bytes : 0u);
+    const int row0 = part * C::kScaleRows + s_row, row = row0 + (lane >> 2);
+    const uint32_t off = row < mrows ? (uint32_t)(row * (int)a.ldxs + (lane & 3)) * 4u : kOutOfRange;
+    // An empty load writes zeros: past the ring, where nothing is read.
+    uint8_t* const to = s_lds + (real ? (g % C::kScaleRing) * C::kScaleBuf + row0 * 16 : C::kScaleRing * C::kScaleBuf);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)to, 4, off, real ? (kb0 + 4 * g) * 4 : 0, 0, 0);
+  };
 
   auto issue = [&](int kb, int st) __attribute__((always_inline)) {
     // A block past the slice is loaded through empty resources: zeros, without touching memory.
     const bool ok = kb < kb1;
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(xp, ok ? x_bytes : 0u);
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, ok ? w_bytes : 0u);
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(sp, ok ? s_bytes : 0u);
     const int sk = ok ? kb : 0;
     uint8_t* const base = smem + st * C::kStage;
     if (ok && a.k - kb * kBlockK <= chunk) {
@@ -126,7 +143,9 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     for (int i = 0; i < C::kXLoads; ++i) load16(rx, base, wave + C::kWaves * i, x_off[i], sk * kBlockK);
 #pragma unroll
     for (int i = 0; i < C::kWLoads; ++i) load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_off[i], sk * kBlockK);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(s_lds + st * BM + s_row0), 4, s_off, sk * 4, 0, 0);
+    const int in_group = (kb - kb0) & 3, g = ((kb - kb0) >> 2) + 1;
+    const int part = in_group - (4 - C::kScaleSteps);
+    issue_scales(g, part < 0 ? 0 : part, part >= 0 && kb0 + 4 * g < kb1);
   };
 
   f4 acc[TM][TN];
@@ -157,6 +176,8 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   float ws64 = load_ws(kb0);
 
 #pragma unroll
+  for (int i = 0; i < C::kScaleSteps; ++i) issue_scales(0, i, true);
+#pragma unroll
   for (int i = 0; i < S; ++i) issue(kb0 + i, i);
   stage_barrier<(S - 1) * C::kLoads>();
   // Software pipeline: the fragments of a step are read one step ahead, its results are scaled one
@@ -172,11 +193,14 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     d[(TM - 1) & 1][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   af[0] = frag(smem, x_at, 0);
-  xs[0] = s_lds[x_row];
+  auto scale = [&](int step, int i) {  // of row x_row + 16 i, K block kb0 + step
+    return *reinterpret_cast<const float*>(s_lds + ((step >> 2) % C::kScaleRing) * C::kScaleBuf + (step & 3) * 4 +
+                                           (x_row + 16 * i) * 16);
+  };
+  xs[0] = scale(0, 0);
   int st = 0;
   for (int kb = kb0; kb < kb1; ++kb) {
     const uint8_t* const stage = smem + st * C::kStage;
-    const float* const scales = s_lds + st * BM + x_row;
     const int next = st + 1 == S ? 0 : st + 1;
     const uint8_t* const stage2 = smem + next * C::kStage;
     const int at = (kb - kb0) & 63;
@@ -189,13 +213,13 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     for (int i = 0; i < TM; ++i) {
       if (i + 1 < TM) {
         af[(i + 1) & 1] = frag(stage, x_at, i + 1);
-        xs[(i + 1) & 1] = scales[16 * (i + 1)];
+        xs[(i + 1) & 1] = scale(kb - kb0, i + 1);
       } else {
         stage_barrier<(S - 2) * C::kLoads>();
         issue(kb + S, st);
         __builtin_amdgcn_sched_barrier(0);
         af[(i + 1) & 1] = frag(stage2, x_at, 0);
-        xs[(i + 1) & 1] = s_lds[next * BM + x_row];
+        xs[(i + 1) & 1] = scale(kb + 1 - kb0, 0);
       }
       sc[i & 1] = xs[i & 1] * ws;
       constexpr int kLast = TM - 1;
@@ -221,28 +245,58 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     for (int q = 0; q < 4; ++q)
       acc[TM - 1][j][q] = __builtin_fmaf(sc[(TM - 1) & 1], d[(TM - 1) & 1][j][q], acc[TM - 1][j][q]);
 
-  __builtin_amdgcn_s_waitcnt((0 & 0xF) | (0x7 << 4) | (0xF << 8));  // the last (empty) loads into LDS have ended
+  // ---- epilogue. A lane holds runs of four columns of 16 rows, 32 bytes of each line; each wave
+  // turns 16 rows x 16 TN columns at a time over through LDS (its own part of the stages, free once every
+  // wave's last, empty loads have ended), so that a store covers whole 128-byte pieces (TN 4) of its
+  // rows.
+  const bool partial = split_k > 1;
+  const bool wide = (a.n & 7) == 0 && (partial || wide_rows(a));
+  const int n_wave = n0 + wn * TN * 16;
   const int g4 = 4 * (lane >> 4);
-  const bool vec = split_k > 1 ? (a.n & 3) == 0 : runs_aligned(a);
+  stage_barrier<0>();
+  if (wide) {
+    constexpr int kCols = 16 * TN, kRow = kCols * 4 + 16;  // LDS row in bytes, padded off the banks of the next
+    constexpr int kLanes = kCols / 8;                      // lanes per row, eight columns each
+    uint8_t* const mine = smem + wave * 16 * kRow;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) *reinterpret_cast<f4*>(mine + c16 * kRow + (16 * j + g4) * 4) = acc[i][j];
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+      for (int h = 0; h < 16 * kLanes / 64; ++h) {
+        const int row = h * (64 / kLanes) + lane / kLanes, col = (lane % kLanes) * 8;
+        const f4 lo = *reinterpret_cast<const f4*>(mine + row * kRow + col * 4);
+        const f4 hi = *reinterpret_cast<const f4*>(mine + row * kRow + col * 4 + 16);
+        const int m = m0 + (wm * TM + i) * 16 + row, n = n_wave + col;
+        if (m >= a.m || n >= a.n) continue;
+        if (partial) {
+          f4* const p = reinterpret_cast<f4*>(part + ((int64_t)z * a.m + m) * a.n + n);
+          p[0] = lo;
+          p[1] = hi;
+        } else {
+          store_block8(a, m, n, lo, hi);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int m = m0 + x_row + 16 * i;
     if (m >= a.m) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = n0 + wn * TN * 16 + 16 * j + g4;
+      const int n = n_wave + 16 * j + g4;
       if (n >= a.n) continue;
-      if (split_k > 1) {
+      if (partial) {
         float* const p = part + ((int64_t)z * a.m + m) * a.n + n;
-        if (vec) {
-          *reinterpret_cast<f4*>(p) = acc[i][j];
-        } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (n + q < a.n) p[q] = acc[i][j][q];
-        }
+        for (int q = 0; q < 4; ++q)
+          if (n + q < a.n) p[q] = acc[i][j][q];
       } else {
-        store_block4(a, m, n, acc[i][j], vec);
+        store_block4(a, m, n, acc[i][j], false);
       }
     }
   }
