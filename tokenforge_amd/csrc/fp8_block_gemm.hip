@@ -124,28 +124,32 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)to, 4, off, real ? (kb0 + 4 * g) * 4 : 0, 0, 0);
   };
 
-  auto issue = [&](int kb, int st) __attribute__((always_inline)) {
-    // A block past the slice is loaded through empty resources: zeros, without touching memory.
+  // Load l of a wave for block kb into stage st: x, w, then the scales that come along. A block past
+  // the slice is loaded through an empty resource: zeros, without touching memory.
+  auto issue = [&](int kb, int st, int l) __attribute__((always_inline)) {
     const bool ok = kb < kb1;
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(xp, ok ? x_bytes : 0u);
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, ok ? w_bytes : 0u);
-    const int sk = ok ? kb : 0;
+    const int soff = ok ? kb * kBlockK : 0;
     uint8_t* const base = smem + st * C::kStage;
-    if (ok && a.k - kb * kBlockK <= chunk) {
-      // K ends inside this block, the last one: chunks past it are zeros on both sides, from here on
-      // (only empty blocks follow).
+    if (l < C::kXLoads) {
+      load16(make_rsrc(xp, ok ? x_bytes : 0u), base, wave + C::kWaves * l, x_off[l < C::kXLoads ? l : 0], soff);
+    } else if (l < C::kXLoads + C::kWLoads) {
+      const int i = l < C::kXLoads || l >= C::kXLoads + C::kWLoads ? 0 : l - C::kXLoads;
+      load16(make_rsrc(wp, ok ? w_bytes : 0u), base + C::kXBytes, wave + C::kWaves * i, w_off[i], soff);
+    } else {
+      const int in_group = (kb - kb0) & 3, g = ((kb - kb0) >> 2) + 1;
+      const int part = in_group - (4 - C::kScaleSteps);
+      issue_scales(g, part < 0 ? 0 : part, part >= 0 && kb0 + 4 * g < kb1);
+    }
+  };
+  // Before a block's first load: where K ends inside it, the last one, chunks past it are zeros on both
+  // sides, from there on (only empty blocks follow).
+  auto mask_tail = [&](int kb) __attribute__((always_inline)) {
+    if (kb < kb1 && a.k - kb * kBlockK <= chunk) {
 #pragma unroll
       for (int i = 0; i < C::kXLoads; ++i) x_off[i] = kOutOfRange;
 #pragma unroll
       for (int i = 0; i < C::kWLoads; ++i) w_off[i] = kOutOfRange;
     }
-#pragma unroll
-    for (int i = 0; i < C::kXLoads; ++i) load16(rx, base, wave + C::kWaves * i, x_off[i], sk * kBlockK);
-#pragma unroll
-    for (int i = 0; i < C::kWLoads; ++i) load16(rw, base + C::kXBytes, wave + C::kWaves * i, w_off[i], sk * kBlockK);
-    const int in_group = (kb - kb0) & 3, g = ((kb - kb0) >> 2) + 1;
-    const int part = in_group - (4 - C::kScaleSteps);
-    issue_scales(g, part < 0 ? 0 : part, part >= 0 && kb0 + 4 * g < kb1);
   };
 
   f4 acc[TM][TN];
@@ -178,12 +182,19 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
 #pragma unroll
   for (int i = 0; i < C::kScaleSteps; ++i) issue_scales(0, i, true);
 #pragma unroll
-  for (int i = 0; i < S; ++i) issue(kb0 + i, i);
-  stage_barrier<(S - 1) * C::kLoads>();
+  for (int s = 0; s < S; ++s) {
+    mask_tail(kb0 + s);
+#pragma unroll
+    for (int l = 0; l < C::kLoads; ++l)
+      if (s < S - 1 || l < TN) issue(kb0 + s, s, l);  // the last stage's others go out in the first block
+  }
+  stage_barrier<(S - 2) * C::kLoads + (TN < C::kLoads ? TN : C::kLoads)>();
   // Software pipeline: the fragments of a step are read one step ahead, its results are scaled one
   // step after its MFMAs, and the barrier to the next block stands before a block's last step: by
   // then a wave has read all of its stage, so the stage is refilled and the next block's first
-  // fragments are read beside that step's MFMAs.
+  // fragments are read beside that step's MFMAs. The refill's loads go out one after each of these
+  // MFMAs and two after each of the next step's: together, ahead of them, they hold the wave up
+  // (gate_up M = 4096 on MI355X: 584 us against 555; later ones arrive late: 592 to 608).
   v8i bf[TN], af[2];
   float xs[2], sc[2] = {0.0f, 0.0f};
   f4 d[2][TN];
@@ -216,8 +227,7 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
         xs[(i + 1) & 1] = scale(kb - kb0, i + 1);
       } else {
         stage_barrier<(S - 2) * C::kLoads>();
-        issue(kb + S, st);
-        __builtin_amdgcn_sched_barrier(0);
+        mask_tail(kb + S);
         af[(i + 1) & 1] = frag(stage2, x_at, 0);
         xs[(i + 1) & 1] = scale(kb + 1 - kb0, 0);
       }
@@ -233,7 +243,15 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
           acc[p][j][q] = __builtin_fmaf(sc[(i + 1) & 1], d[(i + 1) & 1][j][q], acc[p][j][q]);
         // Holds the MFMA and the scaling here: without a use in order they are moved to their results' uses.
         __asm__ volatile("" : "+v"(d[i & 1][j]), "+v"(acc[p][j]));
-        if (i + 1 == TM) bf[j] = frag(stage2, w_at, j);  // in place, its last MFMA issued
+        if (i + 1 == TM) {
+          bf[j] = frag(stage2, w_at, j);  // in place, its last MFMA issued
+          if (j < C::kLoads) issue(kb + S, st, j);
+        }
+        if (i == 0) {
+#pragma unroll
+          for (int l = TN; l < C::kLoads; ++l)
+            if ((l - TN) / 2 == j || (j + 1 == TN && (l - TN) / 2 > j)) issue(kb + S - 1, st == 0 ? S - 1 : st - 1, l);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
