@@ -17,7 +17,14 @@ namespace tf {
 typedef int v8i __attribute__((ext_vector_type(8)));
 
 constexpr int kBlockK = 128;        // K per scale block, and per MFMA
+constexpr int kStream = 2;          // nt: data read once
 constexpr int kUnitScale = 127;     // E8M0 2^0: the MFMA's own block scales leave the product as is
+
+// v of the lane N below, cyclic in each row of 16 lanes.
+template <int N>
+__device__ __forceinline__ uint32_t dpp_ror(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x120 + N, 0xF, 0xF, false);
+}
 
 struct BlockArgs {
   const uint8_t* x8;  // [m, k] codes, row stride ldx bytes (16-byte aligned rows)

@@ -372,8 +372,8 @@ struct Entry {
 
 #define TF_BLOCK(BM, BN, WM, WN, S) {BM, BN, WM * WN, S, launch<BM, BN, WM, WN, S>}
 const Entry kEntries[] = {
-    TF_BLOCK(256, 256, 2, 4, 2), TF_BLOCK(256, 128, 4, 2, 3), TF_BLOCK(128, 256, 2, 4, 3), TF_BLOCK(128, 128, 2, 2, 2),
-    TF_BLOCK(128, 128, 2, 4, 4), TF_BLOCK(64, 128, 2, 4, 3),  TF_BLOCK(64, 64, 2, 2, 4),
+    TF_BLOCK(256, 256, 2, 4, 2), TF_BLOCK(128, 256, 2, 4, 3), TF_BLOCK(128, 128, 2, 4, 4), TF_BLOCK(64, 256, 2, 4, 3),
+    TF_BLOCK(64, 64, 2, 2, 4),   TF_BLOCK(32, 256, 1, 4, 4),  TF_BLOCK(32, 128, 1, 4, 4),
 };
 
 const Entry* find(const tf_gemm_config& cfg) {
