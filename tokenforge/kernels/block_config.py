@@ -1,10 +1,11 @@
 """Launch configurations of the block-scaled e4m3 linear (``fp8_block_linear``).
 
-A call's config follows from its M, N and K alone: of the compiled kernels and K splits, the one whose
-modelled time is least. The models' constants were fitted to the measured times of every config on
-about 4000 layers and row counts on MI355X (M 1 to 4096, weights of 16 KB to 136 MB, read from HBM): the
-choice is 2.0% slower than the best compiled config on average, 5% at the 90th percentile. There is no
-table of tuned layers.
+A call's config follows from its M, N and K alone. Few rows take the gemv form up to a weight size
+(:func:`_gemv_waves`); else, of the compiled tiles and K splits, the one whose modelled time is least. The
+limits and the model's constants come from the measured times of every config on about 6000 layers and
+row counts on MI355X (M 1 to 4096, weights of 16 KB to 136 MB, read from HBM): the choice is 2 to 3% slower
+than the best compiled config on average (M <= 4 1.5%, 9 to 16 rows 2.8%, 33 to 128 rows on small weights
+4%). There is no table of tuned layers.
 """
 
 from __future__ import annotations
@@ -37,28 +38,6 @@ class BlockConfig:
     split_k: int
     num_warps: int
     num_stages: int
-
-
-@dataclass(frozen=True)
-class _Gemv:
-    """Time in us: a start, the wave's share of blocks at ``block`` each, more where many waves share a CU,
-    and the weight bytes at ``rate`` (bytes/us), ``again`` of them for every further row tile."""
-
-    block_m: int
-    num_warps: int
-    start: float
-    block: float
-    crowd: float
-    rate: float
-    again: float
-
-    def us(self, m: int, n: int, k: int) -> float:
-        tiles_m = -(-m // self.block_m)
-        groups = -(-n // 16) * tiles_m
-        wave = -(-_blocks(k) // self.num_warps) * self.block
-        compute = wave * (1 + groups * self.num_warps / (NUM_CUS * self.crowd))
-        memory = n * k * (1 + self.again * (tiles_m - 1)) / self.rate
-        return self.start + (compute**4 + memory**4) ** 0.25
 
 
 @dataclass(frozen=True)
@@ -95,12 +74,6 @@ class _Gemm:
         return us + self.reduce + 8 * m * n * split / self.reduce_rate if split > 1 else us
 
 
-_GEMV = (
-    _Gemv(4, 8, 3.19, 0.610, 9.1, 4.41e6, 0.3),
-    _Gemv(4, 4, 3.26, 0.363, 6.6, 4.28e6, 0.3),
-    _Gemv(8, 4, 3.37, 0.377, 12.7, 3.50e6, 0.3),
-    _Gemv(16, 4, 3.36, 0.505, 36.0, 2.79e6, 1.0),
-)
 _GEMM = (
     _Gemm(256, 256, 8, 2, 1, 6.00, 3.19, 1.296, 1.824, 3.92e6, 2.19, 6.95e6),
     _Gemm(128, 256, 8, 3, 1, 4.43, 2.86, 0.795, 1.060, 5.37e6, 2.42, 6.14e6),
@@ -110,15 +83,14 @@ _GEMM = (
     _Gemm(32, 256, 4, 4, 1, 2.19, 2.97, 0.597, 0.666, 5.08e6, 2.68, 4.85e6),
     _Gemm(32, 128, 4, 4, 1, 1.79, 2.45, 0.417, 0.444, 6.03e6, 2.76, 4.44e6),
 )
+_GEMV_TILES = ((4, 8), (4, 4), (8, 4), (16, 4))  # rows, waves
 _GEMV_STAGES = 4
-GEMV_MAX_M = 128
-"""Row count up to which the gemv form is weighed (it reads the weight once per 16 rows)."""
 _SPLITS = (1, 2, 3, 4, 6, 8, 12, 16)
 _MAX_SPLIT_GROUPS = 700
 """Workgroups up to which K is split: past that the chip is full."""
 
 BLOCK_TILES: tuple[tuple[str, int, int, int, int], ...] = tuple(
-    [("gemv_block", g.block_m, 16, g.num_warps, _GEMV_STAGES) for g in _GEMV]
+    [("gemv_block", rows, 16, waves, _GEMV_STAGES) for rows, waves in _GEMV_TILES]
     + [("gemm_block", t.block_m, t.block_n, t.num_warps, t.num_stages) for t in _GEMM]
 )
 """(kernel, block_m, block_n, num_warps, num_stages) of every compiled kernel."""
@@ -128,18 +100,33 @@ def _blocks(k: int) -> int:
     return -(-k // BLOCK)
 
 
+def _gemv_waves(m: int, n: int, k: int) -> int:
+    """Waves per workgroup of the gemv form, 0 where a tile is faster. The form reads the weight once per 16
+    rows without staging x: on MI355X it wins while the weight is small (3584 x 3584 M = 7: 6.2 us against
+    10.6 for the best tile; 896 x 4864 M = 12: 7.7 against 9.8) and loses on wide layers with more rows
+    (37888 x 3584 M = 7: 29.6 against 25.1 to 31 over boxes, M = 12: 43 against 29.6). From K = 2048 on eight
+    waves along K are faster than four at M <= 4 (3584 x 18944: 15.8 us against 17.9; 1152 x 896 the other
+    way, 3.9 against 3.7)."""
+    weight = n * k
+    if m <= 4:
+        return 8 if k >= 2048 else 4
+    if m <= 8:
+        return 4 if weight < 48e6 else 0
+    if m <= 16:
+        return 4 if weight < 24e6 else 0
+    if m <= 32:
+        return 4 if weight < 8e6 else 0
+    return 4 if m <= 128 and weight * -(-m // 16) < 12e6 else 0
+
+
 @functools.lru_cache(maxsize=4096)
 def block_config(m: int, n: int, k: int) -> BlockConfig:
-    """The launch of an M x N x K call: the least modelled time."""
+    """The launch of an M x N x K call."""
+    waves = _gemv_waves(m, n, k)
+    if waves:
+        return BlockConfig("gemv_block", 4 if m <= 4 else 8 if m <= 8 else 16, 16, 1, waves, _GEMV_STAGES)
     nkb = _blocks(k)
-    rows = 4 if m <= 4 else 8 if m <= 8 else 16
     best: tuple[float, BlockConfig] | None = None
-    if m <= GEMV_MAX_M:
-        for g in _GEMV:
-            if g.block_m == rows:
-                us = g.us(m, n, k)
-                if best is None or us < best[0]:
-                    best = us, BlockConfig("gemv_block", rows, 16, 1, g.num_warps, _GEMV_STAGES)
     for t in _GEMM:
         tiles = -(-m // t.block_m) * -(-n // t.block_n)
         for split in _SPLITS:

@@ -17,7 +17,6 @@ namespace tf {
 typedef int v8i __attribute__((ext_vector_type(8)));
 
 constexpr int kBlockK = 128;        // K per scale block, and per MFMA
-constexpr int kStream = 2;          // nt: data read once
 constexpr int kUnitScale = 127;     // E8M0 2^0: the MFMA's own block scales leave the product as is
 
 // v of the lane N below, cyclic in each row of 16 lanes.

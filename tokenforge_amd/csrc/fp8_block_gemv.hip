@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64 * KS) void block_gemv_kernel(BlockArgs a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           w[s * G + j][h] = __builtin_amdgcn_raw_buffer_load_b128(
-              rw, (int)(16 * h < left ? w_off : kOutOfRange), (ok ? kb + j * KS : 0) * kBlockK + 16 * h, kStream);
+              rw, (int)(16 * h < left ? w_off : kOutOfRange), (ok ? kb + j * KS : 0) * kBlockK + 16 * h, 0);
       }
     };
     auto wide = [](const u4(&v)[2]) {
