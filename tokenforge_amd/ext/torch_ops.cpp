@@ -21,6 +21,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
@@ -530,13 +531,17 @@ at::Tensor plain_rows(const at::Tensor& t) {
 
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// The outputs' options and [..., blocks] (or [..., 1]) shape of a quantizer's codes and scales.
+// An output straight from the caching allocator, without another pass through the dispatcher.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const c10::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, dev, std::nullopt));
+}
+
+// A quantizer's codes [..., k] and scales [..., blocks] (or [..., 1]).
 at::Tensor empty_codes(const at::Tensor& x, int64_t k) {
-  return at::empty(with_last(x.sizes().slice(0, x.dim() - 1), k), x.options().dtype(at::kFloat8_e4m3fn));
+  return fresh(with_last(x.sizes().slice(0, x.dim() - 1), k), at::kFloat8_e4m3fn, x.device());
 }
 at::Tensor empty_scales(const at::Tensor& x, int64_t k, int64_t g) {
-  return at::empty(with_last(x.sizes().slice(0, x.dim() - 1), g ? (k + kBlock - 1) / kBlock : 1),
-                   x.options().dtype(at::kFloat));
+  return fresh(with_last(x.sizes().slice(0, x.dim() - 1), g ? (k + kBlock - 1) / kBlock : 1), at::kFloat, x.device());
 }
 
 // Whether a quantizer's input takes the fast path; rows out.
@@ -589,7 +594,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_norm_fast(const at::Tensor& x
   }
   c10::OptionalDeviceGuard guard(dev);
   at::Tensor q = empty_codes(x, h), s = empty_scales(x, h, g);
-  at::Tensor hidden = r2.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  at::Tensor hidden = r2.defined() ? fresh(x.sizes(), x.scalar_type(), dev) : fresh({0}, x.scalar_type(), dev);
   check(api().add_norm(data<const uint16_t>(x2), row_stride(x2), r2.defined() ? data<const uint16_t>(r2) : nullptr,
                        r2.defined() ? row_stride(r2) : 0, data<const uint16_t>(w), dtype_code(x.scalar_type()),
                        data<uint8_t>(q), data<float>(s), r2.defined() ? data<uint16_t>(hidden) : nullptr, x2.size(0),
@@ -649,9 +654,9 @@ at::Tensor block_linear_fast(const at::Tensor& x8, const at::Tensor& xs, const a
   const Launch l = resolve(Key{kBlockLinear, TF_EPILOGUE_NONE, m, n, k, kBlock, dev.index()});
   count(l);
   c10::OptionalDeviceGuard guard(dev);
-  at::Tensor out = at::empty(out_shape, x8.options().dtype(out_dtype));
+  at::Tensor out = fresh(out_shape, out_dtype, dev);
   at::Tensor work;
-  if (l.need > 0) work = at::empty({(l.need + 3) / 4}, x8.options().dtype(at::kFloat));
+  if (l.need > 0) work = fresh({(l.need + 3) / 4}, at::kFloat, dev);
   check(api().block_linear(data<const uint8_t>(x2), row_stride(x2), data<const float>(s2), row_stride(s2),
                            data<const uint8_t>(w2), row_stride(w2), data<const float>(ws2), row_stride(ws2),
                            static_cast<const uint16_t*>(ptr_or_null(bias)),
