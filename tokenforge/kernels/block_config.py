@@ -1,7 +1,7 @@
 """Launch configurations of the block-scaled e4m3 linear (``fp8_block_linear``).
 
 A call's config follows from its M, N and K alone. Few rows take the gemv form up to a weight size
-(:func:`_gemv_waves`); else, of the compiled tiles and K splits, the one whose modelled time is least. The
+(:func:`_gemv_tile`); else, of the compiled tiles and K splits, the one whose modelled time is least. The
 limits and the model's constants come from the measured times of every config on about 6000 layers and
 row counts on MI355X (M 1 to 4096, weights of 16 KB to 136 MB, read from HBM): the choice is 2 to 3% slower
 than the best compiled config on average (M <= 4 1.5%, 9 to 16 rows 2.8%, 33 to 128 rows on small weights
@@ -25,7 +25,7 @@ class BlockConfig:
     ========== ============================== ==============================================
     kernel     block_m / block_n              split_k / num_warps / num_stages
     ========== ============================== ==============================================
-    gemv_block rows per workgroup (4, 8, 16)  1 / waves that share K / K blocks in flight
+    gemv_block rows per workgroup (4 to 32)   1 / waves that share K / K blocks in flight
                / 16 columns                   per wave
     gemm_block tile rows / tile columns       K slices, added by a second kernel / waves /
                                               LDS stages
@@ -83,14 +83,14 @@ _GEMM = (
     _Gemm(32, 256, 4, 4, 1, 2.19, 2.97, 0.597, 0.666, 5.08e6, 2.68, 4.85e6),
     _Gemm(32, 128, 4, 4, 1, 1.79, 2.45, 0.417, 0.444, 6.03e6, 2.76, 4.44e6),
 )
-_GEMV_TILES = ((4, 8), (4, 4), (8, 4), (16, 4))  # rows, waves
-_GEMV_STAGES = 4
+_GEMV_TILES = ((4, 8, 4), (4, 4, 4), (8, 4, 4), (16, 4, 4), (32, 4, 2))
+"""(block_m, num_warps, num_stages) of the gemv form."""
 _SPLITS = (1, 2, 3, 4, 6, 8, 12, 16)
 _MAX_SPLIT_GROUPS = 700
 """Workgroups up to which K is split: past that the chip is full."""
 
 BLOCK_TILES: tuple[tuple[str, int, int, int, int], ...] = tuple(
-    [("gemv_block", rows, 16, waves, _GEMV_STAGES) for rows, waves in _GEMV_TILES]
+    [("gemv_block", rows, 16, waves, stages) for rows, waves, stages in _GEMV_TILES]
     + [("gemm_block", t.block_m, t.block_n, t.num_warps, t.num_stages) for t in _GEMM]
 )
 """(kernel, block_m, block_n, num_warps, num_stages) of every compiled kernel."""
@@ -100,31 +100,35 @@ def _blocks(k: int) -> int:
     return -(-k // BLOCK)
 
 
-def _gemv_waves(m: int, n: int, k: int) -> int:
-    """Waves per workgroup of the gemv form, 0 where a tile is faster. The form reads the weight once per 16
-    rows without staging x: on MI355X it wins while the weight is small (3584 x 3584 M = 7: 6.2 us against
-    10.6 for the best tile; 896 x 4864 M = 12: 7.7 against 9.8) and loses on wide layers with more rows
-    (37888 x 3584 M = 7: 29.6 against 25.1 to 31 over boxes, M = 12: 43 against 29.6). From K = 2048 on eight
-    waves along K are faster than four at M <= 4 (3584 x 18944: 15.8 us against 17.9; 1152 x 896 the other
-    way, 3.9 against 3.7)."""
+def _gemv_tile(m: int, n: int, k: int) -> tuple[int, int, int] | None:
+    """The gemv form's tile for a call, None where the gemm form is faster.
+
+    The gemv form stages nothing: it wins while the weight is small and the rows are few, and loses where
+    its reads of x (once per 16 columns) or of the weight (once per row tile) weigh more. MI355X, the two
+    forms' best: 3584 x 3584 M = 7 6.2 us against 10.6, M = 20 8.4 against 11.0, M = 48 13.6 against 11.7;
+    896 x 4864 M = 48 8.4 against 10.2, M = 128 10.6 against 11.6; 37888 x 3584 M = 12 43 against 29.6;
+    3584 x 18944 M = 7 18.8 either way. Eight waves along K against four at M <= 4: 3584 x 18944 15.8 us
+    against 17.9, 1152 x 896 3.9 against 3.7."""
     weight = n * k
     if m <= 4:
-        return 8 if k >= 2048 else 4
+        return _GEMV_TILES[0] if k >= 2048 else _GEMV_TILES[1]
     if m <= 8:
-        return 4 if weight < 48e6 else 0
+        return _GEMV_TILES[2] if weight < 70e6 else None
     if m <= 16:
-        return 4 if weight < 24e6 else 0
-    if m <= 32:
-        return 4 if weight < 8e6 else 0
-    return 4 if m <= 128 and weight * -(-m // 16) < 12e6 else 0
+        return _GEMV_TILES[3] if weight < 24e6 else None
+    if m <= 64 and weight < 5e6:
+        return _GEMV_TILES[3]
+    if (m <= 32 and weight < 16e6) or (m <= 128 and weight < 5e6) or (m <= 256 and weight < 1.5e6):
+        return _GEMV_TILES[4]
+    return None
 
 
 @functools.lru_cache(maxsize=4096)
 def block_config(m: int, n: int, k: int) -> BlockConfig:
     """The launch of an M x N x K call."""
-    waves = _gemv_waves(m, n, k)
-    if waves:
-        return BlockConfig("gemv_block", 4 if m <= 4 else 8 if m <= 8 else 16, 16, 1, waves, _GEMV_STAGES)
+    gemv = _gemv_tile(m, n, k)
+    if gemv is not None:
+        return BlockConfig("gemv_block", gemv[0], 16, 1, gemv[1], gemv[2])
     nkb = _blocks(k)
     best: tuple[float, BlockConfig] | None = None
     for t in _GEMM:
