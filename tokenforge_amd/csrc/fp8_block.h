@@ -93,7 +93,9 @@ __device__ __forceinline__ bool wide_rows(const BlockArgs& a) {
          (a.residual == nullptr || ((a.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0));
 }
 
-// Columns n .. n + 7 of row m, as store_block4 (n % 8 == 0, N % 8 == 0 and wide_rows hold).
+// Columns n .. n + 7 of row m, as store_block4 (n % 8 == 0, N % 8 == 0 and wide_rows hold). STREAM: a
+// non-temporal store.
+template <bool STREAM>
 __device__ __forceinline__ void store_block8(const BlockArgs& a, int m, int n, const f4& lo, const f4& hi) {
   float v[8];
 #pragma unroll
@@ -110,7 +112,11 @@ __device__ __forceinline__ void store_block8(const BlockArgs& a, int m, int n, c
   u4 h;
 #pragma unroll
   for (int j = 0; j < 4; ++j) h[j] = (uint32_t)to_16(a, v[2 * j]) | ((uint32_t)to_16(a, v[2 * j + 1]) << 16);
-  *reinterpret_cast<u4*>(a.out + (int64_t)m * a.ldo + n) = h;
+  u4* const o = reinterpret_cast<u4*>(a.out + (int64_t)m * a.ldo + n);
+  if (STREAM)
+    __builtin_nontemporal_store(h, o);
+  else
+    *o = h;
 }
 
 // Row strides (bytes of codes, elements of scales) below which a tile's offsets stay in 31 bits.

@@ -45,6 +45,8 @@ struct Tile {
   static_assert(kLds <= 160 * 1024, "LDS");
 };
 
+constexpr int64_t kL2Bytes = 4 << 20;  // of one XCD
+
 template <int N>
 __device__ __forceinline__ void stage_barrier() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
@@ -61,7 +63,9 @@ __device__ __forceinline__ void load16(__amdgpu_buffer_rsrc_t r, uint8_t* base, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(base + j * 1024), 16, off, soff, 0, 0);
 }
 
-template <int BM, int BN, int WM, int WN, int S>
+// STREAM: the output, larger than the XCDs' L2s, goes past them and leaves them to the panels (gate_up M =
+// 4096 on MI355X: 548 us against 532).
+template <int BM, int BN, int WM, int WN, int S, bool STREAM>
 __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, float* __restrict__ part, int split_k,
                                                                   int tiles_m, int tiles_n) {
   using C = Tile<BM, BN, WM, WN, S>;
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
           p[0] = lo;
           p[1] = hi;
         } else {
-          store_block8(a, m, n, lo, hi);
+          store_block8<STREAM>(a, m, n, lo, hi);
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
@@ -331,10 +335,15 @@ __global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs a, const fl
   const float* const p = part + m * a.n + n;
   f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   if ((a.n & 3) == 0) {
-    for (int z = 0; z < split_k; ++z) {
-      const f4 v = *reinterpret_cast<const f4*>(p + z * plane);
+    for (int z0 = 0; z0 < split_k; z0 += 4) {  // four slices' loads in flight
+      f4 v[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) sum[q] += v[q];
+      for (int z = 0; z < 4; ++z)
+        v[z] = z0 + z < split_k ? *reinterpret_cast<const f4*>(p + (z0 + z) * plane) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[q] += v[z][q];
     }
   } else {
     for (int z = 0; z < split_k; ++z)
@@ -351,7 +360,9 @@ int launch(const BlockArgs& a, int split, float* part, hipStream_t stream) {
   const int tiles_m = (int)cdiv(a.m, BM), tiles_n = (int)cdiv(a.n, BN);
   const int64_t grid = (int64_t)tiles_m * tiles_n * split;
   if (grid > 0x7FFFFFFF) return fail(TF_EINVAL, "tf_fp8_block_linear: too many tiles");
-  auto kernel = block_gemm_kernel<BM, BN, WM, WN, S>;
+  constexpr bool kMayStream = BM == 256;  // the tile of large outputs
+  const bool stream_out = kMayStream && split == 1 && (int64_t)a.m * a.n * 2 > (int64_t)kXcds * kL2Bytes;
+  auto kernel = stream_out ? block_gemm_kernel<BM, BN, WM, WN, S, kMayStream> : block_gemm_kernel<BM, BN, WM, WN, S, false>;
   if (C::kLds > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                           C::kLds) != hipSuccess)
