@@ -321,7 +321,7 @@ int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t ldx, const uint16_t* res
  * bias [n], residual [m, n] (stride ldr) or NULL and out [m, n] (stride ldo) of type `dtype`. k a
  * multiple of 16; n and m any; code rows less than 4 MiB apart, rows of xscale less than 2^20 elements. A block's products are summed by the MFMA, the blocks in fp32, and
  * bias and residual are added in fp32 before the one rounding. cfg: one of the compiled configs
- * (else TF_EINVAL); workspace: fp32, 16-byte aligned, >= tf_fp8_block_workspace_bytes
+ * (block_k 128; else TF_EINVAL); workspace: fp32, 16-byte aligned, >= tf_fp8_block_workspace_bytes
  * (-1 for an unknown config). */
 int64_t tf_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k, const tf_gemm_config* cfg);
 int tf_fp8_block_linear(const uint8_t* x8, int64_t ldx8, const float* xscale, int64_t ldxs,

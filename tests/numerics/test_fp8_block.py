@@ -267,6 +267,47 @@ def test_linear_takes_any_layout(device: torch.device) -> None:
     bc.check_linear(first, (x8[:1].cpu(), xs[:1].cpu(), w8.cpu(), ws.cpu()), "first row", None, res[:1].cpu())
 
 
+@pytest.mark.parametrize("m", [1, 3, 7, 12, 40])
+def test_linear_of_more_than_64_blocks_a_wave(m: int, device: torch.device) -> None:
+    """K so long that a wave runs out of its 64 weight scales and loads the next."""
+    n, k = 40, 66064
+    inputs = bc.linear_inputs(m, n, k, seed=7)
+    d = _to(device, inputs)
+    bc.check_linear(ops.fp8_block_linear(*d, None, torch.bfloat16, "hip"), inputs, "op")
+    for tile in BLOCK_TILES:
+        if tile[0] == "gemv_block" or tile[1] <= 64:
+            bc.check_linear(fp8_block_gemm(*d, _config(tile)), inputs, str(tile))
+
+
+def test_rows_far_apart(device: torch.device) -> None:
+    """Rows of codes 5 MB apart and of scales 2^20 elements apart are copied; the result is that of near ones."""
+    x8, xs, w8, ws = _to(device, bc.linear_inputs(3, 40, 256, seed=8))
+    want = ops.fp8_block_linear(x8, xs, w8, ws, None, torch.float16, "hip")
+    far = torch.full((3, 5 << 20), 0x7F, dtype=torch.uint8, device=device)
+    far[:, :256] = x8.view(torch.uint8)
+    sfar = torch.full((3, 1 << 20), float("nan"), device=device)
+    sfar[:, :2] = xs
+    got = ops.fp8_block_linear(far.view(torch.float8_e4m3fn)[:, :256], sfar[:, :2], w8, ws, None, torch.float16, "hip")
+    assert torch.equal(got, want)
+
+
+def test_calls_on_two_streams_at_once(device: torch.device) -> None:
+    """K-split calls (each with a workspace of its own) that overlap on two streams."""
+    sets = [_to(device, bc.linear_inputs(64, 512, 8192, seed=s)) for s in (9, 10)]
+    cfg = BlockConfig("gemm_block", 64, 64, 8, 4, 4)
+    want = [fp8_block_gemm(*d, cfg) for d in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got: list[list[torch.Tensor]] = [[], []]
+    for _ in range(20):
+        for i, (d, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(fp8_block_gemm(*d, cfg))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
 @pytest.mark.parametrize(("m", "n", "k"), [(3, 135000, 16384), (140000, 48, 16384), (70000, 35000, 128)])
 def test_linear_past_32_bit_offsets(m: int, n: int, k: int, device: torch.device) -> None:
     """x8, the weight and the output beyond 2 GiB: the first and last rows and columns are those of a small

@@ -136,6 +136,8 @@ def test_linear_refuses() -> None:
         (ValueError, "bias shape", {"bias": bias[:129]}),
         (TypeError, "bias must be", {"bias": bias.bfloat16()}),
         (ValueError, "weight", {"w8": w8[0]}),
+        (ValueError, "below", {"x8": torch.zeros((1, 1 << 22), dtype=torch.uint8).view(F8), "xs": xs[:1],
+                               "w8": torch.zeros((1, 1 << 22), dtype=torch.uint8).view(F8)}),
     ]
     for error, match, args in cases:
         with pytest.raises(error, match=match):
@@ -146,7 +148,7 @@ def test_linear_refuses() -> None:
 _X, _S, _W, _T, _O, _WS = (0x10000 * (i + 1) for i in range(6))
 
 
-def _entry(m: int = 4, n: int = 64, k: int = 256, cfg: tuple[int, ...] = (4, 16, 16, 128, 1, 8, 1), dtype: int = 0,
+def _entry(m: int = 4, n: int = 64, k: int = 256, cfg: tuple[int, ...] = (4, 16, 16, 128, 1, 4, 4), dtype: int = 0,
            x: int = _X, ldx: int = 256, ldxs: int = 2, ldw: int = 256, ldws: int = 2, ldo: int = 64, ldr: int = 64,
            residual: int | None = None, ws: int | None = None, ws_bytes: int = 0) -> tuple[int, bytes]:
     h = _lib.lib()
@@ -162,6 +164,11 @@ def _entry(m: int = 4, n: int = 64, k: int = 256, cfg: tuple[int, ...] = (4, 16,
     ({"ldo": 63}, b"row stride"), ({"residual": _O, "ldr": 1}, b"row stride"), ({"ldx": 264}, b"16-byte"),
     ({"x": _X + 8}, b"16-byte"), ({"ldw": 264}, b"16-byte"), ({"cfg": (1, 16, 16, 128, 1, 8, 1)}, b"compiled config"),
     ({"cfg": (4, 48, 16, 128, 1, 8, 1)}, b"compiled"), ({"x": 0}, b"null pointer"),
+    ({"cfg": (5, 256, 256, 64, 1, 8, 2)}, b"compiled"), ({"cfg": (5, 256, 256, 128, 0, 8, 2)}, b"compiled"),
+    ({"cfg": (5, 64, 64, 128, 2, 4, 4)}, b"workspace too small"),
+    ({"cfg": (5, 64, 64, 128, 2, 4, 4), "ws": _WS + 8, "ws_bytes": 1 << 20}, b"16-byte"),
+    ({"k": 1 << 22, "ldx": 1 << 22, "ldw": 1 << 22, "ldxs": 1 << 15, "ldws": 1 << 15}, b"apart"),
+    ({"ldxs": 1 << 20}, b"apart"),
 ])
 def test_linear_entry_refuses_on_the_host(args: dict, message: bytes) -> None:  # type: ignore[type-arg]
     rc, text = _entry(**args)

@@ -12,7 +12,7 @@ bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(
 using namespace tf;
 
 extern "C" int64_t tf_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k, const tf_gemm_config* cfg) {
-  if (!cfg || m < 0 || n < 0 || k < 0) return -1;
+  if (!cfg || m < 0 || n < 0 || k < 0 || cfg->block_k != kBlockK) return -1;
   if (cfg->kernel == TF_KERNEL_FP8_BLOCK_GEMV) return block_gemv_known(*cfg) ? 0 : -1;
   if (cfg->kernel != TF_KERNEL_FP8_BLOCK_GEMM || !block_gemm_known(*cfg)) return -1;
   const int split = block_split(*cfg, cdiv(k, kBlockK));

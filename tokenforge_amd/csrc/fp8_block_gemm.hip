@@ -1,11 +1,23 @@
 // Block-scaled e4m3 linear, many rows: BM x BN tiles through LDS.
 //
 // A workgroup of WM x WN waves streams 128-wide K blocks of x and the weight, and the rows' scales of
-// the block, into S LDS stages by buffer->LDS loads issued S - 1 blocks ahead, one barrier a block.
+// the block, into S LDS stages by buffer->LDS loads issued up to S blocks ahead, one barrier a block.
 // A wave computes a (16 TM) x (16 TN) sub-tile: per block one v_mfma_scale_f32_16x16x128_f8f6f4
 // (unit MFMA scales) per 16 x 16 from a zero accumulator, then acc += (xs[m] * ws) * that in fp32.
 // The weight fragment is the first operand: lane l holds row l % 16 and columns 4 (l / 16) + q, so a
 // lane's four results share one scale, and the wave's columns lie in one 128-wide scale block.
+//
+// A block's scale needs its own sum, so four VALU multiply-adds go with each MFMA of 32 cycles: with both
+// interleaved in registers alone, random codes reach 3.5 PFLOP/s on MI355X (MFMAs alone 4.0 to 4.4; the
+// nominal peak 5.0). The 256 x 256 tile reaches 2.05 (gate_up, N = 37888, K = 3584, M = 4096: 542 us; the
+// library's fp8 product of that size with one scale per tensor 504 us). Without its loads it takes 416
+// us, the loads alone 417, both 500: a stage of 64 KB is one block ahead (LDS holds two), so its latency is
+// covered by one block's MFMAs only. Of 9.25 rounds of tiles the last is a quarter full. The smaller
+// tiles serve fewer rows, where the weight's bytes bind: gate_up M = 48 29 us (4.8 TB/s) on 64 x 256.
+//
+// What did not help: w refilled half a block earlier behind a second barrier (602 us against 584), lines
+// asked for ahead into L2 (620 against 600), wave priorities (no change), bands of 4 or 16 rows (552, 568
+// against 553).
 //
 // LDS rows are 128 bytes, 16-byte chunk c of row r in slot c ^ s(r), s(r) = 2 (r % 4) ^ ((r / 4) % 2):
 // with lane l at row l % 16 and chunks 2 (l / 16) + {0, 1} the reads are free of bank conflicts.
