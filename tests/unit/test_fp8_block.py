@@ -227,3 +227,33 @@ def test_the_rule_names_compiled_configs() -> None:
             assert (cfg.kernel, cfg.block_m, cfg.block_n, cfg.num_warps, cfg.num_stages) in BLOCK_TILES
             assert 1 <= cfg.split_k <= max(1, -(-k // 128))
             assert fp8_block.workspace_bytes(m, n, k, cfg) >= 0
+
+
+# ----------------------------------------------------------------------------- the oracle
+
+
+def test_oracle_linear_against_scalar_loops() -> None:
+    from fractions import Fraction
+
+    from oracle.reference import e4m3_decode
+
+    x8, xs, w8, ws = bc.linear_inputs(2, 130, 144)
+    y, size, length = oblk.linear(bc.codes(x8), xs.numpy(), bc.codes(w8), ws.numpy())
+    xd, wd = e4m3_decode(bc.codes(x8)), e4m3_decode(bc.codes(w8))
+    for m, n in ((0, 0), (1, 127), (1, 129)):
+        terms = [Fraction(float(xd[m, k])) * Fraction(float(wd[n, k])) * Fraction(float(xs[m, k // 128]))
+                 * Fraction(float(ws[n // 128, k // 128])) for k in range(144)]
+        assert abs(float(sum(terms)) - y[m, n]) <= 144 * 2.0**-52 * size[m, n]
+        assert abs(float(sum(abs(t) for t in terms)) - size[m, n]) <= 144 * 2.0**-52 * size[m, n]
+        assert abs(float(sum(t * t for t in terms)) ** 0.5 - length[m, n]) <= 144 * 2.0**-52 * length[m, n]
+
+
+def test_oracle_half_step_and_scales() -> None:
+    values = np.sort(np.unique(np.abs(torch.arange(0, 127, dtype=torch.uint8).view(F8).float().numpy()))).astype(np.float64)
+    for lo, hi in zip(values[:-1], values[1:]):
+        assert oblk.half_step(np.array([lo]))[0] == (hi - lo) / 2, lo
+    y = np.array([[1.0, -448.0] + [0.0] * 126 + [-896.0, 2.0]])
+    assert np.array_equal(oblk.block_scales(y, 128), [[1.0, 2.0]])
+    assert np.array_equal(oblk.block_scales(y, 0), [[2.0]])
+    assert np.array_equal(oblk.block_scales(np.zeros((1, 3)), 128), [[1.0 / (448 * 512)]])
+    assert np.array_equal(oblk.spread(np.array([[1.0, 2.0]]), 130, 128), [[1.0] * 128 + [2.0] * 2])
