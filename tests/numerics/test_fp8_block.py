@@ -294,7 +294,7 @@ def test_rows_far_apart(device: torch.device) -> None:
 def test_calls_on_two_streams_at_once(device: torch.device) -> None:
     """K-split calls (each with a workspace of its own) that overlap on two streams."""
     sets = [_to(device, bc.linear_inputs(64, 512, 8192, seed=s)) for s in (9, 10)]
-    cfg = BlockConfig("gemm_block", 64, 64, 8, 4, 4)
+    cfg = BlockConfig("gemm_block", 64, 64, 8, 8, 4)
     want = [fp8_block_gemm(*d, cfg) for d in sets]
     streams = [torch.cuda.Stream() for _ in sets]
     torch.cuda.synchronize()

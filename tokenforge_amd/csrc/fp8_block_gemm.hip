@@ -1,6 +1,6 @@
 // Block-scaled e4m3 linear, many rows: BM x BN tiles through LDS.
 //
-// A workgroup of WM x WN waves streams 128-wide K blocks of x and the weight, and the rows' scales of
+// A group of WM x WN waves streams 128-wide K blocks of x and the weight, and the rows' scales of
 // the block, into S LDS stages by buffer->LDS loads issued up to S blocks ahead, one barrier a block.
 // A wave computes a (16 TM) x (16 TN) sub-tile: per block one v_mfma_scale_f32_16x16x128_f8f6f4
 // (unit MFMA scales) per 16 x 16 from a zero accumulator, then acc += (xs[m] * ws) * that in fp32.
@@ -15,6 +15,12 @@
 // covered by one block's MFMAs only. Of 9.25 rounds of tiles the last is a quarter full. The smaller
 // tiles serve fewer rows, where the weight's bytes bind: gate_up M = 48 29 us (4.8 TB/s) on 64 x 256.
 //
+// WK: K groups of a workgroup, each with waves and stages of its own over a share of the K blocks; the
+// sums of the others go to the first through LDS. For tiles so few that a CU has one: it then has WK times
+// the waves and loads in flight, and needs neither a second kernel nor partial sums in memory. Best of the
+// tiles with WK > 1 against best of those without, us on MI355X: 3584 x 3584 M = 48 9.4 (32 x 64, WK 4)
+// against 11.5, M = 333 15.6 (64 x 128, WK 2) against 21.5; 896 x 4864 M = 333 11.2 against 14.7.
+//
 // What did not help: w refilled half a block earlier behind a second barrier (602 us against 584), lines
 // asked for ahead into L2 (620 against 600), wave priorities (no change), bands of 4 or 16 rows (552, 568
 // against 553).
@@ -28,9 +34,9 @@ namespace {
 
 __device__ __forceinline__ int slot_xor(int row) { return ((row & 3) << 1) ^ ((row >> 2) & 1); }
 
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN, int S, int WK>
 struct Tile {
-  static constexpr int kWaves = WM * WN;
+  static constexpr int kWaves = WM * WN;  // of one K group
   static constexpr int TM = BM / WM / 16;
   static constexpr int TN = BN / WN / 16;
   static constexpr int kXBytes = BM * kBlockK;
@@ -42,9 +48,10 @@ struct Tile {
   static constexpr int kScaleSteps = BM / kScaleRows;
   static constexpr int kScaleRing = S <= 3 ? 2 : 4;
   static constexpr int kScaleBuf = BM * 16;
-  static constexpr int kLoop = S * kStage + kScaleRing * kScaleBuf + 256;
-  static constexpr int kOut = kWaves * 16 * (16 * TN * 4 + 16);  // the epilogue's transposition
-  static constexpr int kLds = kLoop > kOut ? kLoop : kOut;
+  static constexpr int kGroup = S * kStage + kScaleRing * kScaleBuf + 256;
+  static constexpr int kOut = kWaves * 16 * (16 * TN * 4 + 16);        // the epilogue's transposition
+  static constexpr int kSums = (WK - 1) * kWaves * TM * TN * 64 * 16;  // the other K groups' sums
+  static constexpr int kLds = WK * kGroup > kOut + kSums ? WK * kGroup : kOut + kSums;
   static constexpr int kXLoads = BM / 8 / kWaves;  // 1 KB loads per wave and stage
   static constexpr int kWLoads = BN / 8 / kWaves;
   static constexpr int kLoads = kXLoads + kWLoads + 1;
@@ -77,16 +84,18 @@ __device__ __forceinline__ void load16(__amdgpu_buffer_rsrc_t r, uint8_t* base, 
 
 // STREAM: the output, larger than the XCDs' L2s, goes past them and leaves them to the panels (gate_up M =
 // 4096 on MI355X: 548 us against 532).
-template <int BM, int BN, int WM, int WN, int S, bool STREAM>
-__global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, float* __restrict__ part, int split_k,
-                                                                  int tiles_m, int tiles_n) {
-  using C = Tile<BM, BN, WM, WN, S>;
+template <int BM, int BN, int WM, int WN, int S, int WK, bool STREAM>
+__global__ __launch_bounds__(64 * WM * WN * WK) void block_gemm_kernel(BlockArgs a, float* __restrict__ part,
+                                                                       int split_k, int tiles_m, int tiles_n) {
+  using C = Tile<BM, BN, WM, WN, S, WK>;
   constexpr int TM = C::TM, TN = C::TN;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  uint8_t* const s_lds = smem + S * C::kStage;
+  extern __shared__ __attribute__((aligned(16))) uint8_t all_smem[];
 
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave_of_all / C::kWaves, wave = wave_of_all % C::kWaves;
+  uint8_t* const smem = all_smem + group * C::kGroup;  // the group's stages
+  uint8_t* const s_lds = smem + S * C::kStage;
   const int wm = wave / WN, wn = wave % WN;
 
   // Tiles in bands of 8 tile rows, the rows of a band innermost: the 32 tiles an XCD has in flight
@@ -101,8 +110,12 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   const int m0 = (band * 8 + in_band % rows) * BM;
   const int n0 = (in_band / rows) * BN;
 
-  const int kb0 = (int)(((int64_t)z * a.nkb) / split_k);
-  const int kb1 = (int)(((int64_t)(z + 1) * a.nkb) / split_k);
+  // The slice's K blocks, and this group's share of them; every group takes as many steps as the longest.
+  const int slice0 = (int)(((int64_t)z * a.nkb) / split_k);
+  const int slice1 = (int)(((int64_t)(z + 1) * a.nkb) / split_k);
+  const int steps = (slice1 - slice0 + WK - 1) / WK;
+  const int kb0 = slice0 + group * steps;
+  const int kb1 = kb0 + steps < slice1 ? kb0 + steps : (kb0 < slice1 ? slice1 : kb0);
 
   const int mrows = a.m - m0 < BM ? a.m - m0 : BM;
   const int ncols = a.n - n0 < BN ? a.n - n0 : BN;
@@ -192,11 +205,12 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   int nb = (n0 + wn * TN * 16) >> 7;
   nb = nb <= ((a.n - 1) >> 7) ? nb : (a.n - 1) >> 7;
   const float* const wsp = a.ws + (int64_t)nb * a.ldws;
-  auto load_ws = [&](int kb) { return wsp[kb + lane < kb1 ? kb + lane : kb1 - 1]; };
+  const int kb_last = (kb1 <= a.nkb ? kb1 : a.nkb) - 1;  // a K group without a block may start past the last
+  auto load_ws = [&](int kb) { return wsp[kb + lane < kb1 ? kb + lane : kb_last]; };
   float ws64 = load_ws(kb0);
 
 #pragma unroll
-  for (int i = 0; i < C::kScaleSteps; ++i) issue_scales(0, i, true);
+  for (int i = 0; i < C::kScaleSteps; ++i) issue_scales(0, i, kb0 < kb1);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     mask_tail(kb0 + s);
@@ -226,7 +240,7 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   };
   xs[0] = scale(0, 0);
   int st = 0;
-  for (int kb = kb0; kb < kb1; ++kb) {
+  for (int kb = kb0; kb < kb0 + steps; ++kb) {
     const uint8_t* const stage = smem + st * C::kStage;
     const int next = st + 1 == S ? 0 : st + 1;
     const uint8_t* const stage2 = smem + next * C::kStage;
@@ -247,7 +261,8 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
         af[(i + 1) & 1] = frag(stage2, x_at, 0);
         xs[(i + 1) & 1] = scale(kb + 1 - kb0, 0);
       }
-      sc[i & 1] = xs[i & 1] * ws;
+      // Past a shorter group's last block the codes are zeros and the scales anything.
+      sc[i & 1] = WK == 1 || kb < kb1 ? xs[i & 1] * ws : 0.0f;
       constexpr int kLast = TM - 1;
       const int p = i == 0 ? kLast : i - 1;  // the step whose results are scaled here
 #pragma unroll
@@ -288,10 +303,26 @@ __global__ __launch_bounds__(64 * WM * WN) void block_gemm_kernel(BlockArgs a, f
   const int n_wave = n0 + wn * TN * 16;
   const int g4 = 4 * (lane >> 4);
   stage_barrier<0>();
+  if (WK > 1) {  // the groups' sums, added in group order
+    f4* const sums = reinterpret_cast<f4*>(all_smem + C::kOut) + wave * TM * TN * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < TM * TN; ++i)
+      if (group > 0) sums[((group - 1) * C::kWaves * TM * TN + i) * 64] = acc[i / TN][i % TN];
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int v = 0; v < WK - 1; ++v)
+#pragma unroll
+      for (int i = 0; i < TM * TN; ++i) {
+        const f4 p = sums[(v * C::kWaves * TM * TN + i) * 64];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[i / TN][i % TN][q] += p[q];
+      }
+  }
   if (wide) {
     constexpr int kCols = 16 * TN, kRow = kCols * 4 + 16;  // LDS row in bytes, padded off the banks of the next
     constexpr int kLanes = kCols / 8;                      // lanes per row, eight columns each
-    uint8_t* const mine = smem + wave * 16 * kRow;
+    uint8_t* const mine = all_smem + wave * 16 * kRow;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -366,20 +397,21 @@ __global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs a, const fl
   store_block4(a, (int)m, n, sum, runs_aligned(a));
 }
 
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN, int S, int WK>
 int launch(const BlockArgs& a, int split, float* part, hipStream_t stream) {
-  using C = Tile<BM, BN, WM, WN, S>;
+  using C = Tile<BM, BN, WM, WN, S, WK>;
   const int tiles_m = (int)cdiv(a.m, BM), tiles_n = (int)cdiv(a.n, BN);
   const int64_t grid = (int64_t)tiles_m * tiles_n * split;
   if (grid > 0x7FFFFFFF) return fail(TF_EINVAL, "tf_fp8_block_linear: too many tiles");
   constexpr bool kMayStream = BM == 256;  // the tile of large outputs
   const bool stream_out = kMayStream && split == 1 && (int64_t)a.m * a.n * 2 > (int64_t)kXcds * kL2Bytes;
-  auto kernel = stream_out ? block_gemm_kernel<BM, BN, WM, WN, S, kMayStream> : block_gemm_kernel<BM, BN, WM, WN, S, false>;
+  auto kernel =
+      stream_out ? block_gemm_kernel<BM, BN, WM, WN, S, WK, kMayStream> : block_gemm_kernel<BM, BN, WM, WN, S, WK, false>;
   if (C::kLds > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                           C::kLds) != hipSuccess)
     return fail(TF_ELAUNCH, "tf_fp8_block_linear: cannot reserve LDS");
-  kernel<<<(unsigned)grid, 64 * C::kWaves, C::kLds, stream>>>(a, part, split, tiles_m, tiles_n);
+  kernel<<<(unsigned)grid, 64 * C::kWaves * WK, C::kLds, stream>>>(a, part, split, tiles_m, tiles_n);
   if (int rc = check_launch("tf_fp8_block_linear(gemm)")) return rc;
   if (split == 1) return TF_OK;
   const int runs = (int)cdiv(a.n, 4);
@@ -393,10 +425,11 @@ struct Entry {
   int (*run)(const BlockArgs&, int, float*, hipStream_t);
 };
 
-#define TF_BLOCK(BM, BN, WM, WN, S) {BM, BN, WM * WN, S, launch<BM, BN, WM, WN, S>}
+#define TF_BLOCK(BM, BN, WM, WN, S, WK) {BM, BN, WM * WN * WK, S, launch<BM, BN, WM, WN, S, WK>}
 const Entry kEntries[] = {
-    TF_BLOCK(256, 256, 2, 4, 2), TF_BLOCK(128, 256, 2, 4, 3), TF_BLOCK(128, 128, 2, 4, 4), TF_BLOCK(64, 256, 2, 4, 3),
-    TF_BLOCK(64, 64, 2, 2, 4),   TF_BLOCK(32, 256, 1, 4, 4),  TF_BLOCK(32, 128, 1, 4, 4),
+    TF_BLOCK(256, 256, 2, 4, 2, 1), TF_BLOCK(128, 256, 2, 4, 3, 1), TF_BLOCK(128, 128, 2, 4, 4, 1),
+    TF_BLOCK(64, 256, 2, 4, 3, 1),  TF_BLOCK(64, 128, 2, 2, 3, 2),  TF_BLOCK(64, 64, 2, 2, 4, 2),
+    TF_BLOCK(32, 128, 1, 4, 4, 1),  TF_BLOCK(32, 64, 1, 2, 3, 4),
 };
 
 const Entry* find(const tf_gemm_config& cfg) {

@@ -1,20 +1,20 @@
 // Block-scaled e4m3 linear, few rows: weights straight from memory into the MFMA's registers.
 //
-// A workgroup owns 16 columns and TM tiles of up to 16 rows; its KS waves take every KS-th K block each, and their sums meet in LDS in
-// wave order. Per block of K = 128 a wave loads the 16 x 128 weight bytes (two 16-byte loads a lane,
+// A workgroup owns 16 columns and TM tiles of up to 16 rows; its KS waves take every KS-th K block each,
+// and their sums meet in LDS in wave order. Per block of K = 128 a wave loads the 16 x 128 weight bytes (two 16-byte loads a lane,
 // whole cache lines), D blocks ahead in a register ring, and runs one
 // v_mfma_scale_f32_16x16x128_f8f6f4 (unit MFMA scales) from a zero accumulator; then acc += (xs * ws) *
 // that in fp32. The weight fragment is the first operand, so a lane holds four consecutive columns
 // of one row of x.
 //
-// With few rows most of the MFMA's 16 are free: G = 16 / (rows, at least 16 / G) K blocks share one x fragment,
+// With few rows most of the MFMA's 16 are free: G K blocks share one x fragment (up to 16 / G rows),
 // lane c holding row c % (16 / G) of block c / (16 / G). The product with the weights of block j is
 // then right in the lanes of block j, and the others take the scale zero, so x and its scales cost one
 // load for G blocks; the lanes of a row are added at the end.
 //
 // Bound by the weight's bytes from a few MB on. On MI355X, weights from HBM: 37888 x 3584 M = 1 26.0 us
-// (5.2 TB/s, the card's copy rate), 3584 x 18944 15.8 us (4.3 TB/s: 224 workgroups), 4608 x 3584 7.4 us, of which
-// 3 us are a launch. G = 4 took the former from 31 to 29 us, loads that go through the caches from 29 to 26.
+// (5.2 TB/s, the card's copy rate), 3584 x 18944 15.8 us (4.3 TB/s: 224 workgroups), 4608 x 3584 7.4 us,
+// of which 3 us are a launch. G = 4 took the former from 31 to 29 us, loads that go through the caches from 29 to 26.
 #include "fp8_block.h"
 
 namespace tf {
