@@ -334,6 +334,24 @@ def test_linear_past_32_bit_offsets(m: int, n: int, k: int, device: torch.device
         bc.check_linear(y[rows][:, cols], inputs, f"{m}x{n}x{k} {cols}")
 
 
+@pytest.mark.parametrize("t", [(1 << 21) + 70, (1 << 26) + 5])
+def test_quantizers_of_more_rows_than_one_launch_takes(t: int, device: torch.device) -> None:
+    """A row's result is that of a call on few rows around it."""
+    g = torch.Generator(device=device).manual_seed(t)
+    x = torch.randn((t, 8), generator=g, device=device, dtype=torch.float16)
+    w = torch.rand(8, generator=g, device=device, dtype=torch.float16)
+    at = [slice(0, 40), slice((1 << 21) - 20, (1 << 21) + 20), slice(t - 40, t)]
+    for group in (128, 0):
+        calls = [lambda v: ops.fp8_quant(v, group), lambda v: ops.silu_mul_fp8_quant(v, group),
+                 lambda v: ops.add_rmsnorm_fp8_quant(v, v, w, 1e-6, group)]
+        for i, call in enumerate(calls):
+            got = call(x)
+            for s in at:
+                for a, b in zip(got, call(x[s])):
+                    assert torch.equal(a[s].view(torch.uint8), b.view(torch.uint8)), (i, group, s)
+            del got
+
+
 def test_empty_calls(device: torch.device) -> None:
     e8 = torch.empty((0, 256), dtype=torch.float8_e4m3fn, device=device)
     _, _, w8, ws = _to(device, bc.linear_inputs(1, 130, 256))

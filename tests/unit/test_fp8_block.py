@@ -165,6 +165,7 @@ def _entry(m: int = 4, n: int = 64, k: int = 256, cfg: tuple[int, ...] = (4, 16,
     ({"x": _X + 8}, b"16-byte"), ({"ldw": 264}, b"16-byte"), ({"cfg": (1, 16, 16, 128, 1, 8, 1)}, b"compiled config"),
     ({"cfg": (4, 48, 16, 128, 1, 8, 1)}, b"compiled"), ({"x": 0}, b"null pointer"),
     ({"cfg": (5, 256, 256, 64, 1, 8, 2)}, b"compiled"), ({"cfg": (5, 256, 256, 128, 0, 8, 2)}, b"compiled"),
+    ({"cfg": (5, 32, 64, 128, 1, 8, 3), "m": (1 << 31) - 1, "k": 16, "n": 64}, b"too many tiles"),
     ({"cfg": (5, 64, 64, 128, 2, 8, 4)}, b"workspace too small"),
     ({"cfg": (5, 64, 64, 128, 2, 8, 4), "ws": _WS + 8, "ws_bytes": 1 << 20}, b"16-byte"),
     ({"k": 1 << 22, "ldx": 1 << 22, "ldw": 1 << 22, "ldxs": 1 << 15, "ldws": 1 << 15}, b"apart"),

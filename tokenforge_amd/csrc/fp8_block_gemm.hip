@@ -402,7 +402,7 @@ int launch(const BlockArgs& a, int split, float* part, hipStream_t stream) {
   using C = Tile<BM, BN, WM, WN, S, WK>;
   const int tiles_m = (int)cdiv(a.m, BM), tiles_n = (int)cdiv(a.n, BN);
   const int64_t grid = (int64_t)tiles_m * tiles_n * split;
-  if (grid > 0x7FFFFFFF) return fail(TF_EINVAL, "tf_fp8_block_linear: too many tiles");
+  if (grid * (64 * C::kWaves * WK) > 0xFFFFFFFF) return fail(TF_EINVAL, "tf_fp8_block_linear: too many tiles");
   constexpr bool kMayStream = BM == 256;  // the tile of large outputs
   const bool stream_out = kMayStream && split == 1 && (int64_t)a.m * a.n * 2 > (int64_t)kXcds * kL2Bytes;
   auto kernel =

@@ -1,8 +1,8 @@
 // Block-scaled e4m3 linear, few rows: weights straight from memory into the MFMA's registers.
 //
 // A workgroup owns 16 columns and TM tiles of up to 16 rows; its KS waves take every KS-th K block each,
-// and their sums meet in LDS in wave order. Per block of K = 128 a wave loads the 16 x 128 weight bytes (two 16-byte loads a lane,
-// whole cache lines), D blocks ahead in a register ring, and runs one
+// and their sums meet in LDS in wave order. Per block of K = 128 a wave loads the 16 x 128 weight bytes
+// (two 16-byte loads a lane, whole cache lines), D blocks ahead in a register ring, and runs one
 // v_mfma_scale_f32_16x16x128_f8f6f4 (unit MFMA scales) from a zero accumulator; then acc += (xs * ws) *
 // that in fp32. The weight fragment is the first operand, so a lane holds four consecutive columns
 // of one row of x.
@@ -14,7 +14,8 @@
 //
 // Bound by the weight's bytes from a few MB on. On MI355X, weights from HBM: 37888 x 3584 M = 1 26.0 us
 // (5.2 TB/s, the card's copy rate), 3584 x 18944 15.8 us (4.3 TB/s: 224 workgroups), 4608 x 3584 7.4 us,
-// of which 3 us are a launch. G = 4 took the former from 31 to 29 us, loads that go through the caches from 29 to 26.
+// of which 3 us are a launch. G = 4 took the first from 31 to 29 us, loads that go through the caches
+// from 29 to 26.
 #include "fp8_block.h"
 
 namespace tf {
@@ -146,6 +147,7 @@ __global__ __launch_bounds__(64 * KS) void block_gemv_kernel(BlockArgs a) {
 
 template <int KS, int D, int G, int TM>
 int launch(const BlockArgs& a, hipStream_t stream) {
+  if (cdiv(a.n, 16) * (64 * KS) > 0xFFFFFFFF) return fail(TF_EINVAL, "tf_fp8_block_linear: too many columns");
   const dim3 grid((unsigned)cdiv(a.n, 16), (unsigned)cdiv(a.m, 16 / G * TM));
   block_gemv_kernel<KS, D, G, TM><<<grid, 64 * KS, 0, stream>>>(a);
   return check_launch("tf_fp8_block_linear(gemv)");

@@ -270,12 +270,24 @@ int run_rows(RowsArgs a, int32_t dtype, int32_t group_size, const char* name, hi
   const bool vec = a.k % 8 == 0 && a.ldx % 8 == 0 && multiple(a.x, 16) && multiple(a.q, 8) &&
                    (MODE != kNorm || multiple(a.w, 16)) &&
                    (!a.residual || (a.ldr % 8 == 0 && multiple(a.residual, 16) && multiple(a.hidden, 16)));
-  int rc;
-  if (dtype == TF_DTYPE_FP16)
-    rc = vec ? launch_vec<MODE, F16, true>(a, stream) : launch_vec<MODE, F16, false>(a, stream);
-  else
-    rc = vec ? launch_vec<MODE, BF16, true>(a, stream) : launch_vec<MODE, BF16, false>(a, stream);
-  return rc ? rc : check_launch(name);
+  // A launch takes fewer than 2^32 threads (2^21 rows of up to 1024, or 16 a block).
+  const int64_t all = a.t, rows = (int64_t(1) << 27) / a.blocks < (1 << 21) ? (int64_t(1) << 27) / a.blocks : 1 << 21;
+  for (int64_t t0 = 0; t0 < all; t0 += rows) {
+    RowsArgs b = a;
+    b.t = all - t0 < rows ? all - t0 : rows;
+    b.x = a.x + t0 * a.ldx;
+    b.residual = a.residual ? a.residual + t0 * a.ldr : nullptr;
+    b.hidden = a.hidden ? a.hidden + t0 * a.k : nullptr;
+    b.q = a.q + t0 * a.k;
+    b.scale = a.scale + t0 * (a.by_row ? 1 : a.blocks);
+    int rc;
+    if (dtype == TF_DTYPE_FP16)
+      rc = vec ? launch_vec<MODE, F16, true>(b, stream) : launch_vec<MODE, F16, false>(b, stream);
+    else
+      rc = vec ? launch_vec<MODE, BF16, true>(b, stream) : launch_vec<MODE, BF16, false>(b, stream);
+    if (rc || (rc = check_launch(name))) return rc;
+  }
+  return TF_OK;
 }
 
 }  // namespace
