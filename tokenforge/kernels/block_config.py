@@ -3,8 +3,9 @@
 A call's config follows from its M, N and K alone: of the compiled tiles and K splits, the one whose
 modelled time is least (up to four rows always the gemv form, by :func:`_one_tile`). The models'
 constants are fitted to measured times of every config on MI355X, weights read from HBM: 4560 layers and row
-counts (M 5 to 2500, weights of 16 KB to 136 MB), where the choice is 0.6% slower on average than the
-best compiled config (99 of 100 within 9%). There is no table of tuned layers.
+counts (M 5 to 2500, weights of 16 KB to 136 MB). There the choice is 0.6% slower on average than the
+best compiled config (99 of 100 within 9%); on others, 0.3% at M 2000 to 9000 and 0.8% at M 1 to 2500, of
+which 2.3% up to four rows. There is no table of tuned layers.
 """
 
 from __future__ import annotations
@@ -105,8 +106,8 @@ _GEMM = (
 )
 _GEMV = (
     _Gemv(5, 8, 8, 4, 4, 3.16, 0.116, 0.339, 5.63e6),
-    _Gemv(9, 256, 16, 4, 4, 3.09, 0.065, 0.489, 4.94e6),
-    _Gemv(17, 256, 32, 4, 2, 3.05, 0.000, 0.684, 2.90e6),
+    _Gemv(9, 300, 16, 4, 4, 3.09, 0.065, 0.489, 4.94e6),
+    _Gemv(17, 300, 32, 4, 2, 3.05, 0.000, 0.684, 2.90e6),
 )
 _ONE_TILES = ((4, 8, 4), (4, 4, 4))
 """(block_m, num_warps, num_stages) of the gemv form up to four rows."""
