@@ -199,6 +199,16 @@ def test_quantizer_entries_refuse_on_the_host() -> None:
     assert h.tf_fp8_quant(_X, 128, 0, _O, _S, 0, 128, 128, None) == _lib.TF_OK  # no rows, no launch
 
 
+@pytest.mark.parametrize("k", [0, -1, 5 - (1 << 32), -(1 << 62)])
+def test_quantizer_entries_refuse_lengths_below_one(k: int) -> None:
+    """Negative lengths whose low 32 bits are a positive number too (no rows: nothing is launched either way)."""
+    h = _lib.lib()
+    for rc in (h.tf_fp8_quant(_X, 128, 0, _O, _S, 0, k, 128, None),
+               h.tf_silu_mul_fp8_quant(_X, 256, 0, _O, _S, 0, k, 128, None),
+               h.tf_add_rmsnorm_fp8_quant(_X, 128, None, 0, _W, 0, _O, _S, None, 0, k, EPS, 128, None)):
+        assert rc == _lib.TF_EINVAL and b"k > 0" in h.tf_last_error()
+
+
 # ----------------------------------------------------------------------------- fakes and the launch rule
 
 

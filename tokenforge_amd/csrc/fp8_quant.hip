@@ -249,6 +249,13 @@ int launch_vec(const RowsArgs& a, hipStream_t stream) {
   return TF_OK;
 }
 
+// A row's length, before it is held in 32 bits.
+int check_length(int64_t k, const char* name) {
+  if (k <= 0) return fail(TF_EINVAL, std::string(name) + ": need k > 0");
+  if (k > 0x3FFFFFFF) return fail(TF_EINVAL, std::string(name) + ": row too long");
+  return TF_OK;
+}
+
 bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 template <int MODE>
@@ -256,7 +263,7 @@ int run_rows(RowsArgs a, int32_t dtype, int32_t group_size, const char* name, hi
   const std::string who(name);
   if (dtype != TF_DTYPE_FP16 && dtype != TF_DTYPE_BF16) return fail(TF_EINVAL, who + ": unknown dtype");
   if (!a.x || !a.q || !a.scale) return fail(TF_EINVAL, who + ": null pointer");
-  if (a.t < 0 || a.k <= 0) return fail(TF_EINVAL, who + ": need t >= 0 and k > 0");
+  if (a.t < 0) return fail(TF_EINVAL, who + ": need t >= 0");
   if (group_size != 0 && group_size != 128)
     return fail(TF_EINVAL, who + ": group_size must be 128, or 0 for one scale per row");
   if (a.ldx < (MODE == kSilu ? 2 : 1) * (int64_t)a.k || (a.residual && a.ldr < a.k))
@@ -297,7 +304,7 @@ using namespace tf;
 
 extern "C" int tf_fp8_quant(const uint16_t* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale, int64_t t,
                             int64_t k, int32_t group_size, void* stream) {
-  if (k > 0x3FFFFFFF) return fail(TF_EINVAL, "tf_fp8_quant: row too long");
+  if (int rc = check_length(k, "tf_fp8_quant")) return rc;
   RowsArgs a{};
   a.x = x, a.ldx = ldx, a.q = q, a.scale = scale, a.t = t, a.k = (int)k;
   return run_rows<kQuant>(a, dtype, group_size, "tf_fp8_quant", (hipStream_t)stream);
@@ -305,7 +312,7 @@ extern "C" int tf_fp8_quant(const uint16_t* x, int64_t ldx, int32_t dtype, uint8
 
 extern "C" int tf_silu_mul_fp8_quant(const uint16_t* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale,
                                      int64_t t, int64_t k, int32_t group_size, void* stream) {
-  if (k > 0x3FFFFFFF) return fail(TF_EINVAL, "tf_silu_mul_fp8_quant: row too long");
+  if (int rc = check_length(k, "tf_silu_mul_fp8_quant")) return rc;
   RowsArgs a{};
   a.x = x, a.ldx = ldx, a.q = q, a.scale = scale, a.t = t, a.k = (int)k;
   return run_rows<kSilu>(a, dtype, group_size, "tf_silu_mul_fp8_quant", (hipStream_t)stream);
@@ -315,10 +322,10 @@ extern "C" int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t ldx, const ui
                                         const uint16_t* weight, int32_t dtype, uint8_t* q, float* scale,
                                         uint16_t* hidden, int64_t t, int64_t k, float eps, int32_t group_size,
                                         void* stream) {
-  if (k > 0x3FFFFFFF) return fail(TF_EINVAL, "tf_add_rmsnorm_fp8_quant: row too long");
+  if (int rc = check_length(k, "tf_add_rmsnorm_fp8_quant")) return rc;
   if (!weight || (residual && !hidden)) return fail(TF_EINVAL, "tf_add_rmsnorm_fp8_quant: null pointer");
   RowsArgs a{};
   a.x = x, a.ldx = ldx, a.residual = residual, a.ldr = ldr, a.w = weight, a.hidden = hidden;
-  a.q = q, a.scale = scale, a.t = t, a.k = (int)k, a.eps = eps, a.inv_k = k > 0 ? 1.0f / (float)k : 0.0f;
+  a.q = q, a.scale = scale, a.t = t, a.k = (int)k, a.eps = eps, a.inv_k = 1.0f / (float)k;
   return run_rows<kNorm>(a, dtype, group_size, "tf_add_rmsnorm_fp8_quant", (hipStream_t)stream);
 }
