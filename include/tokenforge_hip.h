@@ -319,10 +319,11 @@ int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t ldx, const uint16_t* res
  * x8 [m, k] and weight [n, k]: e4m3fn codes, 16-byte aligned rows (strides ldx8, ldw in bytes);
  * xscale fp32 [m, ceil(k/128)] and wscale fp32 [ceil(n/128), ceil(k/128)] (strides in elements);
  * bias [n], residual [m, n] (stride ldr) or NULL and out [m, n] (stride ldo) of type `dtype`. k a
- * multiple of 16; n and m any; code rows less than 4 MiB apart, rows of xscale less than 2^20 elements. A block's products are summed by the MFMA, the blocks in fp32, and
- * bias and residual are added in fp32 before the one rounding. cfg: one of the compiled configs
- * (block_k 128; else TF_EINVAL); workspace: fp32, 16-byte aligned, >= tf_fp8_block_workspace_bytes
- * (-1 for an unknown config). */
+ * multiple of 16; code rows less than 4 MiB apart, rows of xscale less than 2^20 elements. A block's
+ * products are summed by the MFMA, the blocks in fp32, and bias and residual are added in fp32 before
+ * the one rounding. cfg: one of the compiled configs (block_k 128; else TF_EINVAL); workspace: fp32,
+ * 16-byte aligned, >= tf_fp8_block_workspace_bytes (-1 for an unknown config, for sizes the linear
+ * refuses and for partial sums of 2^63 bytes). */
 int64_t tf_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k, const tf_gemm_config* cfg);
 int tf_fp8_block_linear(const uint8_t* x8, int64_t ldx8, const float* xscale, int64_t ldxs,
                         const uint8_t* weight, int64_t ldw, const float* wscale, int64_t ldws,

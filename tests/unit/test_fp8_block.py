@@ -209,6 +209,20 @@ def test_quantizer_entries_refuse_lengths_below_one(k: int) -> None:
         assert rc == _lib.TF_EINVAL and b"k > 0" in h.tf_last_error()
 
 
+def test_workspace_bytes_never_wrap() -> None:
+    """The partial sums' bytes, or -1 where they pass 63 bits or a size is one the linear refuses."""
+    top = (1 << 31) - 1
+    for split in (1, 2, 5, 16):
+        cfg = ctypes.byref(_lib.TfGemmConfig(5, 64, 64, 128, split, 8, 4))
+        for m in (0, 1, 1000, 1 << 28, 1 << 30, top, top + 1, 1 << 40, -1):
+            for n in (0, 1, 1000, 1 << 30, 0x7FFFFF00, 0x7FFFFF01, 1 << 40, -1):
+                for k in (16, 4096, 0x7FFFFF00, (1 << 63) - 1):
+                    got = _lib.lib().tf_fp8_block_workspace_bytes(m, n, k, cfg)
+                    bytes_ = 4 * m * n * min(split, -(-k // 128)) if min(split, -(-k // 128)) > 1 else 0
+                    known = 0 <= m <= top and 0 <= n <= 0x7FFFFF00 and k <= 0x7FFFFF00 and bytes_ < 1 << 63
+                    assert got == (bytes_ if known else -1), (m, n, k, split)
+
+
 # ----------------------------------------------------------------------------- fakes and the launch rule
 
 
