@@ -12,6 +12,7 @@ import torch
 import tokenforge.kernels.ops  # noqa: F401
 from oracle import fp8_block as oblk
 from tests.numerics import block_cases as bc
+from tests.numerics import block_codes
 from tokenforge.kernels import _lib
 from tokenforge.kernels.block_config import BLOCK_TILES, block_config
 from tokenforge.kernels.hip import fp8_block
@@ -43,6 +44,13 @@ def test_host_quantizers(t: int, k: int, group: int, dtype: torch.dtype) -> None
     y = oblk.rmsnorm((x + r).double().numpy(), w.double().numpy(), EPS)
     bc.check_codes(q, s, y, (k / 2 + 8) * bc.U32, group, "norm")
     assert ops.add_rmsnorm_fp8_quant(x, None, w, EPS, group)[2].shape == (0,)
+
+
+@pytest.mark.parametrize("group", [128, 0])
+@pytest.mark.parametrize("k", [128, 130])
+def test_host_silu_mul_of_gates_far_below_zero(k: int, group: int) -> None:
+    x = block_codes.far_gates(k)
+    block_codes.check_far_gates(*ops.silu_mul_fp8_quant(x, group), x, group)
 
 
 @pytest.mark.parametrize("dtype", bc.DTYPES, ids=str)

@@ -245,10 +245,14 @@ def block_quant(y: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.T
 
 
 def silu_mul_block_quant(x: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """:func:`block_quant` of ``silu(x[:, :K]) * x[:, K:]`` in fp32."""
+    """:func:`block_quant` of ``silu(x[:, :K]) * x[:, K:]`` in fp32. Below a gate of -80, where ``1 +
+    exp(-gate)`` nears fp32's end and the 1 is lost in it, as ``gate e^(gate/2) up e^(gate/2)``: a bf16
+    ``up`` can be large enough for the product to count."""
     xf = x.to(torch.float32)
     gate, up = xf.chunk(2, dim=-1)
-    return block_quant(torch.nn.functional.silu(gate) * up, group_size)
+    root = torch.exp(gate * 0.5)
+    y = torch.where(gate < -80.0, gate * root * up * root, torch.nn.functional.silu(gate) * up)
+    return block_quant(y, group_size)
 
 
 def add_rmsnorm_block_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float,

@@ -35,11 +35,36 @@ struct RowsArgs {
 };
 
 // silu(g) * u = g / (1 + 2^(-g log2 e)) * u through v_exp_f32 and v_rcp_f32 (an ulp each): within
-// (7 + |g|) 2^-24 of the exact value, where an IEEE division and expf cost three times the instructions
-// (2048 x 18944 on MI355X: 48 us against 43). g = -inf gives NaN, as the expression does.
+// (7 + 1.23 |g|) 2^-24 of the exact value (the argument is rounded, and the constant off by 0.23 2^-24),
+// where an IEEE division and expf cost three times the instructions (2048 x 18944 on MI355X: 48 us against
+// 43). g = -inf gives NaN, as the expression does.
+//
+// From g = -87.3 down its denominator passes 2^126 and the reciprocal fp32's normal range: silu_far8.
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float e = __builtin_amdgcn_exp2f(g * -1.44269504f);
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+
+// y = silu(g) * u again where g < -80, of a lane's eight bf16 gates and values: an `up` of bf16's size (to
+// 3.4e38; fp16 ends at 65504) brings a gate's sigmoid of down to e^-112 back above the smallest scale. There
+// the 1 is below 2^-115 of 1 + e^-g, and g e^(g/2) u e^(g/2) stays in range, within the bound above.
+// Taken behind one comparison of the eight (negative bf16 order as their bits; below -80.0 = 0xC2A0): as a
+// selection in silu_mul it cost every call 11% (2048 x 18944 on MI355X 42.5 us against 38.3).
+__device__ __forceinline__ void silu_far8(const u4& gates, const u4& ups, float (&y)[8]) {
+  us2 m = __builtin_bit_cast(us2, gates[0]);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, gates[j]));
+  if (m[0] <= 0xC2A0u && m[1] <= 0xC2A0u) return;
+  float g[8], u[8];
+  unpack8<BF16>(gates, g);
+  unpack8<BF16>(ups, u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float e = __builtin_amdgcn_exp2f(g[j] * 0.72134752f);
+    if (g[j] < -80.0f) y[j] = g[j] * e * u[j] * e;
+  }
 }
 
 // Eight elements of a row at e0 (zeros past k). VEC: one 16-byte load (k % 8 == 0, aligned rows).
@@ -102,6 +127,7 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(RowsArgs a) {
       unpack8<T>(w[i], u);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = silu_mul(y[j], u[j]);
+      if (T::kWide) silu_far8(v[i], w[i], y);
     }
     const uint32_t amax = max16_u32(absmax8(y));
     const float s = dynamic_scale(as_f32(amax));
@@ -177,6 +203,7 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(RowsArgs a) {
     unpack8<T>(w[i], u);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = MODE == kSilu ? silu_mul(y[j], u[j]) : y[j] * rstd * u[j];
+    if (MODE == kSilu && T::kWide) silu_far8(v[i], w[i], y);
     if (MODE == kNorm) {
       // Past k the loads are zeros, and 0 * rstd is NaN where rstd is not finite.
       const int e0 = (tid + i * threads) * 8;
@@ -186,12 +213,12 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(RowsArgs a) {
   };
   uint8_t* const q = a.q + row * a.k;
   if (a.by_row) {
+    float y[CPT][8];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
-      float y[8];
-      values(i, y);
-      m = __builtin_elementwise_max(m, absmax8(y));
+      values(i, y[i]);
+      m = __builtin_elementwise_max(m, absmax8(y[i]));
     }
     m = wave_max_u32(m);
     if ((tid & 63) == 0) red[wave] = m;
@@ -200,11 +227,7 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(RowsArgs a) {
     const float s = dynamic_scale(as_f32(m));
     if (tid == 0) a.scale[row] = s;
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      float y[8];
-      values(i, y);
-      store8<VEC>(q, (tid + i * threads) * 8, a.k, encode8(y, s, m));
-    }
+    for (int i = 0; i < CPT; ++i) store8<VEC>(q, (tid + i * threads) * 8, a.k, encode8(y[i], s, m));
     return;
   }
 #pragma unroll

@@ -12,12 +12,14 @@
 namespace tf {
 
 struct F16 {  // IEEE binary16
+  static constexpr bool kWide = false;  // fp32's exponent range
   static __device__ __forceinline__ float lo(uint32_t pair) { return (float)as_h2(pair)[0]; }
   static __device__ __forceinline__ float hi(uint32_t pair) { return (float)as_h2(pair)[1]; }
   static __device__ __forceinline__ uint32_t round(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 };
 
 struct BF16 {  // the upper half of an fp32
+  static constexpr bool kWide = true;
   static __device__ __forceinline__ float lo(uint32_t pair) { return as_f32(pair << 16); }
   static __device__ __forceinline__ float hi(uint32_t pair) { return as_f32(pair & 0xFFFF0000u); }
   static __device__ __forceinline__ uint32_t round(float v) {  // to nearest, ties to even; NaN kept
