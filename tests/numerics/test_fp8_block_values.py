@@ -1,4 +1,9 @@
-"""FP8 with a scale per 128 on the GPU, further values: gates whose sigmoid leaves fp32's normal range."""
+"""FP8 with a scale per 128 on the GPU, further values: gates whose sigmoid leaves fp32's normal range; codes
+that have to be numbers at every size and layout.
+
+The norm's error: hidden squared, a tree of three and one of six levels, up to 64 sums of those in order, 1 / k,
+its product and eps are 1 + 3 + 6 + 64 + 3 roundings of the mean, half as many of its root; root, quotient and
+two products are four more: 43 roundings of 2^-24."""
 
 from __future__ import annotations
 
@@ -6,10 +11,14 @@ import pytest
 import torch
 
 import tokenforge.kernels.ops  # noqa: F401  (registers torch.ops.tokenforge)
+from oracle import fp8_block as oblk
+from tests.numerics import block_cases as bc
 from tests.numerics import block_codes
 
 pytestmark = pytest.mark.gpu
 ops = torch.ops.tokenforge
+EPS = 1e-6
+NORM_ERR = 43 * bc.U32
 
 
 @pytest.mark.parametrize("group", [128, 0])
@@ -17,3 +26,22 @@ ops = torch.ops.tokenforge
 def test_silu_mul_of_gates_far_below_zero(k: int, group: int, device: torch.device) -> None:
     x = block_codes.far_gates(k)
     block_codes.check_far_gates(*ops.silu_mul_fp8_quant(x.to(device), group), x, group)
+
+
+@pytest.mark.parametrize("dtype", bc.DTYPES, ids=str)
+@pytest.mark.parametrize("group", [128, 0])
+@pytest.mark.parametrize(("t", "k"), [(1, 1), (4, 7), (3, 130), (2, 1000), (17, 1296), (129, 264), (1030, 896), (1, 8200),
+                                      (2, 18944), (1, 32767), (1, 32768)])
+def test_codes_are_numbers(t: int, k: int, group: int, dtype: torch.dtype, device: torch.device) -> None:
+    """Every code of every producer, the last ones of a ragged row and of each lane among them."""
+    x, r, gu = (bc.rows(t, n, dtype, seed) for n, seed in ((k, 30), (k, 31), (2 * k, 32)))
+    w = (torch.rand((k,), generator=bc.gen("w", k)) + 0.5).to(dtype)
+    q, s = ops.fp8_quant(x.to(device), group)
+    block_codes.check_codes(q, s, x.double().numpy(), 0.0, group, "fp8_quant")
+    q, s = ops.silu_mul_fp8_quant(gu.to(device), group)
+    block_codes.check_codes(q, s, oblk.silu_mul(gu.double().numpy()), block_codes.silu_err(gu), group, "silu")
+    for res in (None, r):
+        q, s, _ = ops.add_rmsnorm_fp8_quant(x.to(device), None if res is None else res.to(device), w.to(device), EPS,
+                                            group)
+        y = oblk.rmsnorm((x if res is None else x + res).double().numpy(), w.double().numpy(), EPS)
+        block_codes.check_codes(q, s, y, NORM_ERR, group, "norm")

@@ -281,6 +281,33 @@ def test_oracle_linear_against_scalar_loops() -> None:
         assert abs(float(sum(t * t for t in terms)) ** 0.5 - length[m, n]) <= 144 * 2.0**-52 * length[m, n]
 
 
+@pytest.mark.parametrize("group", [128, 0])
+def test_code_check_refuses_wrong_codes_and_scales(group: int) -> None:
+    """The check itself: right codes pass; a NaN code, a code one step off, a sign and a wrong scale do not."""
+    x = bc.rows(5, 260, torch.float16, seed=40)
+    y = x.double().numpy()
+    q, s = ops.fp8_quant(x, group)
+    block_codes.check_codes(q, s, y, 0.0, group, "right")
+    at = [int(i) for i in np.unravel_index(np.abs(bc.codes(q) & 0x7F).argmax(), q.shape)]
+
+    def planted(code: int) -> torch.Tensor:
+        out = q.view(torch.uint8).clone()
+        out[at[0], at[1]] = code
+        return out.view(F8)
+
+    right = int(bc.codes(q)[at[0], at[1]])
+    for code in (0x7F, 0xFF, right - 1, right ^ 0x80, 0):
+        with pytest.raises(AssertionError):
+            block_codes.check_codes(planted(code), s, y, 0.0, group, "planted")
+    with pytest.raises(AssertionError):  # every code
+        block_codes.check_codes(torch.full(q.shape, 0x7F, dtype=torch.uint8).view(F8), s, y, 0.0, group, "planted")
+    for wrong in (float("nan"), float("inf"), 0.0, float(s[at[0], 0]) * (1 + 2.0**-20)):
+        t = s.clone()
+        t[at[0], 0] = wrong
+        with pytest.raises(AssertionError):
+            block_codes.check_codes(q, t, y, 0.0, group, "planted")
+
+
 def test_oracle_half_step_and_scales() -> None:
     values = np.sort(np.unique(np.abs(torch.arange(0, 127, dtype=torch.uint8).view(F8).float().numpy()))).astype(np.float64)
     for lo, hi in zip(values[:-1], values[1:]):
