@@ -319,8 +319,9 @@ int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t ldx, const uint16_t* res
  * x8 [m, k] and weight [n, k]: e4m3fn codes, 16-byte aligned rows (strides ldx8, ldw in bytes);
  * xscale fp32 [m, ceil(k/128)] and wscale fp32 [ceil(n/128), ceil(k/128)] (strides in elements);
  * bias [n], residual [m, n] (stride ldr) or NULL and out [m, n] (stride ldo) of type `dtype`. k a
- * multiple of 16; code rows less than 4 MiB apart, rows of xscale less than 2^20 elements. A block's
- * products are summed by the MFMA, the blocks in fp32, and bias and residual are added in fp32 before
+ * multiple of 16; code rows less than 4 MiB apart, rows of xscale less than 2^20 elements; m, n and a
+ * config whose launch stays below 2^32 threads (n below 2^27 for the GEMV of eight waves; else TF_EINVAL). A
+ * block's products are summed by the MFMA, the blocks in fp32, and bias and residual are added in fp32 before
  * the one rounding. cfg: one of the compiled configs (block_k 128; else TF_EINVAL); workspace: fp32,
  * 16-byte aligned, >= tf_fp8_block_workspace_bytes (-1 for an unknown config, for sizes the linear
  * refuses and for partial sums of 2^63 bytes). */

@@ -1,5 +1,5 @@
-"""FP8 with a scale per 128 on the GPU, further values: gates whose sigmoid leaves fp32's normal range; codes
-that have to be numbers at every size and layout.
+"""FP8 with a scale per 128 on the GPU, further values and sizes: gates whose sigmoid leaves fp32's normal range;
+codes that have to be numbers at every size; linears too long or wide for their usual launch.
 
 The norm's error: hidden squared, a tree of three and one of six levels, up to 64 sums of those in order, 1 / k,
 its product and eps are 1 + 3 + 6 + 64 + 3 roundings of the mean, half as many of its root; root, quotient and
@@ -45,3 +45,22 @@ def test_codes_are_numbers(t: int, k: int, group: int, dtype: torch.dtype, devic
                                             group)
         y = oblk.rmsnorm((x if res is None else x + res).double().numpy(), w.double().numpy(), EPS)
         block_codes.check_codes(q, s, y, NORM_ERR, group, "norm")
+
+
+@pytest.mark.parametrize(("m", "n"), [(3, 300_000_000), ((1 << 30) + 5, 1)])
+def test_linear_too_large_for_its_usual_launch(m: int, n: int, device: torch.device) -> None:
+    """Where the gemv form, or the tile the time model prefers, would take 2^32 threads: outputs of the first,
+    middle and last rows or columns. (The codes have one sign. With two groups of eight the cuts of either, 7 of
+    2^-13 of its largest product, are within ``linear_bound``'s 7 sqrt(7) 2^-13 of the length all the same.)"""
+    g = torch.Generator(device=device).manual_seed(m)
+    x8, w8 = (torch.randint(0, 0x7F, (r, 16), generator=g, device=device, dtype=torch.uint8).view(torch.float8_e4m3fn)
+              for r in (m, n))
+    xs = torch.rand((m, 1), generator=g, device=device) * 1e-2
+    ws = torch.rand((-(-n // 128), 1), generator=g, device=device) * 1e-3
+    y = ops.fp8_block_linear(x8, xs, w8, ws, None, torch.bfloat16, "hip")
+    assert y.shape == (m, n)
+    for r0 in sorted({0, m // 2, max(0, m - 40)}):
+        for c0 in sorted({0, n // 256 * 128, (n - 1) // 128 * 128}):
+            r, c = slice(r0, min(m, r0 + 40)), slice(c0, min(n, c0 + 128))
+            inputs = (x8[r].cpu(), xs[r].cpu(), w8[c].cpu(), ws[c0 // 128:c0 // 128 + 1].cpu())
+            bc.check_linear(y[r, c], inputs, f"{m}x{n} at {r0}, {c0}")

@@ -262,6 +262,17 @@ def test_the_rule_names_compiled_configs() -> None:
             assert fp8_block.workspace_bytes(m, n, k, cfg) >= 0
 
 
+def test_the_rule_stays_within_one_launch() -> None:
+    """Every call that some compiled config can launch (fewer than 2^32 threads) gets one that can."""
+    for m, n, k in ((1, 300_000_000, 16), (4, 300_000_000, 16), (2, 150_000_000, 2048), (16, 300_000_000, 16),
+                    (300, 140_000_000, 16), (1, 0x7FFFFF00, 16), (1 << 30, 1, 16), ((1 << 30) + 5, 1, 16),
+                    (280_000_000, 16, 16), (0x7FFFFF00, 1, 16)):
+        c = block_config(m, n, k)
+        gemv = c.kernel == "gemv_block"  # rows on the grid's second axis
+        groups = (1 if gemv else -(-m // c.block_m)) * -(-n // c.block_n) * c.split_k
+        assert groups * 64 * c.num_warps < 1 << 32, (m, n, k, c)
+
+
 # ----------------------------------------------------------------------------- the oracle
 
 

@@ -114,6 +114,8 @@ _ONE_TILES = ((4, 8, 4), (4, 4, 4))
 _SPLITS = (1, 2, 3, 4, 6, 8, 12, 16)
 _MAX_SPLIT_GROUPS = 700
 """Workgroups up to which K is split: past that the chip is full."""
+_MAX_THREADS = 0xFFFFFFFF
+"""Of one launch."""
 
 BLOCK_TILES: tuple[tuple[str, int, int, int, int], ...] = tuple(
     [("gemv_block", rows, 16, waves, stages) for rows, waves, stages in _ONE_TILES]
@@ -136,13 +138,13 @@ def _one_tile(k: int) -> tuple[int, int, int]:
 @functools.lru_cache(maxsize=4096)
 def block_config(m: int, n: int, k: int) -> BlockConfig:
     """The launch of an M x N x K call."""
-    if m <= 4:
-        rows, waves, stages = _one_tile(k)
+    rows, waves, stages = _one_tile(k)
+    if m <= 4 and -(-n // 16) * 64 * waves <= _MAX_THREADS:
         return BlockConfig("gemv_block", rows, 16, 1, waves, stages)
     nkb = _blocks(k)
     best: tuple[float, BlockConfig] | None = None
     for v in _GEMV:
-        if v.fewest <= m <= v.most:
+        if v.fewest <= m <= v.most and -(-n // 16) * 64 * v.num_warps <= _MAX_THREADS:
             us = v.us(m, n, k)
             if best is None or us < best[0]:
                 best = us, BlockConfig("gemv_block", v.block_m, 16, 1, v.num_warps, v.num_stages)
@@ -150,6 +152,9 @@ def block_config(m: int, n: int, k: int) -> BlockConfig:
         tiles = -(-m // t.block_m) * -(-n // t.block_n)
         for split in _SPLITS:
             if split > 1 and (split > nkb // 2 or tiles > NUM_CUS or tiles * split > _MAX_SPLIT_GROUPS):
+                break
+            # The first tile, the largest, takes the fewest threads: where it takes too many, all do.
+            if best is not None and tiles * split * 64 * t.num_warps > _MAX_THREADS:
                 break
             us = t.us(m, n, k, split)
             if best is None or us < best[0]:
