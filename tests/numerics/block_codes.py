@@ -48,3 +48,68 @@ def check_far_gates(q: torch.Tensor, s: torch.Tensor, x: torch.Tensor, group: in
     largest = np.abs(e4m3_decode(bc.codes(q))).max(axis=1)
     # Rows 0 to 6 (gates down to -100) have scales above the smallest one, rows 7 to 9 codes at the smallest.
     assert (largest[:7] == 448).all() and (largest[7:10] > 0).all() and largest[19] == 0
+
+
+# ----------------------------------------------------------------------------- what the matrix instruction cuts
+
+GROUP = 8
+"""Consecutive k whose products the matrix instruction adds in one window."""
+
+
+def cut_bound(x8: torch.Tensor, xs: torch.Tensor, w8: torch.Tensor, ws: torch.Tensor) -> np.ndarray:
+    """How much the cuts of products can take from each output, whatever their signs: a product loses less than
+    2^-13 of the power of two below the largest of its group of eight consecutive k, and the largest nothing."""
+    n, k = w8.shape
+    x, w = np.abs(e4m3_decode(bc.codes(x8)).astype(np.float64)), np.abs(e4m3_decode(bc.codes(w8)).astype(np.float64))
+    scales = np.repeat(ws.double().numpy(), oblk.BLOCK, axis=0)[:n]
+    total = np.zeros((x.shape[0], n))
+    for k0 in range(0, k, GROUP):
+        peak = (x[:, None, k0:k0 + GROUP] * w[None, :, k0:k0 + GROUP]).max(axis=2)
+        unit = np.where(peak > 0, np.exp2(np.floor(np.log2(np.where(peak > 0, peak, 1.0))) - 13), 0.0)
+        total += (GROUP - 1) * unit * xs.double().numpy()[:, k0 // 128, None] * scales[None, :, k0 // 128]
+    return total
+
+
+def hard_inputs(kind: str, m: int, n: int, k: int) -> tuple[torch.Tensor, ...]:
+    """Operands of a linear whose products differ much in size inside a group of eight.
+
+    ``outliers``: one channel of x in eight is 20 times the others, as hidden states have them. ``one sign``:
+    the same without signs, so that every cut has one sign too. ``cancelling``: in each group two products of
+    up to 2^17 that cancel, and six of one sign and about 2^3, which are all that is left of the sum."""
+    g = bc.gen(kind, m, n, k)
+    x, w = torch.randn((m, k), generator=g) * 7, torch.randn((n, k), generator=g) * 100
+    x[:, ::GROUP] *= 20
+    if kind == "one sign":
+        x, w = x.abs(), w.abs()
+    if kind == "cancelling":
+        x, w = 2 + torch.rand((m, k), generator=g), 2 + 2 * torch.rand((n, k), generator=g)
+        x[:, 0::GROUP] = x[:, 1::GROUP] = 448
+        w[:, 0::GROUP] = 100 + 300 * torch.rand(w[:, 0::GROUP].shape, generator=g)
+        w[:, 1::GROUP] = -w[:, 0::GROUP]
+    nkb, nnb = -(-k // 128), -(-n // 128)
+    xs = torch.exp2(torch.rand((m, nkb), generator=g) - 10)
+    ws = torch.exp2(torch.rand((nnb, nkb), generator=g) - 12)
+    f8 = torch.float8_e4m3fn
+    return x.clamp(-448, 448).to(f8), xs, w.clamp(-448, 448).to(f8), ws
+
+
+def remainder_residual(inputs: tuple[torch.Tensor, ...]) -> torch.Tensor:
+    """The fp16 residual that leaves of a linear's outputs what their own rounding would hide."""
+    x8, xs, w8, ws = inputs
+    y = oblk.linear(bc.codes(x8), xs.numpy(), bc.codes(w8), ws.numpy())[0]
+    assert np.abs(y).max() < 60000
+    return torch.from_numpy(-y).to(torch.float16)
+
+
+def check_remainder(out: torch.Tensor, inputs: tuple[torch.Tensor, ...], residual: torch.Tensor, what: str) -> None:
+    """``out`` = the linear plus :func:`remainder_residual`: off by the cuts, the fp32 additions (a relative
+    2^-23 of the sum of magnitudes each: sixteen groups, the blocks, two of scales, the residual's) and half
+    an fp16 step of what is left."""
+    x8, xs, w8, ws = inputs
+    y, size, _ = oblk.linear(bc.codes(x8), xs.numpy(), bc.codes(w8), ws.numpy())
+    r = residual.double().numpy()
+    additions = 16 + -(-x8.shape[1] // 128) + 3
+    carried = cut_bound(*inputs) + additions * 2 * bc.U32 * (size + np.abs(r))
+    bound = carried + bc.HALF_STEP[torch.float16] * (np.abs(y + r) + carried) + 2.0**-25
+    off = np.abs(out.detach().cpu().double().numpy() - (y + r))
+    assert (off <= bound).all(), f"{what}: {int((~(off <= bound)).sum())} off, by up to {(off - bound).max():.3e} too much"

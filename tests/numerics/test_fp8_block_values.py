@@ -1,5 +1,6 @@
 """FP8 with a scale per 128 on the GPU, further values and sizes: gates whose sigmoid leaves fp32's normal range;
-codes that have to be numbers at every size; linears too long or wide for their usual launch.
+codes that have to be numbers at every size; linears too long or wide for their usual launch; linears whose
+products differ so much in size that the matrix instruction cuts some.
 
 The norm's error: hidden squared, a tree of three and one of six levels, up to 64 sums of those in order, 1 / k,
 its product and eps are 1 + 3 + 6 + 64 + 3 roundings of the mean, half as many of its root; root, quotient and
@@ -14,6 +15,8 @@ import tokenforge.kernels.ops  # noqa: F401  (registers torch.ops.tokenforge)
 from oracle import fp8_block as oblk
 from tests.numerics import block_cases as bc
 from tests.numerics import block_codes
+from tokenforge.kernels.block_config import BLOCK_TILES, BlockConfig
+from tokenforge.kernels.hip.fp8_block import fp8_block_gemm
 
 pytestmark = pytest.mark.gpu
 ops = torch.ops.tokenforge
@@ -64,3 +67,44 @@ def test_linear_too_large_for_its_usual_launch(m: int, n: int, device: torch.dev
             r, c = slice(r0, min(m, r0 + 40)), slice(c0, min(n, c0 + 128))
             inputs = (x8[r].cpu(), xs[r].cpu(), w8[c].cpu(), ws[c0 // 128:c0 // 128 + 1].cpu())
             bc.check_linear(y[r, c], inputs, f"{m}x{n} at {r0}, {c0}")
+
+
+def _config(tile: tuple[str, int, int, int, int]) -> BlockConfig:
+    kernel, bm, bn, warps, stages = tile
+    return BlockConfig(kernel, bm, bn, 1, warps, stages)
+
+
+@pytest.mark.parametrize("tile", BLOCK_TILES, ids=str)
+def test_small_products_beside_a_large_one(tile, device: torch.device) -> None:  # type: ignore[no-untyped-def]
+    """A product of 2^16 at one k, its negative 16 k further on (another group of eight), a small one at each
+    other k in turn, a row of x each: in the large ones' groups 2^3 is kept whole and less may be lost, in the
+    other groups 2^-7 is kept whole. (fp32's 24 bits hold 2^16 + 2^-7, but for 2^16 + 2^-8 it takes 25.)"""
+    k, at = 128, 37
+    back = at + 16
+    others = [j for j in range(k) if j not in (at, back)]
+    for e in (6, 3, 2, 0, -7, -8):
+        x = torch.zeros((len(others), k))
+        w = torch.ones((3, k))
+        x[:, at] = x[:, back] = 256.0
+        w[:, at], w[:, back] = 256.0, -256.0
+        small = 2.0 ** (e / 2 if e % 2 == 0 else (e - 1) / 2)
+        for r, j in enumerate(others):
+            x[r, j] = small
+        w[:, others] = 2.0**e / small
+        f8 = torch.float8_e4m3fn
+        assert torch.equal(x.to(f8).float(), x) and torch.equal(w.to(f8).float(), w)
+        y = fp8_block_gemm(x.to(f8).to(device), torch.ones((len(others), 1), device=device), w.to(f8).to(device),
+                           torch.ones((1, 1), device=device), _config(tile)).cpu()
+        for r, j in enumerate(others):
+            near = j // 8 in (at // 8, back // 8)
+            ok = (y[r] == 2.0**e) | ((y[r] >= 0) & (y[r] <= 2.0**e) if (near and e < 3) or e < -7 else False)
+            assert bool(ok.all()), (e, j, y[r])
+
+
+@pytest.mark.parametrize("kind", ["outliers", "one sign", "cancelling"])
+@pytest.mark.parametrize("tile", BLOCK_TILES, ids=str)
+def test_linear_of_products_far_apart(tile, kind: str, device: torch.device) -> None:  # type: ignore[no-untyped-def]
+    inputs = block_codes.hard_inputs(kind, 21, 150, 1040)
+    residual = block_codes.remainder_residual(inputs)
+    y = fp8_block_gemm(*(t.to(device) for t in inputs), _config(tile), None, torch.float16, residual.to(device))
+    block_codes.check_remainder(y, inputs, residual, f"{kind} {tile}")

@@ -319,6 +319,36 @@ def test_code_check_refuses_wrong_codes_and_scales(group: int) -> None:
             block_codes.check_codes(q, t, y, 0.0, group, "planted")
 
 
+@pytest.mark.parametrize("kind", ["outliers", "one sign", "cancelling"])
+def test_remainder_check_against_the_stated_rule(kind: str) -> None:
+    """The check of the linear's remainder: the rule itself (products cut toward zero in groups of eight) passes,
+    a cut four bits higher, a group left out and a NaN do not."""
+    from oracle.reference import e4m3_decode
+
+    inputs = block_codes.hard_inputs(kind, 3, 10, 272)
+    residual = block_codes.remainder_residual(inputs)
+    x8, xs, w8, ws = inputs
+    p = e4m3_decode(bc.codes(x8)).astype(np.float64)[:, None] * e4m3_decode(bc.codes(w8)).astype(np.float64)[None]
+    scale = xs.double().numpy()[:, None] * np.repeat(ws.double().numpy(), 128, axis=0)[:10][None]
+
+    def linear(bits: int, skip: int = -1) -> torch.Tensor:
+        y = np.zeros(p.shape[:2])
+        for g, k0 in enumerate(range(0, 272, 8)):
+            part = p[:, :, k0:k0 + 8]
+            unit = np.exp2(np.floor(np.log2(np.abs(part).max(axis=2, keepdims=True))) - bits)
+            y += 0.0 if g == skip else (np.trunc(part / unit) * unit).sum(axis=2) * scale[:, :, k0 // 128]
+        return torch.from_numpy(y + residual.double().numpy()).to(torch.float16)
+
+    block_codes.check_remainder(linear(13), inputs, residual, "the rule")
+    block_codes.check_remainder(linear(40), inputs, residual, "no cut")
+    nan = linear(13)
+    nan[1, 2] = float("nan")
+    # ("cancelling": by the rule a group's sum is lost whole)
+    for wrong in (nan,) if kind == "cancelling" else (linear(9), linear(13, 5), nan):
+        with pytest.raises(AssertionError):
+            block_codes.check_remainder(wrong, inputs, residual, "planted")
+
+
 def test_oracle_half_step_and_scales() -> None:
     values = np.sort(np.unique(np.abs(torch.arange(0, 127, dtype=torch.uint8).view(F8).float().numpy()))).astype(np.float64)
     for lo, hi in zip(values[:-1], values[1:]):
