@@ -108,3 +108,21 @@ def test_linear_of_products_far_apart(tile, kind: str, device: torch.device) -> 
     residual = block_codes.remainder_residual(inputs)
     y = fp8_block_gemm(*(t.to(device) for t in inputs), _config(tile), None, torch.float16, residual.to(device))
     block_codes.check_remainder(y, inputs, residual, f"{kind} {tile}")
+
+
+@pytest.mark.parametrize("dtype", bc.DTYPES, ids=str)
+@pytest.mark.parametrize(("n", "with_bias", "with_residual"), [(8000, True, True), (8000, False, True), (8000, True, False),
+                                                               (8001, True, True)])
+def test_outputs_past_the_caches(n: int, with_bias: bool, with_residual: bool, dtype: torch.dtype,
+                                 device: torch.device) -> None:
+    """Outputs above 32 MB of the largest tile, which are stored past the L2s: bias, residual and rows whose
+    length takes no 16-byte store."""
+    m, k = 2201, 256
+    inputs = bc.linear_inputs(m, n, k, seed=50)
+    g = bc.gen("past", n)
+    bias = (torch.randn((n,), generator=g) * 4).to(dtype) if with_bias else None
+    residual = (torch.randn((m, n), generator=g) * 4).to(dtype) if with_residual else None
+    y = fp8_block_gemm(*(t.to(device) for t in inputs), BlockConfig("gemm_block", 256, 256, 1, 8, 2),
+                       None if bias is None else bias.to(device), dtype,
+                       None if residual is None else residual.to(device))
+    bc.check_linear(y, inputs, f"{n} {dtype}", bias, residual)
