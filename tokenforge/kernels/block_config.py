@@ -5,7 +5,9 @@ modelled time is least (up to four rows always the gemv form, by :func:`_one_til
 constants are fitted to measured times of every config on MI355X, weights read from HBM: 4560 layers and row
 counts (M 5 to 2500, weights of 16 KB to 136 MB). There the choice is 0.6% slower on average than the
 best compiled config (99 of 100 within 9%); on others, 0.3% at M 2000 to 9000 and 0.8% at M 1 to 2500, of
-which 2.3% up to four rows. There is no table of tuned layers.
+which 2.3% up to four rows. There is no table of tuned layers. ``bench_probes/block_choice.py`` times every
+config of a call, the data of such a fit (the small decoder's down projection at M = 16 loses most: 7.9 us
+against 6.4 of the four-row gemv form, which the rule keeps to four rows).
 """
 
 from __future__ import annotations

@@ -9,11 +9,15 @@
 //
 // A block's scale needs its own sum, so four VALU multiply-adds go with each MFMA of 32 cycles: with both
 // interleaved in registers alone, random codes reach 3.5 PFLOP/s on MI355X (MFMAs alone 4.0 to 4.4; the
-// nominal peak 5.0). The 256 x 256 tile reaches 2.05 (gate_up, N = 37888, K = 3584, M = 4096: 542 us; the
-// library's fp8 product of that size with one scale per tensor 504 us). Without its loads it takes 416
+// nominal peak 5.0). The 256 x 256 tile reaches 2.06 (gate_up, N = 37888, K = 3584, M = 4096: 539 us a call
+// among others; the library's fp8 product of that size with one scale per tensor 504 us). Without its loads it takes 416
 // us, the loads alone 417, both 500: a stage of 64 KB is one block ahead (LDS holds two), so its latency is
 // covered by one block's MFMAs only. Of 9.25 rounds of tiles the last is a quarter full. The smaller
-// tiles serve fewer rows, where the weight's bytes bind: gate_up M = 48 29 us (4.8 TB/s) on 64 x 256.
+// tiles serve fewer rows, where the weight's bytes bind: gate_up M = 48 33.7 us (4.1 TB/s) on 64 x 256.
+//
+// Farthest from the floor are 64 to 2500 rows (1.4 to 5 times the bytes or products alone): a tile count just
+// past the CUs' costs a round more, each row tile reads the weight again, and with one workgroup a CU its
+// first loads and its epilogue stand alone.
 //
 // WK: K groups of a workgroup, each with waves and stages of its own over a share of the K blocks; the
 // sums of the others go to the first through LDS. For tiles so few that a CU has one: it then has WK times
@@ -83,7 +87,7 @@ __device__ __forceinline__ void load16(__amdgpu_buffer_rsrc_t r, uint8_t* base, 
 }
 
 // STREAM: the output, larger than the XCDs' L2s, goes past them and leaves them to the panels (gate_up M =
-// 4096 on MI355X: 548 us against 532).
+// 4096 on MI355X: 532 us, and 548 through them).
 template <int BM, int BN, int WM, int WN, int S, int WK, bool STREAM>
 __global__ __launch_bounds__(64 * WM * WN * WK) void block_gemm_kernel(BlockArgs a, float* __restrict__ part,
                                                                        int split_k, int tiles_m, int tiles_n) {

@@ -12,8 +12,8 @@
 // then right in the lanes of block j, and the others take the scale zero, so x and its scales cost one
 // load for G blocks; the lanes of a row are added at the end.
 //
-// Bound by the weight's bytes from a few MB on. On MI355X, weights from HBM: 37888 x 3584 M = 1 26.0 us
-// (5.2 TB/s, the card's copy rate), 3584 x 18944 15.8 us (4.3 TB/s: 224 workgroups), 4608 x 3584 7.4 us,
+// Bound by the weight's bytes from a few MB on. On MI355X, weights from HBM: 37888 x 3584 M = 1 25.2 us
+// (5.4 TB/s, the card's copy rate), 3584 x 18944 15.0 us (4.5 TB/s: 224 workgroups), 4608 x 3584 7.6 us,
 // of which 3 us are a launch. G = 4 took the first from 31 to 29 us, loads that go through the caches
 // from 29 to 26.
 #include "fp8_block.h"

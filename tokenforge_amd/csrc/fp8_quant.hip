@@ -7,9 +7,11 @@
 //
 // All three read and write each element once: 3 (quant), 5 (silu) or 7 (norm with its residual)
 // bytes per element, memory bound from a few hundred rows on, launch bound below. On MI355X (a copy
-// of 1 GiB: 5.2 TB/s): quant 4095 x 3584 9.0 us (4.9 TB/s), silu 2048 x 18944 39 us (5.0), norm 4095 x 3584
-// 19.5 us (5.3). Loads and stores take the caches' default policy: the inputs were just written and the
-// codes are read next (non-temporal loads: norm 23.4 us).
+// of 1 GiB: 5.2 TB/s), bf16, us: quant 4095 x 3584 8.9 (4.9 TB/s), silu 2048 x 18944 38.9 (5.0), norm 4095 x
+// 3584 18.9 (5.4); with one scale per row 8.7, 50.7 (a CU holds one row of four chunks a thread), 19.1.
+// Rows that 16 bytes do not divide, or that start off them, go by elements: 25, 108 and 63. Loads and
+// stores take the caches' default policy: the inputs were just written and the codes are read next
+// (non-temporal loads: norm 23.4 us).
 #include "fp8_rows.h"
 
 namespace tf {
