@@ -10,10 +10,11 @@ Usage (needs the GPU)::
 
 ``layers`` and ``random`` (layers with N 64 .. 32768 and K 256 .. 16384, half of them the decoders') print a
 JSON line per call: the times of every compiled tile and K split, the data a refit of the model needs.
-Times are the median of 7 replays, in turn, of HIP graphs that launch once per copy of the operands, the
-copies together 400 MB (at most 40 of them), 40 launches a graph, so weights come from HBM. The floor is the larger of the call's bytes
-at 5.17 TB/s (a copy of 1 GiB) and its products at 2605 TFLOP/s (the library's fp8 product of 8192^3 with
-one scale a tensor). ``calls`` makes 12 calls of a case of ``perf/operators.py`` over three sets of inputs.
+Times are the median of 7 replays, in turn, of HIP graphs of 40 launches or more over as many copies of the
+operands as 400 MB hold, 40 at most: from a weight of 10 MB on they come from HBM, smaller ones from the
+caches. The floor is the larger of the call's bytes at 5.17 TB/s (a copy of 1 GiB) and its products at 2605
+TFLOP/s (the library's fp8 product of 8192^3 with one scale a tensor). ``calls`` makes 12 calls of a case of
+``perf/operators.py`` over three sets of inputs.
 """
 
 from __future__ import annotations
@@ -125,8 +126,9 @@ def summary(log: str) -> None:
     out = ["# The block-scaled e4m3 linear on the layers of two decoders", "", "Commands (on an MI355X):", "", "```",
            "python bench_probes/block_choice.py layers > block_choice.log",
            "python bench_probes/block_choice.py summary block_choice.log", "```", "",
-           "us a launch in a HIP graph, bf16 output, operands from HBM, the config of `block_config` / the floor",
-           "(bytes at 5.17 TB/s or products at 2605 TFLOP/s, no launch in it: a launch alone takes 2 to 3 us).", "",
+           "us a launch in a HIP graph, bf16 output, the config of `block_config` / the floor. 7B operands come from HBM,",
+           "0.5B ones, 40 copies, partly from the caches. The floor is bytes at 5.17 TB/s or products at 2605 TFLOP/s,",
+           "without a launch, which alone takes 2 to 3 us.", "",
            "| Layer | N x K | " + " | ".join(f"M = {m}" for m in ms) + " |", "|---|---|" + "---:|" * len(ms)]
     for layer, (n, k) in LAYERS.items():
         at = {r["m"]: r for r in named if r["layer"] == layer}

@@ -10,10 +10,10 @@
 // A block's scale needs its own sum, so four VALU multiply-adds go with each MFMA of 32 cycles: with both
 // interleaved in registers alone, random codes reach 3.5 PFLOP/s on MI355X (MFMAs alone 4.0 to 4.4; the
 // nominal peak 5.0). The 256 x 256 tile reaches 2.06 (gate_up, N = 37888, K = 3584, M = 4096: 539 us a call
-// among others; the library's fp8 product of that size with one scale per tensor 504 us). Without its loads it takes 416
-// us, the loads alone 417, both 500: a stage of 64 KB is one block ahead (LDS holds two), so its latency is
-// covered by one block's MFMAs only. Of 9.25 rounds of tiles the last is a quarter full. The smaller
-// tiles serve fewer rows, where the weight's bytes bind: gate_up M = 48 33.7 us (4.1 TB/s) on 64 x 256.
+// among others; the library's fp8 product of that size with one scale per tensor 504 us). Without its
+// loads it takes 416 us, the loads alone 417, both 500: a stage of 64 KB is one block ahead (LDS holds two),
+// so its latency is covered by one block's MFMAs only. Of 9.25 rounds of tiles the last is a quarter full.
+// The smaller tiles serve fewer rows, where the weight's bytes bind: gate_up M = 48 33.7 us (4.1 TB/s) on 64 x 256.
 //
 // Farthest from the floor are 64 to 2500 rows (1.4 to 5 times the bytes or products alone): a tile count just
 // past the CUs' costs a round more, each row tile reads the weight again, and with one workgroup a CU its
