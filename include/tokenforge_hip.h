@@ -333,6 +333,80 @@ int tf_fp8_block_linear(const uint8_t* x8, int64_t ldx8, const float* xscale, in
                         const tf_gemm_config* cfg, float* workspace, int64_t workspace_bytes,
                         void* stream);
 
+/* --------------------------------------------------------------- paged key-value cache and attention */
+
+#define TF_DTYPE_E4M3 2 /* a cache of e4m3fn codes with a scale per token and head */
+
+/* Longest head of the entry points below; heads are multiples of 8. */
+#define TF_KV_MAX_HEAD_DIM 256
+
+/* A paged cache: keys and values [pages, heads, page_size, head_dim], the last dimension contiguous,
+ * the other strides (page, head, token; in elements) any that keep rows apart and start each on 16
+ * bytes (8 for e4m3 codes), less than 2^24 elements between tokens. Token i of a page in slot page * page_size
+ * + i. dtype TF_DTYPE_E4M3: codes, and fp32 scales [pages, heads, page_size] with strides of their own (less
+ * than 2^24 between tokens); else 16-bit values and no scales. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int32_t heads;
+  int32_t page_size;
+  int32_t head_dim;
+  int32_t dtype;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t k_scale_strides[3];
+  int64_t v_scale_strides[3];
+} tf_kv_cache;
+
+/* No counterparts in the reference, which has no attention.
+ *
+ * tf_kv_cache_write: keys and values of t tokens into their slots. k, v [t, heads, head_dim] of the 16-bit
+ * type `dtype` (strides token, head in elements; rows on 16 bytes), the cache's own type or TF_DTYPE_E4M3: then
+ *   scale = max(amax / 448, 1/(448*512)) over the head, code = e4m3fn(RNE(value / scale)).
+ * slots int64 [t]; a slot outside [0, pages * page_size) is not written (padding). Slots of one call must
+ * differ: of two tokens with one slot it is not specified whose values stay.
+ *
+ * tf_rope_kv_cache_write: the same with q [t, q_heads, head_dim] and k rotated first, in fp32 up to the one
+ * rounding (or the codes): with i < rot / 2, (a, b) = elements (i, i + rot/2), or (2i, 2i+1) if interleaved,
+ *   a' = a cos - b sin, b' = b cos + a sin,  cos = cos_sin[positions[t]][i], sin = cos_sin[..][rot/2 + i];
+ * elements from rot on stay. cos_sin fp32 [max_positions, rot] contiguous, 16-byte aligned, rot even and at
+ * most head_dim; positions int64 [t]; a position outside the table gives NaN in the rotated elements. q_out
+ * [t, q_heads, head_dim] contiguous.
+ *
+ * tf_kv_cache_read: k_out, v_out [t, heads, head_dim] contiguous, of the 16-bit type `dtype` (the cache's own,
+ * or any for e4m3): the tokens in slots int64 [t], code * scale rounded once; zeros for a slot out of range. */
+int tf_kv_cache_write(const tf_kv_cache* cache, const uint16_t* k, int64_t k_token, int64_t k_head,
+                      const uint16_t* v, int64_t v_token, int64_t v_head, int32_t dtype,
+                      const int64_t* slots, int64_t t, void* stream);
+int tf_rope_kv_cache_write(const tf_kv_cache* cache, const uint16_t* q, int64_t q_token, int64_t q_head,
+                           int32_t q_heads, const uint16_t* k, int64_t k_token, int64_t k_head,
+                           const uint16_t* v, int64_t v_token, int64_t v_head, int32_t dtype,
+                           const float* cos_sin, int64_t max_positions, int32_t rot, int32_t interleaved,
+                           const int64_t* positions, const int64_t* slots, uint16_t* q_out, int64_t t,
+                           void* stream);
+int tf_kv_cache_read(const tf_kv_cache* cache, const int64_t* slots, uint16_t* k_out, uint16_t* v_out,
+                     int32_t dtype, int64_t t, void* stream);
+
+/* Attention of one new token of each of m sequences over its cached tokens:
+ *   out[b][j] = sum_i p_i v_i / sum_i p_i,  p_i = exp(scale * q[b][j] . k_i - max)
+ * over i in [max(0, n - window), n) (window 0: [0, n)), n = seq_lens[b] clamped to [0, width * page_size], head
+ * j reading key-value head j / (q_heads / heads). Token i lies in page block_table[b][i / page_size]; the tokens
+ * of a page index outside [0, pages) take no part. No token left: zeros. q [m, q_heads, head_dim] (strides in
+ * elements, rows on 16 bytes) and out [m, q_heads, head_dim] contiguous of the 16-bit type `dtype`, the cache's own
+ * or any for e4m3; block_table int32 [m, width], row stride table_stride; seq_lens int32 [m]; width *
+ * page_size < 2^31 - 256 and the steps of 16 tokens of all heads' table rows below 2^31. Products are exact and
+ * summed in fp32, probabilities carry 16 bits or more into the second product.
+ * workspace: fp32, 16-byte aligned, >= tf_paged_attention_workspace_bytes (-1 for sizes the attention refuses).
+ * Two calls that may overlap need workspaces of their own. */
+int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads, int64_t width);
+int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, int64_t q_row, int64_t q_head, int32_t q_heads,
+                       int32_t dtype, const int32_t* block_table, int64_t table_stride, int64_t width,
+                       const int32_t* seq_lens, int64_t m, float scale, int32_t window, uint16_t* out,
+                       float* workspace, int64_t workspace_bytes, void* stream);
+
 /* Test hook for the e4m3fn encoding used by tf_rmsnorm_fp8_quant
  * (rmsnorm_fp8.py:29-41 _round_to_e4m3_grid + cast): fp32 [count] -> uint8 [count], through
  * the same hardware conversion (v_cvt_pk_fp8_f32) and NaN handling as that kernel.

@@ -28,6 +28,10 @@ BLOCK_KERNEL_IDS = {"gemv_block": 4, "gemm_block": 5}
 """Kernel families of ``tf_fp8_block_linear`` (TF_KERNEL_FP8_BLOCK_*)."""
 FP8_MAX_ROW = 32768
 """TF_FP8_MAX_ROW: longest row the FP8 quantizers reduce as a whole."""
+DTYPE_E4M3 = 2
+"""TF_DTYPE_E4M3: a key-value cache of e4m3 codes."""
+KV_MAX_HEAD_DIM = 256
+"""TF_KV_MAX_HEAD_DIM: longest head of the cache's operators."""
 EPILOGUE_NONE = 0
 EPILOGUE_RESIDUAL = 1
 EPILOGUE_SILU_MUL = 2
@@ -45,6 +49,26 @@ class TfGemmConfig(ctypes.Structure):
         ("split_k", ctypes.c_int32),
         ("num_warps", ctypes.c_int32),
         ("num_stages", ctypes.c_int32),
+    ]
+
+
+class TfKvCache(ctypes.Structure):
+    """``tf_kv_cache``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_scale_strides", ctypes.c_int64 * 3),
+        ("v_scale_strides", ctypes.c_int64 * 3),
     ]
 
 
@@ -117,6 +141,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64,
          ctypes.POINTER(TfGemmConfig), _p, _i64, _p]),
+    "tf_kv_cache_write": (
+        ctypes.c_int, [ctypes.POINTER(TfKvCache), _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _p]),
+    "tf_rope_kv_cache_write": (
+        ctypes.c_int,
+        [ctypes.POINTER(TfKvCache), _p, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i32, _i32,
+         _p, _p, _p, _i64, _p]),
+    "tf_kv_cache_read": (ctypes.c_int, [ctypes.POINTER(TfKvCache), _p, _p, _p, _i32, _i64, _p]),
+    "tf_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(TfKvCache), _i64, _i32, _i64]),
+    "tf_paged_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(TfKvCache), _p, _i64, _i64, _i32, _i32, _p, _i64, _i64, _p, _i64, _f32, _i32, _p, _p, _i64,
+         _p]),
     "tf_e4m3_encode": (ctypes.c_int, [_p, _p, _i64, _p]),
 }
 

@@ -276,3 +276,75 @@ def block_linear(x8: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, 
     for extra in (bias, residual):
         y = y if extra is None else y + extra.to(torch.float32)
     return y.to(out_dtype)
+
+
+# ----------------------------------------------------------------------------- key-value cache and attention
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, slots: torch.Tensor) -> None:
+    """fp32 ``k``, ``v [T, heads, head_dim]`` into their slots of the cache ``[pages, heads, page_size, head_dim]``:
+    rounded to its type, or as e4m3 codes with a scale per token and head. Slots out of range are left out."""
+    pages, heads, page, d = k_cache.shape
+    kept = (slots >= 0) & (slots < pages * page)
+    at, off = slots[kept] // page, slots[kept] % page
+    for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+        x = x[kept]
+        if scale is None:
+            cache[at, :, off] = x.to(cache.dtype)
+            continue
+        q, s = block_quant(x.reshape(-1, d), 0)
+        cache.view(torch.uint8)[at, :, off] = q.view(torch.uint8).reshape(-1, heads, d)
+        scale[at, :, off] = s.reshape(-1, heads)
+
+
+def rotate(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    """fp32 ``x [T, heads, head_dim]`` with its first ``rot`` elements turned in pairs (i, i + rot/2), or (2i, 2i + 1)
+    if interleaved, by the table's row (cosines, then sines) at the token's position; NaN where the table has none."""
+    known = (positions >= 0) & (positions < cos_sin.shape[0])
+    turn = torch.where(known[:, None], cos_sin[positions.clamp(0, cos_sin.shape[0] - 1)], float("nan"))
+    cos, sin = turn[:, None].chunk(2, dim=-1)
+    rot = cos_sin.shape[1]
+    a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else x[..., :rot].chunk(2, dim=-1)
+    pair = a * cos - b * sin, b * cos + a * sin
+    turned = torch.stack(pair, -1).flatten(-2) if interleaved else torch.cat(pair, -1)
+    return torch.cat([turned, x[..., rot:]], -1)
+
+
+def _cached(cache: torch.Tensor, scale: torch.Tensor | None, at: torch.Tensor, off: torch.Tensor) -> torch.Tensor:
+    """fp32 tokens at pages ``at`` and offsets ``off``: ``[T, heads, head_dim]``."""
+    if scale is None:
+        return cache[at, :, off].to(torch.float32)
+    codes = cache.view(torch.uint8)[at, :, off].view(torch.float8_e4m3fn)
+    return codes.to(torch.float32) * scale[at, :, off][..., None]
+
+
+def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor | None,
+                  v_scale: torch.Tensor | None, slots: torch.Tensor,
+                  out_dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """The tokens in ``slots``, rounded once to ``out_dtype``; zeros for a slot out of range."""
+    pages, _, page, _ = k_cache.shape
+    kept = ((slots >= 0) & (slots < pages * page))[:, None, None]
+    slots = torch.where(kept[:, 0, 0], slots, 0)
+    k, v = (_cached(c, s, slots // page, slots % page) for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+    return torch.where(kept, k, 0.0).to(out_dtype), torch.where(kept, v, 0.0).to(out_dtype)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor | None,
+                    v_scale: torch.Tensor | None, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                    window: int) -> torch.Tensor:
+    """Softmax attention of ``q [m, q_heads, head_dim]`` over each sequence's cached tokens in fp32, one rounding."""
+    pages, heads, page, _ = k_cache.shape
+    out = torch.zeros(q.shape, dtype=q.dtype)
+    for b, n in enumerate(seq_lens.clamp(0, block_table.shape[1] * page).tolist()):
+        pos = torch.arange(max(0, n - window) if window > 0 else 0, n)
+        at = block_table[b].to(torch.int64)[pos // page]
+        there = (at >= 0) & (at < pages)
+        pos, at = pos[there], at[there]
+        if pos.numel() == 0:
+            continue
+        k, v = (_cached(c, s, at, pos % page).transpose(0, 1) for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+        x = q[b].to(torch.float32).unflatten(0, (heads, -1))
+        p = torch.softmax(x @ k.transpose(1, 2) * scale, dim=-1)
+        out[b] = (p @ v).flatten(0, 1).to(q.dtype)
+    return out

@@ -57,6 +57,17 @@ such codes with e4m3 weights that have a scale per 128 x 128 block, as FP8 check
   residual)`` = ``x8 @ weight^T`` with the scales applied, plus bias, plus the residual (epilogue
   ``"residual"``), in fp32 with one rounding to fp16 or bf16
 
+and the paged key-value cache with the attention that reads it (no counterparts; :mod:`tokenforge.kernels.hip.kv_cache`
+says what a cache is). The first two write into the caches and scales they are given:
+
+* ``tokenforge::kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots)``: keys and values ``[T, heads,
+  head_dim]`` into their slots, in the cache's 16-bit type or as e4m3 codes with a scale per token and head
+* ``tokenforge::rope_kv_cache_write(q, k, v, cos_sin, positions, k_cache, v_cache, k_scale, v_scale, slots,
+  interleaved)`` = rotated ``q``: the same with ``q`` and ``k`` turned by their positions first
+* ``tokenforge::kv_cache_read(k_cache, v_cache, k_scale, v_scale, slots, out_dtype)`` = ``(k, v)``
+* ``tokenforge::paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, window)``: one
+  new token of each sequence over its cached tokens
+
 On GPU tensors every op runs the hand-written HIP kernels, and a missing kernel library (or
 a GPU other than gfx950) raises instead of falling back. Host (CPU) tensors take the
 reference's ``torch_reference`` route (ops.py:79-81): the torch expressions of
@@ -91,6 +102,7 @@ from tokenforge.kernels.config import (
 )
 from tokenforge.kernels.device import SUPPORTED_ARCHS, device_arch, gpu_identity
 from tokenforge.kernels.hip import fp8_block as _block
+from tokenforge.kernels.hip import kv_cache as _kv
 from tokenforge.kernels.hip import rmsnorm_fp8 as _rms
 from tokenforge.kernels.hip import w4a16 as _w4a16
 from tokenforge.kernels.metrics import KERNEL_CALLS
@@ -580,6 +592,68 @@ def _fp8_block_linear_fake(x8, x_scale, weight, w_scale, bias, out_dtype, backen
     return x8.new_empty((*x8.shape[:-1], weight.shape[0]), dtype=out_dtype)
 
 
+# ----------------------------------------------------------------------------- key-value cache and attention
+
+
+def _kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots):  # type: ignore[no-untyped-def]
+    cache = (k_cache, v_cache, k_scale, v_scale)
+    _kv.check_write(k, v, cache, slots)
+    if _on_host("kv_cache_write", k, v, *cache, slots):
+        host.kv_cache_write(k.to(torch.float32), v.to(torch.float32), *cache, slots)
+    else:
+        _kv.kv_cache_write(k, v, cache, slots)
+
+
+def _rope_kv_cache_write(q, k, v, cos_sin, positions, k_cache, v_cache, k_scale, v_scale, slots,  # type: ignore[no-untyped-def]
+                         interleaved=False):
+    cache = (k_cache, v_cache, k_scale, v_scale)
+    _kv.check_write(k, v, cache, slots)
+    _kv.check_rope(q, k, cos_sin, positions)
+    if _on_host("rope_kv_cache_write", q, k, v, cos_sin, positions, *cache, slots):
+        qf, kf = (host.rotate(x.to(torch.float32), cos_sin, positions, interleaved) for x in (q, k))
+        host.kv_cache_write(kf, v.to(torch.float32), *cache, slots)
+        return qf.to(q.dtype)
+    return _kv.rope_kv_cache_write(q, k, v, cos_sin, positions, cache, slots, interleaved)
+
+
+def _kv_cache_read(k_cache, v_cache, k_scale, v_scale, slots, out_dtype):  # type: ignore[no-untyped-def]
+    cache = (k_cache, v_cache, k_scale, v_scale)
+    _kv.check_read(cache, slots, out_dtype)
+    if _on_host("kv_cache_read", *cache, slots):
+        return host.kv_cache_read(*cache, slots, out_dtype)
+    return _kv.kv_cache_read(cache, slots, out_dtype)
+
+
+def _paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, window=0):  # type: ignore[no-untyped-def]
+    cache = (k_cache, v_cache, k_scale, v_scale)
+    _kv.check_attention(q, cache, block_table, seq_lens, window)
+    if _on_host("paged_attention", q, *cache, block_table, seq_lens):
+        return host.paged_attention(q, *cache, block_table, seq_lens, scale, window)
+    return _kv.paged_attention(q, cache, block_table, seq_lens, scale, window)
+
+
+@torch.library.register_fake("tokenforge::kv_cache_write")
+def _kv_cache_write_fake(k, v, k_cache, v_cache, k_scale, v_scale, slots):  # type: ignore[no-untyped-def]
+    return None
+
+
+@torch.library.register_fake("tokenforge::rope_kv_cache_write")
+def _rope_kv_cache_write_fake(q, k, v, cos_sin, positions, k_cache, v_cache, k_scale, v_scale, slots,  # type: ignore[no-untyped-def]
+                              interleaved=False):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("tokenforge::kv_cache_read")
+def _kv_cache_read_fake(k_cache, v_cache, k_scale, v_scale, slots, out_dtype):  # type: ignore[no-untyped-def]
+    shape = (slots.shape[0], k_cache.shape[1], k_cache.shape[3])
+    return k_cache.new_empty(shape, dtype=out_dtype), k_cache.new_empty(shape, dtype=out_dtype)
+
+
+@torch.library.register_fake("tokenforge::paged_attention")
+def _paged_attention_fake(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, window=0):  # type: ignore[no-untyped-def]
+    return q.new_empty(q.shape)
+
+
 # ----------------------------------------------------------------------------- registrations
 
 # Each operator's Python body: the CPU kernel (the torch route) and tokenforge::_py_<op>, which
@@ -597,6 +671,10 @@ _BODIES = {
     "silu_mul_fp8_quant": _silu_mul_fp8_quant,
     "add_rmsnorm_fp8_quant": _add_rmsnorm_fp8_quant,
     "fp8_block_linear": _fp8_block_linear,
+    "kv_cache_write": _kv_cache_write,
+    "rope_kv_cache_write": _rope_kv_cache_write,
+    "kv_cache_read": _kv_cache_read,
+    "paged_attention": _paged_attention,
 }
 for _name, _body in _BODIES.items():
     _schema = str(getattr(torch.ops.tokenforge, _name).default._schema)

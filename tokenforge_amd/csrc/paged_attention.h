@@ -1,0 +1,645 @@
+// Attention of one new token per sequence over a paged cache: the kernel template, instantiated by head length
+// in paged_attention_d*.hip, launched and joined by paged_attention.hip.
+//
+// Work. Items are (sequence, key-value head, 16 of its query heads); an item is a run of steps of 16 NT tokens.
+// All items' steps form one line, and workgroup w takes the steps [w share, (w + 1) share) of it, so every
+// workgroup gets the same number whatever the sequences' lengths are. Lengths are read on the device; the host
+// knows none. Items that lie in one workgroup are finished by it, the others leave (maximum, sum, accumulator)
+// in the workspace for the join.
+//
+// A wave takes every fourth step. S^T = K Q^T by v_mfma_f32_16x16x32 with 16 tokens as rows and 16 query heads as
+// columns: lane 16g + c then holds head c's scores of tokens 4g .. 4g + 3 of each tile, which is, for the second
+// product O^T = V^T P^T, the operand P^T of two tiles (its 8 consecutive k of lane 16g + c are those tokens):
+// probabilities never leave their lane. V^T's operand wants 8 tokens of one channel; a lane loads the same 8
+// tokens' CS consecutive channels (whole rows, 16 lanes a row) and turns them over in registers, one v_perm_b32
+// for 4 bytes. No step goes through LDS. Running maximum, sum and accumulator are fp32; the waves' are joined in
+// LDS when an item ends.
+//
+// Probabilities go into the second product as two 16-bit halves (p truncated, and the rest), 16 to 22 bits
+// together: the product is memory bound, and with one half alone a bf16 result is off by 1.4 times its own
+// rounding. The lower half is never zero where the upper is not, so that an infinite value times it is infinite
+// and not NaN. Scales of e4m3 values go into the probabilities before the split, e4m3 codes into bf16 (exact).
+#pragma once
+
+#include "kv_cache.h"
+
+namespace tf {
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;  // elements
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t k_page, k_head, v_page, v_head;  // bytes
+  uint32_t k_token, v_token;               // bytes
+  const float* ks;
+  const float* vs;
+  int64_t ks_page, ks_head, vs_page, vs_head;  // elements
+  uint32_t ks_token, vs_token;
+  const int32_t* table;
+  int64_t table_row;
+  const int32_t* lens;
+  uint16_t* out;
+  float* part;  // [2 grid] pieces of part_rows rows: accumulators [part_rows][DP], then (maximum, sum) [part_rows]
+  int2* ends;   // [items] first and last workgroup of an item
+  int64_t pages;
+  PageDiv page;
+  int m, heads, group, row_groups, part_rows, d;
+  int cap;     // tokens a row of the table covers
+  int window;
+  float scale_log2;
+  uint32_t least;  // fewest steps of a workgroup
+  int direct;      // a workgroup an item, whole
+};
+
+constexpr int kAttnGrid = 512;
+
+// Tokens [begin, end) of sequence b, and its steps of KS tokens.
+template <int KS>
+struct Span {
+  int begin, end;
+  uint32_t first, count;
+  __device__ __forceinline__ Span(const AttnArgs& a, int b) {
+    int n = a.lens[b];
+    n = n < 0 ? 0 : n > a.cap ? a.cap : n;
+    end = n;
+    begin = a.window > 0 && n > a.window ? n - a.window : 0;
+    first = (uint32_t)begin / KS;
+    count = n > 0 ? ((uint32_t)n + KS - 1) / KS - first : 0u;
+  }
+};
+
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+
+template <bool WIDE>
+__device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
+  if (WIDE)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// Two codes (the low or high half of a word) as a pair of 16-bit values, exactly.
+template <bool WIDE, bool HI>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+  if (WIDE) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+}
+
+// Max (sum) over lanes c, c + 16, c + 32, c + 48, in each of them.
+__device__ __forceinline__ float max4(float v) {
+  auto s = __builtin_amdgcn_permlane16_swap(as_u32(v), as_u32(v), false, false);
+  v = __builtin_fmaxf(as_f32(s[0]), as_f32(s[1]));
+  s = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
+  return __builtin_fmaxf(as_f32(s[0]), as_f32(s[1]));
+}
+__device__ __forceinline__ float sum4(float v) {
+  auto s = __builtin_amdgcn_permlane16_swap(as_u32(v), as_u32(v), false, false);
+  v = as_f32(s[0]) + as_f32(s[1]);
+  s = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
+  return as_f32(s[0]) + as_f32(s[1]);
+}
+
+// Probabilities p0, p1 as two pairs: truncated, and what is left (see the top). fp16 ones come multiplied by
+// 2^kBias, which keeps them normal down to 2^-24 of the row's largest; the factor cancels in the quotient.
+constexpr float kBias = 10.0f;
+
+template <bool WIDE>
+__device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  if (WIDE) {
+    hi = __builtin_amdgcn_perm(as_u32(p1), as_u32(p0), 0x07060302u);
+    const float r0 = __builtin_fmaxf(p0 - as_f32(as_u32(p0) & 0xFFFF0000u), p0 * 0x1p-20f);
+    const float r1 = __builtin_fmaxf(p1 - as_f32(as_u32(p1) & 0xFFFF0000u), p1 * 0x1p-20f);
+    lo = round_pair<BF16>(r0, r1);
+  } else {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+    hi = __builtin_bit_cast(uint32_t, h);
+    const float h0 = (float)h[0], h1 = (float)h[1];
+    const float r0 = __builtin_fmaxf(p0 - h0, h0 > 0.0f ? 0x1p-24f : 0.0f);
+    const float r1 = __builtin_fmaxf(p1 - h1, h1 > 0.0f ? 0x1p-24f : 0.0f);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+  }
+}
+
+// T: type of q, out and 16-bit caches. DP: head length the tiles hold (d <= DP). PAGED: pages hold whole tiles of
+// 16 tokens, so a tile's page is one scalar; else every token's page is looked up. FULL: d == DP.
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+struct Attn {
+  static constexpr int kWaves = 4;
+  static constexpr int NT = DP == 64 || (FP8 && DP == 128) ? 4 : 2;  // tiles of 16 tokens a step
+  static constexpr int KS = 16 * NT;
+  static constexpr int NK = DP / 32;                  // MFMAs over the channels
+  static constexpr int NSUB = DP > 128 ? DP / 128 : 1;
+  static constexpr int CS = DP / NSUB / 16;           // channels of a lane's V load: 8, or 4 (DP 64)
+  static constexpr int KW = FP8 ? DP / 64 : DP / 32;  // 16-byte words of a lane's K row part
+  static constexpr int VW = FP8 ? CS / 4 : CS / 2;    // words of a lane's V load
+  static constexpr bool PW = FP8 || T::kWide;         // the second product in bf16
+  static constexpr int ROW = DP + 4;                  // floats of a row in LDS
+
+  u4 k[NT][KW];
+  uint32_t v[NT][4][NSUB][VW];
+  float ks[NT][4], vs[NT][4];
+  int hi[NT];        // PAGED: tokens below are valid (0: no page)
+  uint32_t seen;     // !PAGED: bit 4 * tile + r: token 4g + r of the tile is there (V rows and scores)
+
+  f4 acc[NSUB * CS];
+  float top, sum;
+  u4 q[NK];
+
+  // Channels of MFMA j of the first product in lane group g: 8 from
+  static __device__ __forceinline__ int k_at(int j, int g) {
+    return FP8 ? 64 * (j >> 1) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
+  }
+};
+
+// ------------------------------------------------------------------ loads
+//
+// Page numbers of the wave's next 64 / NT steps (PAGED: one a tile) or of a step's tokens (else) are fetched ahead
+// by one lane each.
+
+template <typename A>
+__device__ __forceinline__ int fetch_pages(const AttnArgs& a, const int32_t* table, uint32_t step, int end, int lane,
+                                           int nt) {
+  const uint32_t tile = (step + 4u * (uint32_t)(lane / nt)) * nt + (uint32_t)(lane % nt);
+  const uint64_t key = (uint64_t)tile * 16;
+  return key < (uint64_t)end ? table[div_page((uint32_t)key, a.page)] : -1;
+}
+
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, const uint8_t* kh,
+                                       const float* ksh, uint32_t step, int end, int pages, int slot, int lane) {
+  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  const int c = lane & 15, g = lane >> 4;
+  constexpr int E = FP8 ? 1 : 2;
+#pragma unroll
+  for (int i = 0; i < A::NT; ++i) {
+    const uint8_t* base;
+    if (PAGED) {
+      const int pg = __builtin_amdgcn_readlane(pages, slot * A::NT + i);
+      const uint32_t key = (step * A::NT + i) * 16u;
+      const bool ok = (uint32_t)pg < (uint64_t)a.pages;
+      s.hi[i] = ok ? end : 0;
+      const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
+      base = kh + (int64_t)(ok ? pg : 0) * a.k_page + (int64_t)off * a.k_token + (uint32_t)c * a.k_token;
+      if (FP8) {
+        const float* const sp = ksh + (int64_t)(ok ? pg : 0) * a.ks_page + (int64_t)off * a.ks_token;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s.ks[i][r] = sp[(uint32_t)(4 * g + r) * a.ks_token];
+      }
+    } else {
+      const int pg = __builtin_amdgcn_ds_bpermute((16 * i + c) * 4, pages);
+      const uint32_t key = step * A::KS + 16u * i + c;
+      const bool ok = (uint32_t)pg < (uint64_t)a.pages;
+      const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
+      base = kh + (int64_t)(ok ? pg : 0) * a.k_page + (int64_t)off * a.k_token;
+      if (FP8) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int pr = __builtin_amdgcn_ds_bpermute((16 * i + 4 * g + r) * 4, pages);
+          const uint32_t kr = step * A::KS + 16u * i + 4u * g + r;
+          const bool there = (uint32_t)pr < (uint64_t)a.pages;
+          const uint32_t o = there ? kr - div_page(kr, a.page) * a.page.page : 0u;
+          s.ks[i][r] = ksh[(int64_t)(there ? pr : 0) * a.ks_page + (int64_t)o * a.ks_token];
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < A::KW; ++w) {
+      const int d0 = FP8 ? 64 * w + 16 * g : 32 * w + 8 * g;
+      if (FULL) {
+        s.k[i][w] = *reinterpret_cast<const u4*>(base + d0 * E);
+      } else if (FP8) {  // rows of 8-byte alignment; channels past d from the row's start, cleared below
+        const u2 lo = *reinterpret_cast<const u2*>(base + (d0 < a.d ? d0 : 0));
+        const u2 hi = *reinterpret_cast<const u2*>(base + (d0 + 8 < a.d ? d0 + 8 : 0));
+        s.k[i][w] = u4{lo[0], lo[1], hi[0], hi[1]};
+      } else {
+        s.k[i][w] = *reinterpret_cast<const u4*>(base + (d0 < a.d ? d0 : 0) * E);
+      }
+    }
+  }
+}
+
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, const uint8_t* vh,
+                                       const float* vsh, uint32_t step, int pages, int slot, int lane) {
+  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  const int c = lane & 15, g = lane >> 4;
+  constexpr int E = FP8 ? 1 : 2;
+#pragma unroll
+  for (int i = 0; i < A::NT; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint8_t* base;
+      const float* sp = nullptr;
+      if (PAGED) {
+        const int pg = __builtin_amdgcn_readlane(pages, slot * A::NT + i);
+        const uint32_t key = (step * A::NT + i) * 16u;
+        const bool ok = (uint32_t)pg < (uint64_t)a.pages;
+        const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
+        base = vh + (int64_t)(ok ? pg : 0) * a.v_page + (int64_t)(off + r) * a.v_token + (uint32_t)(4 * g) * a.v_token;
+        if (FP8)
+          sp = vsh + (int64_t)(ok ? pg : 0) * a.vs_page + (int64_t)off * a.vs_token + (uint32_t)(4 * g + r) * a.vs_token;
+      } else {
+        const int pg = __builtin_amdgcn_ds_bpermute((16 * i + 4 * g + r) * 4, pages);
+        const uint32_t key = step * A::KS + 16u * i + 4u * g + r;
+        const bool ok = (uint32_t)pg < (uint64_t)a.pages;
+        const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
+        base = vh + (int64_t)(ok ? pg : 0) * a.v_page + (int64_t)off * a.v_token;
+        if (FP8) sp = vsh + (int64_t)(ok ? pg : 0) * a.vs_page + (int64_t)off * a.vs_token;
+      }
+      if (FP8) s.vs[i][r] = *sp;
+#pragma unroll
+      for (int n = 0; n < A::NSUB; ++n) {
+        const int d0 = 128 * n + A::CS * c;
+        const uint8_t* const p = base + (FULL || d0 < a.d ? d0 : 0) * E;
+        if (A::VW == 4) {
+          const u4 w = *reinterpret_cast<const u4*>(p);
+#pragma unroll
+          for (int x = 0; x < A::VW; ++x) s.v[i][r][n][x] = w[x & 3];
+        } else if (A::VW == 2) {
+          const u2 w = *reinterpret_cast<const u2*>(p);
+#pragma unroll
+          for (int x = 0; x < A::VW; ++x) s.v[i][r][n][x] = w[x & 1];
+        } else {
+          s.v[i][r][n][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ one step
+
+// Scores of the step's tokens, in units of log2, -inf where a token takes no part: x[tile][r] of head c, token
+// 4g + r.
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, uint32_t step, int begin,
+                                       int end, int pages, int lane, float (&x)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
+  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  const int g = lane >> 4;
+  if (!PAGED) s.seen = 0;
+#pragma unroll
+  for (int i = 0; i < A::NT; ++i) {
+    f4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < A::NK; ++j) {
+      u4 f;
+      if (FP8) {
+        const u4 w = s.k[i][j >> 1];
+        const uint32_t w0 = j & 1 ? w[2] : w[0], w1 = j & 1 ? w[3] : w[1];
+        f = u4{codes2<T::kWide, false>(w0), codes2<T::kWide, true>(w0), codes2<T::kWide, false>(w1),
+               codes2<T::kWide, true>(w1)};
+      } else {
+        f = s.k[i][j];
+      }
+      if (!FULL && A::k_at(j, g) >= a.d) f = u4{0u, 0u, 0u, 0u};
+      t = mfma16<T::kWide>(f, s.q[j], t);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int key = (int)(step * A::KS + 16u * i + 4u * g + r);
+      bool in = key >= begin;
+      if (PAGED) {
+        in = in && key < s.hi[i];
+      } else {
+        const int pg = __builtin_amdgcn_ds_bpermute((16 * i + 4 * g + r) * 4, pages);
+        in = in && key < end && (uint32_t)pg < (uint64_t)a.pages;
+        s.seen |= in ? 1u << (4 * i + r) : 0u;
+      }
+      float y = t[r] * a.scale_log2;
+      if (FP8) y *= s.ks[i][r];
+      x[i][r] = in ? y : -__builtin_inff();
+    }
+  }
+}
+
+// Scores -> probabilities: the running maximum, the accumulators' rescaling, the sum.
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void softmax(Attn<T, FP8, DP, PAGED, FULL>& s,
+                                        float (&x)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
+  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  float m = x[0][0];
+#pragma unroll
+  for (int i = 0; i < A::NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = __builtin_fmaxf(m, x[i][r]);
+  m = __builtin_fmaxf(s.top, max4(m));
+  if (__builtin_amdgcn_ballot_w64(m > s.top)) {
+    // -inf -> anything: nothing is there to rescale
+    const float f = s.top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s.top - m);
+    s.sum *= f;
+#pragma unroll
+    for (int j = 0; j < A::NSUB * A::CS; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.acc[j][r] *= f;
+    s.top = m;
+  }
+  const float ref = (m == -__builtin_inff() ? 0.0f : m) - (A::PW ? 0.0f : kBias);
+#pragma unroll
+  for (int i = 0; i < A::NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[i][r] = __builtin_amdgcn_exp2f(x[i][r] - ref);
+      s.sum += x[i][r];
+    }
+}
+
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+__device__ __forceinline__ void accumulate(Attn<T, FP8, DP, PAGED, FULL>& s, uint32_t step, int begin, int end,
+                                           int lane, float (&p)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
+  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  const int g = lane >> 4;
+  // Values (and scales) of tokens that take no part may be anything: NaN times a probability of zero is NaN.
+  bool whole = (int)(step * A::KS) >= begin && (int)(step * A::KS) + A::KS <= end;
+  if (PAGED) {
+#pragma unroll
+    for (int i = 0; i < A::NT; ++i) whole = whole && s.hi[i] != 0;
+  } else {
+    whole = whole && !__builtin_amdgcn_ballot_w64(s.seen != (1u << (4 * A::NT)) - 1u);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < A::NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = (int)(step * A::KS + 16u * i + 4u * g + r);
+        const bool in = PAGED ? key >= begin && key < s.hi[i] : (s.seen >> (4 * i + r)) & 1u;
+        if (FP8) s.vs[i][r] = in ? s.vs[i][r] : 0.0f;
+#pragma unroll
+        for (int n = 0; n < A::NSUB; ++n)
+#pragma unroll
+          for (int w = 0; w < A::VW; ++w) s.v[i][r][n][w] = in ? s.v[i][r][n][w] : 0u;
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < A::NT; u += 2) {
+    u4 hi, lo;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = u + (x >> 1), r = 2 * (x & 1);
+      const float p0 = FP8 ? p[i][r] * s.vs[i][r] : p[i][r];
+      const float p1 = FP8 ? p[i][r + 1] * s.vs[i][r + 1] : p[i][r + 1];
+      uint32_t h, l;
+      split2<A::PW>(p0, p1, h, l);
+      hi[x] = h, lo[x] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < A::NSUB; ++n)
+#pragma unroll
+      for (int w = 0; w < A::VW; ++w) {
+        // word w of eight tokens (tile u: r = 0..3, tile u + 1: r = 0..3) turned over to channels
+        u4 f[FP8 ? 4 : 2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = u + (x >> 1), r = 2 * (x & 1);
+          const uint32_t a0 = s.v[i][r][n][w], a1 = s.v[i][r + 1][n][w];
+          if (FP8) {
+            const uint32_t e = __builtin_amdgcn_perm(a1, a0, 0x05010400u);  // channels 0 and 1 of both tokens
+            const uint32_t o = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+            f[0][x] = codes2<true, false>(e), f[1][x] = codes2<true, true>(e);
+            f[FP8 ? 2 : 0][x] = codes2<true, false>(o), f[FP8 ? 3 : 1][x] = codes2<true, true>(o);
+          } else {
+            f[0][x] = __builtin_amdgcn_perm(a1, a0, 0x05040100u);
+            f[1][x] = __builtin_amdgcn_perm(a1, a0, 0x07060302u);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < (FP8 ? 4 : 2); ++y) {
+          f4& t = s.acc[n * A::CS + (FP8 ? 4 : 2) * w + y];
+          t = mfma16<A::PW>(f[y], hi, t);
+          t = mfma16<A::PW>(f[y], lo, t);
+        }
+      }
+  }
+}
+
+// ------------------------------------------------------------------ the kernel
+
+template <typename T>
+__device__ __forceinline__ void store4(uint16_t* p, const f4& y) {
+  *reinterpret_cast<u2*>(p) = u2{round_pair<T>(y[0], y[1]), round_pair<T>(y[2], y[3])};
+}
+
+template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+__global__ __launch_bounds__(256, DP > 128 && !FP8 ? 1 : 2) void attention_kernel(AttnArgs a) {
+  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  using S = Span<A::KS>;
+  __shared__ float rows[A::kWaves][16][A::ROW];
+  __shared__ float tops[A::kWaves][16], sums[A::kWaves][16];
+  __shared__ uint32_t found[4 + 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const uint32_t per = (uint32_t)(a.heads * a.row_groups);  // items of a sequence
+
+  int b;
+  uint32_t item, at, left;  // item of sequence b, its next step, steps left of this workgroup
+  uint32_t share = 0;
+  if (a.direct) {
+    b = (int)(blockIdx.x / per);
+    item = blockIdx.x - (uint32_t)b * per;
+    at = 0;
+    left = S(a, b).count;
+  } else {
+    // All steps, then the sequence that holds this workgroup's first.
+    uint32_t n = 0;
+    for (int i = tid; i < a.m; i += 256) n += S(a, i).count;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) n += (uint32_t)__shfl_xor((int)n, o);
+    if (lane == 0) found[wave] = n;
+    __syncthreads();
+    const uint32_t total = (found[0] + found[1] + found[2] + found[3]) * per;
+    share = (total + gridDim.x - 1) / gridDim.x;
+    share = share < a.least ? a.least : share;
+    const uint64_t start = (uint64_t)blockIdx.x * share;
+    if (start >= total) return;
+    left = total - (uint32_t)start < share ? total - (uint32_t)start : share;
+    const uint32_t want = (uint32_t)start / per;
+    uint32_t before = 0;
+    for (int i0 = 0; i0 < a.m; i0 += 256) {
+      uint32_t own = i0 + tid < a.m ? S(a, i0 + tid).count : 0u, incl = own;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = (uint32_t)__shfl_up((int)incl, o);
+        incl += lane >= o ? up : 0u;
+      }
+      __syncthreads();
+      if (lane == 63) found[wave] = incl;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) incl += found[w];
+      incl += before;
+      if (incl - own <= want && want < incl) found[4] = (uint32_t)(i0 + tid), found[5] = incl - own;
+      before += found[0] + found[1] + found[2] + found[3];
+      if (want < before) break;
+    }
+    __syncthreads();
+    b = (int)found[4];
+    const uint32_t rest = (uint32_t)start - found[5] * per, count = S(a, b).count;
+    item = rest / count;
+    at = rest - item * count;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  item = (uint32_t)__builtin_amdgcn_readfirstlane((int)item);
+  at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+  left = (uint32_t)__builtin_amdgcn_readfirstlane((int)left);
+
+  for (;;) {
+    const S span(a, b);
+    const uint32_t stop = span.count - at < left ? span.count : at + left;  // steps [at, stop) of this item
+    const int head = (int)(item / (uint32_t)a.row_groups), rg = (int)(item - (uint32_t)head * a.row_groups);
+    const int nrows = a.group - 16 * rg < 16 ? a.group - 16 * rg : 16;
+    const int q0 = head * a.group + 16 * rg;
+    const int32_t* const table = a.table + (int64_t)b * a.table_row;
+    const uint8_t* const kh = a.k + head * a.k_head;
+    const uint8_t* const vh = a.v + head * a.v_head;
+    const float* const ksh = FP8 ? a.ks + head * a.ks_head : nullptr;
+    const float* const vsh = FP8 ? a.vs + head * a.vs_head : nullptr;
+
+    A s;
+    s.top = -__builtin_inff(), s.sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < A::NSUB * A::CS; ++j) s.acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t step = span.first + at + (uint32_t)wave;
+    const uint32_t last = span.first + stop;
+    if (step < last) {
+      const uint16_t* const qp = a.q + (int64_t)b * a.q_row + (int64_t)(q0 + (c < nrows ? c : 0)) * a.q_head;
+#pragma unroll
+      for (int j = 0; j < A::NK; ++j) {
+        const int d0 = A::k_at(j, g);
+        s.q[j] = u4{0u, 0u, 0u, 0u};
+        if (c < nrows && (FULL || d0 < a.d)) s.q[j] = *reinterpret_cast<const u4*>(qp + d0);
+      }
+      constexpr int kAhead = 64 / A::NT;  // PAGED: steps whose pages one fetch holds
+      int pages = PAGED ? fetch_pages<A>(a, table, step, span.end, lane, A::NT) : 0, next = 0;
+      const auto lookup = [&](uint32_t st) {
+        const uint32_t key = st * A::KS + (uint32_t)lane;
+        return lane < A::KS && (int64_t)key < span.end && st < last ? table[div_page(key, a.page)] : -1;
+      };
+      if (!PAGED) pages = lookup(step), next = lookup(step + 4);
+      int slot = 0;
+      float x[A::NT][4];
+      load_k(a, s, kh, ksh, step, span.end, pages, slot, lane);
+      load_v(a, s, vh, vsh, step, pages, slot, lane);
+      for (; step + 4 < last; step += 4) {
+        scores(a, s, step, span.begin, span.end, pages, lane, x);
+        int hi[A::NT];
+        if (PAGED) {
+#pragma unroll
+          for (int i = 0; i < A::NT; ++i) hi[i] = s.hi[i];
+        }
+        if (PAGED) {
+          if (++slot == kAhead) slot = 0, pages = fetch_pages<A>(a, table, step + 4, span.end, lane, A::NT);
+        } else {
+          pages = next, next = lookup(step + 8);
+        }
+        load_k(a, s, kh, ksh, step + 4, span.end, pages, slot, lane);
+        int hi_next[A::NT];
+        if (PAGED) {
+#pragma unroll
+          for (int i = 0; i < A::NT; ++i) hi_next[i] = s.hi[i], s.hi[i] = hi[i];
+        }
+        softmax(s, x);
+        accumulate(s, step, span.begin, span.end, lane, x);
+        if (PAGED) {
+#pragma unroll
+          for (int i = 0; i < A::NT; ++i) s.hi[i] = hi_next[i];
+        }
+        load_v(a, s, vh, vsh, step + 4, pages, slot, lane);
+      }
+      scores(a, s, step, span.begin, span.end, pages, lane, x);
+      softmax(s, x);
+      accumulate(s, step, span.begin, span.end, lane, x);
+    }
+
+    // The waves' parts: one maximum, then their rows side by side.
+    const float own = sum4(s.sum);
+    if (g == 0) tops[wave][c] = s.top, sums[wave][c] = own;
+    __syncthreads();
+    const float top = __builtin_fmaxf(__builtin_fmaxf(tops[0][c], tops[1][c]), __builtin_fmaxf(tops[2][c], tops[3][c]));
+    const float f = s.top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s.top - top);
+    if (c < nrows) {
+#pragma unroll
+      for (int n = 0; n < A::NSUB; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < A::CS; j += 4) {
+            f4 y;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) y[x] = s.acc[n * A::CS + j + x][r] * f;
+            *reinterpret_cast<f4*>(&rows[wave][c][128 * n + (4 * g + r) * A::CS + j]) = y;
+          }
+    }
+    __syncthreads();
+    const bool starts = at == 0, whole = starts && stop == span.count;
+    float* const piece =
+        whole ? nullptr : a.part + (int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * a.part_rows * (DP + 2);
+    for (int e = tid; e < nrows * (DP / 4); e += 256) {
+      const int row = e / (DP / 4), d0 = (e - row * (DP / 4)) * 4;
+      const float t = __builtin_fmaxf(__builtin_fmaxf(tops[0][row], tops[1][row]),
+                                      __builtin_fmaxf(tops[2][row], tops[3][row]));
+      float l = 0.0f;
+      f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < A::kWaves; ++w) {
+        const float tw = tops[w][row];
+        l += tw == -__builtin_inff() ? 0.0f : sums[w][row] * __builtin_amdgcn_exp2f(tw - t);
+        y += *reinterpret_cast<const f4*>(&rows[w][row][d0]);
+      }
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (FULL || d0 < a.d)
+          store4<T>(a.out + ((int64_t)b * a.heads * a.group + q0 + row) * a.d + d0, y * inv);
+      } else {
+        *reinterpret_cast<f4*>(piece + row * DP + d0) = y;
+        if (d0 == 0) *reinterpret_cast<float2*>(piece + a.part_rows * DP + 2 * row) = float2{t, l};
+      }
+    }
+    if (a.direct) return;
+    if (starts && tid == 0) {
+      // an item's last workgroup: `rest` steps of it lie behind this workgroup's
+      const uint32_t rest = span.count - stop;
+      a.ends[(int64_t)b * per + item] = int2{(int)blockIdx.x, (int)(blockIdx.x + (rest + share - 1) / share)};
+    }
+    left -= stop - at;
+    if (left == 0) return;
+    at = 0;
+    if (++item == per) {
+      item = 0;
+      do ++b;
+      while (b < a.m && S(a, b).count == 0);
+      if (b >= a.m) return;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, bool FP8, int DP>
+int launch_attention_as(const AttnArgs& a, bool paged, bool full, unsigned grid, hipStream_t stream) {
+  if (paged && full)
+    attention_kernel<T, FP8, DP, true, true><<<grid, 256, 0, stream>>>(a);
+  else if (paged)
+    attention_kernel<T, FP8, DP, true, false><<<grid, 256, 0, stream>>>(a);
+  else
+    attention_kernel<T, FP8, DP, false, false><<<grid, 256, 0, stream>>>(a);
+  return check_launch("tf_paged_attention");
+}
+
+template <int DP>
+int launch_attention(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid,
+                     hipStream_t stream) {
+  if (bf16)
+    return fp8 ? launch_attention_as<BF16, true, DP>(a, paged, full, grid, stream)
+               : launch_attention_as<BF16, false, DP>(a, paged, full, grid, stream);
+  return fp8 ? launch_attention_as<F16, true, DP>(a, paged, full, grid, stream)
+             : launch_attention_as<F16, false, DP>(a, paged, full, grid, stream);
+}
+
+// One per head length, each in a file of its own.
+int launch_attention_d64(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
+int launch_attention_d128(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
+int launch_attention_d256(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
+
+// Tokens of a step, as the kernels above take them.
+constexpr int attention_step(bool fp8, int dp) { return dp == 64 || (fp8 && dp == 128) ? 64 : 32; }
+
+}  // namespace tf

@@ -1,0 +1,156 @@
+// C entry of the paged attention: checks, the choice of the compiled kernel, and the join of items that several
+// workgroups share.
+#include "paged_attention.h"
+
+namespace tf {
+namespace {
+
+struct JoinArgs {
+  const float* part;
+  const int2* ends;
+  const int32_t* lens;
+  uint16_t* out;
+  int heads, group, row_groups, part_rows, d, dp;
+};
+
+// A workgroup per sequence and query head: out = sum_p acc_p 2^(top_p - top) / sum_p sum_p 2^(top_p - top) over the
+// pieces p that the attention's workgroups left, in their order. Items that one workgroup held are done already;
+// sequences without tokens get zeros here.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
+  __shared__ float acc[4][TF_KV_MAX_HEAD_DIM];
+  __shared__ float sums[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int q_heads = a.heads * a.group;
+  const int b = (int)(blockIdx.x / (uint32_t)q_heads), qh = (int)(blockIdx.x - (uint32_t)b * q_heads);
+  uint16_t* const out = a.out + (int64_t)blockIdx.x * a.d;
+  if (a.lens[b] <= 0) {
+    for (int e = tid * 8; e < a.d; e += 256 * 8) *reinterpret_cast<u4*>(out + e) = u4{0u, 0u, 0u, 0u};
+    return;
+  }
+  const int head = qh / a.group, in = qh - head * a.group, rg = in >> 4, row = in & 15;
+  const int2 ends = a.ends[((int64_t)b * a.heads + head) * a.row_groups + rg];
+  if (ends.x == ends.y) return;
+  const int64_t size = (int64_t)a.part_rows * (a.dp + 2);
+  const auto piece = [&](int p) { return a.part + (2 * (int64_t)p + (p == ends.x ? 1 : 0)) * size; };
+  const auto pair = [&](int p) {
+    return *reinterpret_cast<const float2*>(piece(p) + a.part_rows * a.dp + 2 * row);
+  };
+  float top = -__builtin_inff();
+  for (int p = ends.x + lane; p <= ends.y; p += 64) top = __builtin_fmaxf(top, pair(p).x);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+  float l = 0.0f;
+  f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int e = lane * 4;
+  for (int p = ends.x + wave; p <= ends.y; p += 4) {
+    const float2 tl = pair(p);
+    const float f = tl.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(tl.x - top);
+    l += tl.y * f;
+    if (e < a.d) y += *reinterpret_cast<const f4*>(piece(p) + row * a.dp + e) * f;
+  }
+  if (e < a.d) *reinterpret_cast<f4*>(&acc[wave][e]) = y;
+  if (lane == 0) sums[wave] = l;
+  __syncthreads();
+  if (wave != 0 || e >= a.d) return;
+  l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  const auto at = [&](int w) { return *reinterpret_cast<const f4*>(&acc[w][e]); };
+  y = (at(0) + at(1)) + (at(2) + at(3));
+  store4<T>(out + e, y * (l == 0.0f ? 0.0f : 1.0f / l));
+}
+
+bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+// Sizes of a call, and "" or what is wrong with them.
+struct Plan {
+  int dp, group, row_groups, part_rows;
+  int64_t items, cap, part_floats;
+  bool fp8;
+};
+
+std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t width, Plan& p) {
+  if (m < 0 || width < 0 || m > 0x7FFFFFFF) return "bad size";
+  if (q_heads <= 0 || q_heads > 0xFFFF || q_heads % c.heads) return "q_heads must be a multiple of the cache's heads";
+  p.fp8 = c.dtype == TF_DTYPE_E4M3;
+  p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+  p.group = q_heads / c.heads;
+  p.row_groups = (int)cdiv(p.group, 16);
+  p.part_rows = p.group < 16 ? p.group : 16;
+  p.items = m * c.heads * p.row_groups;
+  if (width > 0x7FFFFF00 / c.page_size) return "block_table covers 2^31 - 256 tokens or more";
+  p.cap = width * c.page_size;
+  if (m * q_heads > 0x7FFFFF || p.items * cdiv(p.cap, 16) > 0x7FFFFFFF)
+    return "more sequences, heads and tokens of block_table than 2^31 steps of 16";
+  p.part_floats = 2 * (int64_t)kAttnGrid * p.part_rows * (p.dp + 2);
+  return "";
+}
+
+}  // namespace
+}  // namespace tf
+
+using namespace tf;
+
+extern "C" int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads,
+                                                      int64_t width) {
+  Plan p;
+  if (!cache || !kv_cache_error(cache, cache->dtype == TF_DTYPE_E4M3 ? TF_DTYPE_FP16 : cache->dtype).empty()) return -1;
+  if (!plan_of(*cache, m, q_heads, width, p).empty()) return -1;
+  return p.part_floats * 4 + p.items * 8;
+}
+
+extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, int64_t q_row, int64_t q_head,
+                                  int32_t q_heads, int32_t dtype, const int32_t* block_table, int64_t table_stride,
+                                  int64_t width, const int32_t* seq_lens, int64_t m, float scale, int32_t window,
+                                  uint16_t* out, float* workspace, int64_t workspace_bytes, void* stream) {
+  const auto bad = [](const std::string& what) { return fail(TF_EINVAL, "tf_paged_attention: " + what); };
+  const std::string e = kv_cache_error(cache, dtype);
+  if (!e.empty()) return bad(e);
+  const tf_kv_cache& c = *cache;
+  if (!q || !out || (!block_table && width) || !seq_lens) return bad("null pointer");
+  if (!multiple(q, 16) || q_row % 8 || q_head % 8 || !multiple(out, 16))
+    return bad("rows of q and out must be 16-byte aligned");
+  if (q_row < 0 || q_head < 0 || table_stride < 0) return bad("negative stride");
+  if (window < 0) return bad("need window >= 0");
+  Plan p;
+  const std::string wrong = plan_of(c, m, q_heads, width, p);
+  if (!wrong.empty()) return bad(wrong);
+  const int64_t need = p.part_floats * 4 + p.items * 8;
+  if (!workspace || workspace_bytes < need)
+    return bad("workspace too small (" + std::to_string(workspace_bytes) + " < " + std::to_string(need) + ")");
+  if (!multiple(workspace, 16)) return bad("workspace not 16-byte aligned");
+  if (m == 0) return TF_OK;
+  const int size = p.fp8 ? 1 : 2;
+  AttnArgs a{};
+  a.q = q, a.q_row = q_row, a.q_head = q_head;
+  a.k = (const uint8_t*)c.k, a.v = (const uint8_t*)c.v;
+  a.k_page = c.k_strides[0] * size, a.k_head = c.k_strides[1] * size, a.k_token = (uint32_t)c.k_strides[2] * size;
+  a.v_page = c.v_strides[0] * size, a.v_head = c.v_strides[1] * size, a.v_token = (uint32_t)c.v_strides[2] * size;
+  a.ks = c.k_scale, a.vs = c.v_scale;
+  a.ks_page = c.k_scale_strides[0], a.ks_head = c.k_scale_strides[1], a.ks_token = (uint32_t)c.k_scale_strides[2];
+  a.vs_page = c.v_scale_strides[0], a.vs_head = c.v_scale_strides[1], a.vs_token = (uint32_t)c.v_scale_strides[2];
+  a.table = block_table, a.table_row = table_stride, a.lens = seq_lens, a.out = out;
+  a.part = workspace, a.ends = reinterpret_cast<int2*>(workspace + p.part_floats);
+  a.pages = c.pages, a.page = page_div((uint32_t)c.page_size);
+  a.m = (int)m, a.heads = c.heads, a.group = p.group, a.row_groups = p.row_groups, a.part_rows = p.part_rows;
+  a.d = c.head_dim, a.cap = (int)p.cap, a.window = window, a.scale_log2 = scale * 1.44269504088896341f;
+  a.least = 4;
+  a.direct = p.cap <= 4 * attention_step(p.fp8, p.dp);
+  const bool paged = c.page_size % 16 == 0;
+  bool full = c.head_dim == p.dp;
+  if (p.fp8) {  // whole rows go by 16-byte loads
+    full = full && multiple(c.k, 16);
+    for (int i = 0; i < 3; ++i) full = full && c.k_strides[i] % 16 == 0;
+  }
+  const unsigned grid = a.direct ? (unsigned)p.items : (unsigned)kAttnGrid;
+  const bool bf16 = dtype == TF_DTYPE_BF16;
+  const auto s = (hipStream_t)stream;
+  const auto launch = p.dp == 64 ? launch_attention_d64 : p.dp == 128 ? launch_attention_d128 : launch_attention_d256;
+  if (int rc = launch(a, bf16, p.fp8, paged, full, grid, s)) return rc;
+  if (a.direct) return TF_OK;
+  const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp};
+  if (bf16)
+    join_kernel<BF16><<<(unsigned)(m * q_heads), 256, 0, s>>>(j);
+  else
+    join_kernel<F16><<<(unsigned)(m * q_heads), 256, 0, s>>>(j);
+  return check_launch("tf_paged_attention");
+}

@@ -27,6 +27,7 @@
 #include <dlfcn.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <atomic>
 #include <cstdint>
@@ -34,6 +35,7 @@
 #include <shared_mutex>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/tokenforge_hip.h"
@@ -51,6 +53,11 @@ struct Api {
   decltype(&tf_silu_mul_fp8_quant) silu_quant = nullptr;
   decltype(&tf_add_rmsnorm_fp8_quant) add_norm = nullptr;
   decltype(&tf_fp8_block_linear) block_linear = nullptr;
+  decltype(&tf_kv_cache_write) kv_write = nullptr;
+  decltype(&tf_rope_kv_cache_write) rope_kv_write = nullptr;
+  decltype(&tf_kv_cache_read) kv_read = nullptr;
+  decltype(&tf_paged_attention_workspace_bytes) attention_bytes = nullptr;
+  decltype(&tf_paged_attention) attention = nullptr;
   decltype(&tf_last_error) last_error = nullptr;
 };
 
@@ -79,6 +86,11 @@ void bind_library(c10::string_view path) {
   bind_symbol(handle, "tf_silu_mul_fp8_quant", api.silu_quant);
   bind_symbol(handle, "tf_add_rmsnorm_fp8_quant", api.add_norm);
   bind_symbol(handle, "tf_fp8_block_linear", api.block_linear);
+  bind_symbol(handle, "tf_kv_cache_write", api.kv_write);
+  bind_symbol(handle, "tf_rope_kv_cache_write", api.rope_kv_write);
+  bind_symbol(handle, "tf_kv_cache_read", api.kv_read);
+  bind_symbol(handle, "tf_paged_attention_workspace_bytes", api.attention_bytes);
+  bind_symbol(handle, "tf_paged_attention", api.attention);
   bind_symbol(handle, "tf_last_error", api.last_error);
   g_api = api;
   g_bound.store(true, std::memory_order_release);
@@ -262,6 +274,17 @@ using AddNormFn = std::tuple<at::Tensor, at::Tensor, at::Tensor>(const at::Tenso
 using BlockLinearFn = at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                                  const std::optional<at::Tensor>&, at::ScalarType, c10::string_view,
                                  c10::string_view, const std::optional<at::Tensor>&);
+
+using OptTensor = std::optional<at::Tensor>;
+using KvWriteFn = void(const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&, const OptTensor&,
+                       const OptTensor&, const at::Tensor&);
+using RopeKvWriteFn = at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                 const at::Tensor&, at::Tensor&, at::Tensor&, const OptTensor&, const OptTensor&,
+                                 const at::Tensor&, bool);
+using KvReadFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const OptTensor&,
+                                                    const OptTensor&, const at::Tensor&, at::ScalarType);
+using AttentionFn = at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                               const OptTensor&, const at::Tensor&, const at::Tensor&, double, c10::SymInt);
 
 // ----------------------------------------------------------------------------- W4A16 linear
 
@@ -677,6 +700,181 @@ at::Tensor fp8_block_linear(const at::Tensor& x8, const at::Tensor& x_scale, con
                                     backend, epilogue, residual);
 }
 
+// ----------------------------------------------------------------------------- key-value cache and attention
+
+// Strides of (page, head, token); a dimension of one has none.
+void cache_strides(const at::Tensor& t, int64_t (&s)[3]) {
+  for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+// Whether no two elements of t share memory (dimensions nested by their strides).
+bool elements_apart(const at::Tensor& t) {
+  std::array<std::pair<int64_t, int64_t>, 4> d;
+  size_t n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d[n++] = {t.stride(i), t.size(i)};
+  std::sort(d.begin(), d.begin() + n);
+  int64_t extent = 0;
+  for (size_t i = 0; i < n; ++i) {
+    if (d[i].first <= extent) return false;
+    extent += d[i].first * (d[i].second - 1);
+  }
+  return true;
+}
+
+constexpr int64_t kMaxTokenStride = int64_t(1) << 24;
+
+// The cache as the C entries take it; false where the Python body has an error to report.
+bool cache_ok(const at::Tensor& k, const at::Tensor& v, const OptTensor& ks, const OptTensor& vs, bool written,
+              tf_kv_cache& c) {
+  if (k.dim() != 4 || !k.is_cuda() || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type()) return false;
+  const c10::Device dev = k.device();
+  const bool fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
+  const int32_t dtype = fp8 ? TF_DTYPE_E4M3 : dtype_code(k.scalar_type());
+  const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2), d = k.size(3);
+  if (dtype < 0 || !on(v, dev) || ks.has_value() != fp8 || vs.has_value() != fp8) return false;
+  if (pages == 0 || heads == 0 || page == 0 || heads > 65535 || page > (1 << 24)) return false;
+  if (d == 0 || d % 8 != 0 || d > TF_KV_MAX_HEAD_DIM) return false;
+  c = tf_kv_cache{};
+  c.k = k.data_ptr(), c.v = v.data_ptr();
+  c.pages = pages, c.heads = static_cast<int32_t>(heads), c.page_size = static_cast<int32_t>(page);
+  c.head_dim = static_cast<int32_t>(d), c.dtype = dtype;
+  cache_strides(k, c.k_strides);
+  cache_strides(v, c.v_strides);
+  for (const at::Tensor* t : {&k, &v}) {
+    if (t->stride(3) != 1 || reinterpret_cast<uintptr_t>(t->data_ptr()) % (fp8 ? 8 : 16) != 0) return false;
+    if (written && !elements_apart(*t)) return false;
+  }
+  for (const int64_t* s : {c.k_strides, c.v_strides})
+    if (s[0] % 8 != 0 || s[1] % 8 != 0 || s[2] % 8 != 0 || s[2] >= kMaxTokenStride) return false;
+  if (!fp8) return true;
+  for (const at::Tensor* t : {&*ks, &*vs}) {
+    if (t->scalar_type() != at::kFloat || !on(*t, dev) || t->sizes() != k.sizes().slice(0, 3)) return false;
+    if (page > 1 && t->stride(2) >= kMaxTokenStride) return false;
+    if (written && !elements_apart(*t)) return false;
+  }
+  c.k_scale = data<float>(*ks), c.v_scale = data<float>(*vs);
+  cache_strides(*ks, c.k_scale_strides);
+  cache_strides(*vs, c.v_scale_strides);
+  return true;
+}
+
+// [tokens, heads, head_dim] of the rows' type, contiguous rows on 16 bytes, on the device.
+bool tokens_ok(const at::Tensor& x, int64_t t, int64_t heads, int64_t d, at::ScalarType dtype, const c10::Device& dev) {
+  if (x.dim() != 3 || x.size(0) != t || x.size(1) != heads || x.size(2) != d || x.scalar_type() != dtype ||
+      !on(x, dev) || x.stride(2) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0)
+    return false;
+  return (t <= 1 || x.stride(0) % 8 == 0) && (heads <= 1 || x.stride(1) % 8 == 0);
+}
+
+int64_t step_of(const at::Tensor& x, int64_t i) { return x.size(i) > 1 ? x.stride(i) : 0; }
+
+bool index_ok(const at::Tensor& x, int64_t n, at::ScalarType dtype, const c10::Device& dev) {
+  return x.dim() == 1 && x.size(0) == n && x.scalar_type() == dtype && on(x, dev) && (n <= 1 || x.stride(0) == 1);
+}
+
+// k and v go into the cache: same type as it, or 16 bits into e4m3.
+bool write_ok(const at::Tensor& k, const at::Tensor& v, const tf_kv_cache& c, at::ScalarType cache_type,
+              const at::Tensor& slots, const c10::Device& dev) {
+  if (k.dim() != 3 || k.size(0) == 0) return false;
+  const at::ScalarType type = k.scalar_type();
+  if (dtype_code(type) < 0 || (c.dtype != TF_DTYPE_E4M3 && type != cache_type)) return false;
+  const int64_t t = k.size(0);
+  return tokens_ok(k, t, c.heads, c.head_dim, type, dev) && tokens_ok(v, t, c.heads, c.head_dim, type, dev) &&
+         index_ok(slots, t, at::kLong, dev);
+}
+
+void kv_cache_write(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache, at::Tensor& v_cache,
+                    const OptTensor& k_scale, const OptTensor& v_scale, const at::Tensor& slots) {
+  tf_kv_cache c;
+  const c10::Device dev = k_cache.device();
+  if (!cache_ok(k_cache, v_cache, k_scale, v_scale, true, c) ||
+      !write_ok(k, v, c, k_cache.scalar_type(), slots, dev)) {
+    python_body<KvWriteFn>("tokenforge::_py_kv_cache_write", k, v, k_cache, v_cache, k_scale, v_scale, slots);
+    return;
+  }
+  c10::OptionalDeviceGuard guard(dev);
+  check(api().kv_write(&c, data<const uint16_t>(k), step_of(k, 0), step_of(k, 1), data<const uint16_t>(v),
+                       step_of(v, 0), step_of(v, 1), dtype_code(k.scalar_type()), data<const int64_t>(slots),
+                       k.size(0), c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        "tf_kv_cache_write");
+}
+
+at::Tensor rope_kv_cache_write(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& cos_sin, const at::Tensor& positions, at::Tensor& k_cache,
+                               at::Tensor& v_cache, const OptTensor& k_scale, const OptTensor& v_scale,
+                               const at::Tensor& slots, bool interleaved) {
+  tf_kv_cache c;
+  const c10::Device dev = k_cache.device();
+  const int64_t q_heads = q.dim() == 3 ? q.size(1) : 0;
+  if (!cache_ok(k_cache, v_cache, k_scale, v_scale, true, c) ||
+      !write_ok(k, v, c, k_cache.scalar_type(), slots, dev) || q_heads == 0 || q_heads > 65535 ||
+      !tokens_ok(q, k.size(0), q_heads, c.head_dim, k.scalar_type(), dev) ||
+      !index_ok(positions, k.size(0), at::kLong, dev) || cos_sin.dim() != 2 || cos_sin.scalar_type() != at::kFloat ||
+      !on(cos_sin, dev) || !cos_sin.is_contiguous() || cos_sin.size(0) == 0 || cos_sin.size(1) == 0 ||
+      cos_sin.size(1) % 2 != 0 || cos_sin.size(1) > c.head_dim ||
+      reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 != 0)
+    return python_body<RopeKvWriteFn>("tokenforge::_py_rope_kv_cache_write", q, k, v, cos_sin, positions, k_cache,
+                                      v_cache, k_scale, v_scale, slots, interleaved);
+  c10::OptionalDeviceGuard guard(dev);
+  at::Tensor out = fresh(q.sizes(), q.scalar_type(), dev);
+  check(api().rope_kv_write(&c, data<const uint16_t>(q), step_of(q, 0), step_of(q, 1), static_cast<int32_t>(q_heads),
+                            data<const uint16_t>(k), step_of(k, 0), step_of(k, 1), data<const uint16_t>(v),
+                            step_of(v, 0), step_of(v, 1), dtype_code(k.scalar_type()), data<const float>(cos_sin),
+                            cos_sin.size(0), static_cast<int32_t>(cos_sin.size(1)), interleaved ? 1 : 0,
+                            data<const int64_t>(positions), data<const int64_t>(slots), data<uint16_t>(out),
+                            k.size(0), c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        "tf_rope_kv_cache_write");
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_cache_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                 const OptTensor& k_scale, const OptTensor& v_scale,
+                                                 const at::Tensor& slots, at::ScalarType out_dtype) {
+  tf_kv_cache c;
+  const c10::Device dev = k_cache.device();
+  const int64_t t = slots.dim() == 1 ? slots.size(0) : 0;
+  if (t == 0 || !cache_ok(k_cache, v_cache, k_scale, v_scale, false, c) || dtype_code(out_dtype) < 0 ||
+      (c.dtype != TF_DTYPE_E4M3 && out_dtype != k_cache.scalar_type()) || !index_ok(slots, t, at::kLong, dev))
+    return python_body<KvReadFn>("tokenforge::_py_kv_cache_read", k_cache, v_cache, k_scale, v_scale, slots,
+                                 out_dtype);
+  c10::OptionalDeviceGuard guard(dev);
+  at::Tensor k = fresh({t, c.heads, c.head_dim}, out_dtype, dev), v = fresh({t, c.heads, c.head_dim}, out_dtype, dev);
+  check(api().kv_read(&c, data<const int64_t>(slots), data<uint16_t>(k), data<uint16_t>(v), dtype_code(out_dtype), t,
+                      c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        "tf_kv_cache_read");
+  return {k, v};
+}
+
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const OptTensor& k_scale, const OptTensor& v_scale, const at::Tensor& block_table,
+                           const at::Tensor& seq_lens, double scale, c10::SymInt window) {
+  const int64_t win = window.guard_int(__FILE__, __LINE__);
+  tf_kv_cache c;
+  const c10::Device dev = k_cache.device();
+  int64_t need = -1;
+  if (q.dim() == 3 && q.size(0) > 0 && win >= 0 && cache_ok(k_cache, v_cache, k_scale, v_scale, false, c) &&
+      dtype_code(q.scalar_type()) >= 0 && (c.dtype == TF_DTYPE_E4M3 || q.scalar_type() == k_cache.scalar_type()) &&
+      tokens_ok(q, q.size(0), q.size(1), c.head_dim, q.scalar_type(), dev) && q.size(1) <= 65535 &&
+      index_ok(seq_lens, q.size(0), at::kInt, dev) && block_table.dim() == 2 && block_table.size(0) == q.size(0) &&
+      block_table.scalar_type() == at::kInt && on(block_table, dev) &&
+      (block_table.size(1) <= 1 || block_table.stride(1) == 1))
+    need = api().attention_bytes(&c, q.size(0), static_cast<int32_t>(q.size(1)), block_table.size(1));
+  if (need < 0)
+    return python_body<AttentionFn>("tokenforge::_py_paged_attention", q, k_cache, v_cache, k_scale, v_scale,
+                                    block_table, seq_lens, scale, window);
+  c10::OptionalDeviceGuard guard(dev);
+  at::Tensor out = fresh(q.sizes(), q.scalar_type(), dev);
+  at::Tensor work = fresh({(need + 3) / 4}, at::kFloat, dev);
+  check(api().attention(&c, data<const uint16_t>(q), step_of(q, 0), step_of(q, 1), static_cast<int32_t>(q.size(1)),
+                        dtype_code(q.scalar_type()), data<const int32_t>(block_table), step_of(block_table, 0),
+                        block_table.size(1), data<const int32_t>(seq_lens), q.size(0), static_cast<float>(scale),
+                        static_cast<int32_t>(std::min<int64_t>(win, 0x7FFFFFFF)), data<uint16_t>(out),
+                        data<float>(work), need, c10::hip::getCurrentHIPStream(dev.index()).stream()),
+        "tf_paged_attention");
+  return out;
+}
+
 }  // namespace
 
 // Schemas: the reference's three ops (ops.py:48-156) and this build's fused forms, with the
@@ -702,6 +900,15 @@ TORCH_LIBRARY(tokenforge, m) {
         "(Tensor, Tensor, Tensor)");
   m.def("fp8_block_linear(Tensor x8, Tensor x_scale, Tensor weight, Tensor w_scale, Tensor? bias, "
         "ScalarType out_dtype, str backend, str epilogue=\"none\", Tensor? residual=None) -> Tensor");
+  m.def("kv_cache_write(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, "
+        "Tensor(d!)? v_scale, Tensor slots) -> ()");
+  m.def("rope_kv_cache_write(Tensor q, Tensor k, Tensor v, Tensor cos_sin, Tensor positions, Tensor(a!) k_cache, "
+        "Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor slots, bool interleaved=False) -> "
+        "Tensor");
+  m.def("kv_cache_read(Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, Tensor slots, "
+        "ScalarType out_dtype) -> (Tensor, Tensor)");
+  m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, "
+        "Tensor block_table, Tensor seq_lens, float scale, SymInt window=0) -> Tensor");
   m.def("_bind_library(str path) -> ()");
   m.def("_native_calls() -> int[]");
   m.def("_clear_launch_cache() -> ()");
@@ -720,6 +927,10 @@ TORCH_LIBRARY_IMPL(tokenforge, CUDA, m) {
   m.impl("silu_mul_fp8_quant", &silu_mul_fp8_quant);
   m.impl("add_rmsnorm_fp8_quant", &add_rmsnorm_fp8_quant);
   m.impl("fp8_block_linear", &fp8_block_linear);
+  m.impl("kv_cache_write", &kv_cache_write);
+  m.impl("rope_kv_cache_write", &rope_kv_cache_write);
+  m.impl("kv_cache_read", &kv_cache_read);
+  m.impl("paged_attention", &paged_attention);
 }
 
 TORCH_LIBRARY_IMPL(tokenforge, CompositeExplicitAutograd, m) {
