@@ -122,7 +122,8 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_
 }
 
 // T: type of q, out and 16-bit caches. DP: head length the tiles hold (d <= DP). PAGED: pages hold whole tiles of
-// 16 tokens, so a tile's page is one scalar; else every token's page is looked up. FULL: d == DP.
+// 16 tokens (and scales go by 16-byte loads), so a tile's place is one scalar; else every token is looked up. FULL:
+// d == DP.
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
 struct Attn {
   static constexpr int kWaves = 4;
@@ -135,12 +136,13 @@ struct Attn {
   static constexpr int VW = FP8 ? CS / 4 : CS / 2;    // words of a lane's V load
   static constexpr bool PW = FP8 || T::kWide;         // the second product in bf16
   static constexpr int ROW = DP + 4;                  // floats of a row in LDS
+  static constexpr int kAhead = PAGED ? 64 / NT : 1;  // steps whose places one lookup holds
+  static constexpr int E = FP8 ? 1 : 2;               // bytes of an element
 
   u4 k[NT][KW];
   uint32_t v[NT][4][NSUB][VW];
-  float ks[NT][4], vs[NT][4];
-  int hi[NT];        // PAGED: tokens below are valid (0: no page)
-  uint32_t seen;     // !PAGED: bit 4 * tile + r: token 4g + r of the tile is there (V rows and scores)
+  f4 ks[NT], vs[NT];  // PAGED: scales of tokens 4g .. 4g + 3
+  float ks1, vs1;     // else: of the lane's own token
 
   f4 acc[NSUB * CS];
   float top, sum;
@@ -152,68 +154,96 @@ struct Attn {
   }
 };
 
-// ------------------------------------------------------------------ loads
+// ------------------------------------------------------------------ places
 //
-// Page numbers of the wave's next 64 / NT steps (PAGED: one a tile) or of a step's tokens (else) are fetched ahead
-// by one lane each.
+// Where tiles (PAGED: 64 / NT steps of the wave, a tile a lane) or a step's tokens (else: a token a lane) lie, each
+// lane looking up its own: byte offsets in the caches, element offsets in the scales, and one bit whether there is
+// such a page.
+struct Places {
+  uint64_t k, v, ks, vs;
+  uint64_t there;
+};
 
-template <typename A>
-__device__ __forceinline__ int fetch_pages(const AttnArgs& a, const int32_t* table, uint32_t step, int end, int lane,
-                                           int nt) {
-  const uint32_t tile = (step + 4u * (uint32_t)(lane / nt)) * nt + (uint32_t)(lane % nt);
-  const uint64_t key = (uint64_t)tile * 16;
-  return key < (uint64_t)end ? table[div_page((uint32_t)key, a.page)] : -1;
+// First token of the lane's tile, or its token, in the lookup that begins with `step`.
+template <typename A, bool PAGED>
+__device__ __forceinline__ uint32_t own_key(uint32_t step, int lane) {
+  if (!PAGED) return step * A::KS + (uint32_t)lane;
+  return ((step + 4u * (uint32_t)(lane / A::NT)) * A::NT + (uint32_t)(lane % A::NT)) * 16u;
 }
+
+// Its entry in the table: independent of the sequence's length, so that both can be on their way at once.
+template <typename A, bool PAGED>
+__device__ __forceinline__ int look_up(const AttnArgs& a, const int32_t* table, uint32_t step, int lane) {
+  const uint32_t key = own_key<A, PAGED>(step, lane);
+  return key < (uint32_t)a.cap ? table[div_page(key, a.page)] : -1;
+}
+
+template <typename A, bool PAGED, bool FP8>
+__device__ __forceinline__ Places places_of(const AttnArgs& a, int entry, uint32_t step, int end, int lane) {
+  const uint32_t key = own_key<A, PAGED>(step, lane);
+  const bool ok = key < (uint32_t)end && (uint64_t)(uint32_t)entry < (uint64_t)a.pages && (PAGED || lane < A::KS);
+  const uint64_t page = ok ? (uint32_t)entry : 0u;
+  const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
+  Places p{};
+  p.there = __builtin_amdgcn_ballot_w64(ok);
+  p.k = page * (uint64_t)a.k_page + (uint64_t)off * a.k_token;
+  p.v = page * (uint64_t)a.v_page + (uint64_t)off * a.v_token;
+  if (FP8) {
+    p.ks = page * (uint64_t)a.ks_page + (uint64_t)off * a.ks_token;
+    p.vs = page * (uint64_t)a.vs_page + (uint64_t)off * a.vs_token;
+  }
+  return p;
+}
+
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return lo | (uint64_t)hi << 32;
+}
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)(v >> 32));
+  return lo | (uint64_t)hi << 32;
+}
+
+__device__ __forceinline__ uint32_t from_lane32(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)v);
+}
+
+// The step's bits of `there`: one a tile (PAGED) or a token.
+template <typename A, bool PAGED>
+__device__ __forceinline__ uint64_t step_bits(const Places& p, int slot) {
+  return PAGED ? (p.there >> (slot * A::NT)) & ((1u << A::NT) - 1u) : p.there;
+}
+
+// ------------------------------------------------------------------ loads
 
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
 __device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, const uint8_t* kh,
-                                       const float* ksh, uint32_t step, int end, int pages, int slot, int lane) {
+                                       const float* ksh, const Places& at, int slot, int lane) {
   using A = Attn<T, FP8, DP, PAGED, FULL>;
   const int c = lane & 15, g = lane >> 4;
-  constexpr int E = FP8 ? 1 : 2;
+  if (FP8 && !PAGED) s.ks1 = ksh[at.ks];
 #pragma unroll
   for (int i = 0; i < A::NT; ++i) {
     const uint8_t* base;
     if (PAGED) {
-      const int pg = __builtin_amdgcn_readlane(pages, slot * A::NT + i);
-      const uint32_t key = (step * A::NT + i) * 16u;
-      const bool ok = (uint32_t)pg < (uint64_t)a.pages;
-      s.hi[i] = ok ? end : 0;
-      const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
-      base = kh + (int64_t)(ok ? pg : 0) * a.k_page + (int64_t)off * a.k_token + (uint32_t)c * a.k_token;
-      if (FP8) {
-        const float* const sp = ksh + (int64_t)(ok ? pg : 0) * a.ks_page + (int64_t)off * a.ks_token;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s.ks[i][r] = sp[(uint32_t)(4 * g + r) * a.ks_token];
-      }
+      base = kh + of_lane(at.k, slot * A::NT + i) + (uint32_t)c * a.k_token;
+      if (FP8) s.ks[i] = *reinterpret_cast<const f4*>(ksh + of_lane(at.ks, slot * A::NT + i) + 4 * g);
     } else {
-      const int pg = __builtin_amdgcn_ds_bpermute((16 * i + c) * 4, pages);
-      const uint32_t key = step * A::KS + 16u * i + c;
-      const bool ok = (uint32_t)pg < (uint64_t)a.pages;
-      const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
-      base = kh + (int64_t)(ok ? pg : 0) * a.k_page + (int64_t)off * a.k_token;
-      if (FP8) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int pr = __builtin_amdgcn_ds_bpermute((16 * i + 4 * g + r) * 4, pages);
-          const uint32_t kr = step * A::KS + 16u * i + 4u * g + r;
-          const bool there = (uint32_t)pr < (uint64_t)a.pages;
-          const uint32_t o = there ? kr - div_page(kr, a.page) * a.page.page : 0u;
-          s.ks[i][r] = ksh[(int64_t)(there ? pr : 0) * a.ks_page + (int64_t)o * a.ks_token];
-        }
-      }
+      base = kh + from_lane(at.k, 16 * i + c);
     }
 #pragma unroll
     for (int w = 0; w < A::KW; ++w) {
       const int d0 = FP8 ? 64 * w + 16 * g : 32 * w + 8 * g;
       if (FULL) {
-        s.k[i][w] = *reinterpret_cast<const u4*>(base + d0 * E);
-      } else if (FP8) {  // rows of 8-byte alignment; channels past d from the row's start, cleared below
+        s.k[i][w] = *reinterpret_cast<const u4*>(base + d0 * A::E);
+      } else if (FP8) {  // rows of 8-byte alignment; channels past d from the row's start, cleared in scores()
         const u2 lo = *reinterpret_cast<const u2*>(base + (d0 < a.d ? d0 : 0));
         const u2 hi = *reinterpret_cast<const u2*>(base + (d0 + 8 < a.d ? d0 + 8 : 0));
         s.k[i][w] = u4{lo[0], lo[1], hi[0], hi[1]};
       } else {
-        s.k[i][w] = *reinterpret_cast<const u4*>(base + (d0 < a.d ? d0 : 0) * E);
+        s.k[i][w] = *reinterpret_cast<const u4*>(base + (d0 < a.d ? d0 : 0) * A::E);
       }
     }
   }
@@ -221,37 +251,25 @@ __device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, PAGED
 
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
 __device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, const uint8_t* vh,
-                                       const float* vsh, uint32_t step, int pages, int slot, int lane) {
+                                       const float* vsh, const Places& at, int slot, int lane) {
   using A = Attn<T, FP8, DP, PAGED, FULL>;
   const int c = lane & 15, g = lane >> 4;
-  constexpr int E = FP8 ? 1 : 2;
+  if (FP8 && !PAGED) s.vs1 = vsh[at.vs];
 #pragma unroll
   for (int i = 0; i < A::NT; ++i) {
+    const uint8_t* tile = nullptr;
+    if (PAGED) {
+      tile = vh + of_lane(at.v, slot * A::NT + i);
+      if (FP8) s.vs[i] = *reinterpret_cast<const f4*>(vsh + of_lane(at.vs, slot * A::NT + i) + 4 * g);
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint8_t* base;
-      const float* sp = nullptr;
-      if (PAGED) {
-        const int pg = __builtin_amdgcn_readlane(pages, slot * A::NT + i);
-        const uint32_t key = (step * A::NT + i) * 16u;
-        const bool ok = (uint32_t)pg < (uint64_t)a.pages;
-        const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
-        base = vh + (int64_t)(ok ? pg : 0) * a.v_page + (int64_t)(off + r) * a.v_token + (uint32_t)(4 * g) * a.v_token;
-        if (FP8)
-          sp = vsh + (int64_t)(ok ? pg : 0) * a.vs_page + (int64_t)off * a.vs_token + (uint32_t)(4 * g + r) * a.vs_token;
-      } else {
-        const int pg = __builtin_amdgcn_ds_bpermute((16 * i + 4 * g + r) * 4, pages);
-        const uint32_t key = step * A::KS + 16u * i + 4u * g + r;
-        const bool ok = (uint32_t)pg < (uint64_t)a.pages;
-        const uint32_t off = ok ? key - div_page(key, a.page) * a.page.page : 0u;
-        base = vh + (int64_t)(ok ? pg : 0) * a.v_page + (int64_t)off * a.v_token;
-        if (FP8) sp = vsh + (int64_t)(ok ? pg : 0) * a.vs_page + (int64_t)off * a.vs_token;
-      }
-      if (FP8) s.vs[i][r] = *sp;
+      const uint8_t* const base =
+          PAGED ? tile + (uint32_t)(4 * g + r) * a.v_token : vh + from_lane(at.v, 16 * i + 4 * g + r);
 #pragma unroll
       for (int n = 0; n < A::NSUB; ++n) {
         const int d0 = 128 * n + A::CS * c;
-        const uint8_t* const p = base + (FULL || d0 < a.d ? d0 : 0) * E;
+        const uint8_t* const p = base + (FULL || d0 < a.d ? d0 : 0) * A::E;
         if (A::VW == 4) {
           const u4 w = *reinterpret_cast<const u4*>(p);
 #pragma unroll
@@ -270,14 +288,21 @@ __device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, PAGED
 
 // ------------------------------------------------------------------ one step
 
+// Whether token 4g + r of tile i of the step takes part.
+template <typename A, bool PAGED>
+__device__ __forceinline__ bool takes_part(uint32_t step, int i, int r, int g, int begin, int end, uint64_t bits) {
+  const int key = (int)(step * A::KS + 16u * i + 4u * g + r);
+  return key >= begin && key < end && ((bits >> (PAGED ? i : 16 * i + 4 * g + r)) & 1u);
+}
+
 // Scores of the step's tokens, in units of log2, -inf where a token takes no part: x[tile][r] of head c, token
 // 4g + r.
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
 __device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, uint32_t step, int begin,
-                                       int end, int pages, int lane, float (&x)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
+                                       int end, uint64_t bits, int lane,
+                                       float (&x)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
   using A = Attn<T, FP8, DP, PAGED, FULL>;
   const int g = lane >> 4;
-  if (!PAGED) s.seen = 0;
 #pragma unroll
   for (int i = 0; i < A::NT; ++i) {
     f4 t = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -297,18 +322,9 @@ __device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int key = (int)(step * A::KS + 16u * i + 4u * g + r);
-      bool in = key >= begin;
-      if (PAGED) {
-        in = in && key < s.hi[i];
-      } else {
-        const int pg = __builtin_amdgcn_ds_bpermute((16 * i + 4 * g + r) * 4, pages);
-        in = in && key < end && (uint32_t)pg < (uint64_t)a.pages;
-        s.seen |= in ? 1u << (4 * i + r) : 0u;
-      }
       float y = t[r] * a.scale_log2;
-      if (FP8) y *= s.ks[i][r];
-      x[i][r] = in ? y : -__builtin_inff();
+      if (FP8) y *= PAGED ? s.ks[i][r] : as_f32((uint32_t)from_lane32(as_u32(s.ks1), 16 * i + 4 * g + r));
+      x[i][r] = takes_part<A, PAGED>(step, i, r, g, begin, end, bits) ? y : -__builtin_inff();
     }
   }
 }
@@ -346,24 +362,24 @@ __device__ __forceinline__ void softmax(Attn<T, FP8, DP, PAGED, FULL>& s,
 
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
 __device__ __forceinline__ void accumulate(Attn<T, FP8, DP, PAGED, FULL>& s, uint32_t step, int begin, int end,
-                                           int lane, float (&p)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
+                                           uint64_t bits, int lane,
+                                           float (&p)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
   using A = Attn<T, FP8, DP, PAGED, FULL>;
   const int g = lane >> 4;
-  // Values (and scales) of tokens that take no part may be anything: NaN times a probability of zero is NaN.
-  bool whole = (int)(step * A::KS) >= begin && (int)(step * A::KS) + A::KS <= end;
-  if (PAGED) {
+  if (FP8 && !PAGED) {
 #pragma unroll
-    for (int i = 0; i < A::NT; ++i) whole = whole && s.hi[i] != 0;
-  } else {
-    whole = whole && !__builtin_amdgcn_ballot_w64(s.seen != (1u << (4 * A::NT)) - 1u);
+    for (int i = 0; i < A::NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.vs[i][r] = as_f32(from_lane32(as_u32(s.vs1), 16 * i + 4 * g + r));
   }
-  if (!whole) {
+  // Values (and scales) of tokens that take no part may be anything: NaN times a probability of zero is NaN.
+  constexpr uint64_t kAll = PAGED || A::KS < 64 ? (uint64_t(1) << (PAGED ? A::NT : A::KS % 64)) - 1 : ~uint64_t(0);
+  if ((int)(step * A::KS) < begin || (int)(step * A::KS) + A::KS > end || bits != kAll) {
 #pragma unroll
     for (int i = 0; i < A::NT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int key = (int)(step * A::KS + 16u * i + 4u * g + r);
-        const bool in = PAGED ? key >= begin && key < s.hi[i] : (s.seen >> (4 * i + r)) & 1u;
+        const bool in = takes_part<A, PAGED>(step, i, r, g, begin, end, bits);
         if (FP8) s.vs[i][r] = in ? s.vs[i][r] : 0.0f;
 #pragma unroll
         for (int n = 0; n < A::NSUB; ++n)
@@ -420,34 +436,52 @@ __device__ __forceinline__ void store4(uint16_t* p, const f4& y) {
   *reinterpret_cast<u2*>(p) = u2{round_pair<T>(y[0], y[1]), round_pair<T>(y[2], y[3])};
 }
 
+template <int N>
+struct template_int {
+  static constexpr int value = N;
+};
+
+// Inclusive sums over a wave's lanes (all active): inside rows of 16, then each row's last lane into the rows behind.
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+  const auto shifted = [](uint32_t x, auto ctrl, auto rows) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  const template_int<0xF> all;
+  v += shifted(v, template_int<0x111>{}, all);  // row_shr 1, 2, 4, 8
+  v += shifted(v, template_int<0x112>{}, all);
+  v += shifted(v, template_int<0x114>{}, all);
+  v += shifted(v, template_int<0x118>{}, all);
+  v += shifted(v, template_int<0x142>{}, template_int<0xA>{});  // row_bcast 15 into rows 1 and 3
+  v += shifted(v, template_int<0x143>{}, template_int<0xC>{});  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
+__device__ __forceinline__ uint32_t scalar(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__global__ __launch_bounds__(256, DP > 128 && !FP8 ? 1 : 2) void attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP > 128 && !(FP8 && FULL) ? 1 : 2) void attention_kernel(AttnArgs a) {
   using A = Attn<T, FP8, DP, PAGED, FULL>;
   using S = Span<A::KS>;
   __shared__ float rows[A::kWaves][16][A::ROW];
   __shared__ float tops[A::kWaves][16], sums[A::kWaves][16];
-  __shared__ uint32_t found[4 + 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const uint32_t per = (uint32_t)(a.heads * a.row_groups);  // items of a sequence
 
   int b;
-  uint32_t item, at, left;  // item of sequence b, its next step, steps left of this workgroup
+  uint32_t item, at = 0, left;  // item of sequence b, its next step, steps left of this workgroup
   uint32_t share = 0;
   if (a.direct) {
     b = (int)(blockIdx.x / per);
     item = blockIdx.x - (uint32_t)b * per;
-    at = 0;
-    left = S(a, b).count;
+    left = ~0u;
   } else {
-    // All steps, then the sequence that holds this workgroup's first.
-    uint32_t n = 0;
-    for (int i = tid; i < a.m; i += 256) n += S(a, i).count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) n += (uint32_t)__shfl_xor((int)n, o);
-    if (lane == 0) found[wave] = n;
-    __syncthreads();
-    const uint32_t total = (found[0] + found[1] + found[2] + found[3]) * per;
+    // All steps, then the sequence that holds this workgroup's first: every wave for itself, a sequence a lane.
+    uint32_t own = lane < a.m ? S(a, lane).count : 0u, n = own;
+    for (int i = lane + 64; i < a.m; i += 64) n += S(a, i).count;
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(n), 63) * per;
     share = (total + gridDim.x - 1) / gridDim.x;
     share = share < a.least ? a.least : share;
     const uint64_t start = (uint64_t)blockIdx.x * share;
@@ -455,36 +489,25 @@ __global__ __launch_bounds__(256, DP > 128 && !FP8 ? 1 : 2) void attention_kerne
     left = total - (uint32_t)start < share ? total - (uint32_t)start : share;
     const uint32_t want = (uint32_t)start / per;
     uint32_t before = 0;
-    for (int i0 = 0; i0 < a.m; i0 += 256) {
-      uint32_t own = i0 + tid < a.m ? S(a, i0 + tid).count : 0u, incl = own;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t up = (uint32_t)__shfl_up((int)incl, o);
-        incl += lane >= o ? up : 0u;
+    for (int i0 = 0;; i0 += 64) {
+      if (i0) own = i0 + lane < a.m ? S(a, i0 + lane).count : 0u;
+      const uint32_t incl = before + wave_scan_u32(own);
+      const int lower = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= want));
+      if (lower < 64) {
+        b = i0 + lower;
+        const uint32_t count = (uint32_t)__builtin_amdgcn_readlane((int)own, lower);
+        const uint32_t rest =
+            (uint32_t)start - ((uint32_t)__builtin_amdgcn_readlane((int)incl, lower) - count) * per;
+        item = rest / count;
+        at = rest - item * count;
+        break;
       }
-      __syncthreads();
-      if (lane == 63) found[wave] = incl;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) incl += found[w];
-      incl += before;
-      if (incl - own <= want && want < incl) found[4] = (uint32_t)(i0 + tid), found[5] = incl - own;
-      before += found[0] + found[1] + found[2] + found[3];
-      if (want < before) break;
+      before = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
-    __syncthreads();
-    b = (int)found[4];
-    const uint32_t rest = (uint32_t)start - found[5] * per, count = S(a, b).count;
-    item = rest / count;
-    at = rest - item * count;
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  item = (uint32_t)__builtin_amdgcn_readfirstlane((int)item);
-  at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-  left = (uint32_t)__builtin_amdgcn_readfirstlane((int)left);
+  b = (int)scalar((uint32_t)b), item = scalar(item), at = scalar(at), left = scalar(left);
 
   for (;;) {
-    const S span(a, b);
-    const uint32_t stop = span.count - at < left ? span.count : at + left;  // steps [at, stop) of this item
     const int head = (int)(item / (uint32_t)a.row_groups), rg = (int)(item - (uint32_t)head * a.row_groups);
     const int nrows = a.group - 16 * rg < 16 ? a.group - 16 * rg : 16;
     const int q0 = head * a.group + 16 * rg;
@@ -494,60 +517,48 @@ __global__ __launch_bounds__(256, DP > 128 && !FP8 ? 1 : 2) void attention_kerne
     const float* const ksh = FP8 ? a.ks + head * a.ks_head : nullptr;
     const float* const vsh = FP8 ? a.vs + head * a.vs_head : nullptr;
 
+    const S span(a, b);
+    const uint32_t stop = span.count - at < left ? span.count : at + left;  // steps [at, stop) of this item
+    uint32_t step = (a.window ? span.first : 0u) + at + (uint32_t)wave;
+    const uint32_t last = span.first + stop;
+    int entry = look_up<A, PAGED>(a, table, step, lane);
     A s;
     s.top = -__builtin_inff(), s.sum = 0.0f;
+    const uint16_t* const qp = a.q + (int64_t)b * a.q_row + (int64_t)(q0 + (c < nrows ? c : 0)) * a.q_head;
+#pragma unroll
+    for (int j = 0; j < A::NK; ++j) {
+      const int d0 = A::k_at(j, g);
+      s.q[j] = *reinterpret_cast<const u4*>(qp + (FULL || d0 < a.d ? d0 : 0));
+    }
 #pragma unroll
     for (int j = 0; j < A::NSUB * A::CS; ++j) s.acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t step = span.first + at + (uint32_t)wave;
-    const uint32_t last = span.first + stop;
     if (step < last) {
-      const uint16_t* const qp = a.q + (int64_t)b * a.q_row + (int64_t)(q0 + (c < nrows ? c : 0)) * a.q_head;
 #pragma unroll
-      for (int j = 0; j < A::NK; ++j) {
-        const int d0 = A::k_at(j, g);
-        s.q[j] = u4{0u, 0u, 0u, 0u};
-        if (c < nrows && (FULL || d0 < a.d)) s.q[j] = *reinterpret_cast<const u4*>(qp + d0);
-      }
-      constexpr int kAhead = 64 / A::NT;  // PAGED: steps whose pages one fetch holds
-      int pages = PAGED ? fetch_pages<A>(a, table, step, span.end, lane, A::NT) : 0, next = 0;
-      const auto lookup = [&](uint32_t st) {
-        const uint32_t key = st * A::KS + (uint32_t)lane;
-        return lane < A::KS && (int64_t)key < span.end && st < last ? table[div_page(key, a.page)] : -1;
-      };
-      if (!PAGED) pages = lookup(step), next = lookup(step + 4);
+      for (int j = 0; j < A::NK; ++j)
+        if (c >= nrows || (!FULL && A::k_at(j, g) >= a.d)) s.q[j] = u4{0u, 0u, 0u, 0u};
+      Places at_k = places_of<A, PAGED, FP8>(a, entry, step, span.end, lane);
       int slot = 0;
+      entry = look_up<A, PAGED>(a, table, step + 4 * A::kAhead, lane);
       float x[A::NT][4];
-      load_k(a, s, kh, ksh, step, span.end, pages, slot, lane);
-      load_v(a, s, vh, vsh, step, pages, slot, lane);
+      load_k(a, s, kh, ksh, at_k, slot, lane);
+      load_v(a, s, vh, vsh, at_k, slot, lane);
       for (; step + 4 < last; step += 4) {
-        scores(a, s, step, span.begin, span.end, pages, lane, x);
-        int hi[A::NT];
-        if (PAGED) {
-#pragma unroll
-          for (int i = 0; i < A::NT; ++i) hi[i] = s.hi[i];
+        const uint64_t bits = step_bits<A, PAGED>(at_k, slot);
+        scores(a, s, step, span.begin, span.end, bits, lane, x);
+        if (++slot == A::kAhead) {
+          slot = 0;
+          at_k = places_of<A, PAGED, FP8>(a, entry, step + 4, span.end, lane);
+          entry = look_up<A, PAGED>(a, table, step + 4 + 4 * A::kAhead, lane);
         }
-        if (PAGED) {
-          if (++slot == kAhead) slot = 0, pages = fetch_pages<A>(a, table, step + 4, span.end, lane, A::NT);
-        } else {
-          pages = next, next = lookup(step + 8);
-        }
-        load_k(a, s, kh, ksh, step + 4, span.end, pages, slot, lane);
-        int hi_next[A::NT];
-        if (PAGED) {
-#pragma unroll
-          for (int i = 0; i < A::NT; ++i) hi_next[i] = s.hi[i], s.hi[i] = hi[i];
-        }
+        load_k(a, s, kh, ksh, at_k, slot, lane);
         softmax(s, x);
-        accumulate(s, step, span.begin, span.end, lane, x);
-        if (PAGED) {
-#pragma unroll
-          for (int i = 0; i < A::NT; ++i) s.hi[i] = hi_next[i];
-        }
-        load_v(a, s, vh, vsh, step + 4, pages, slot, lane);
+        accumulate(s, step, span.begin, span.end, bits, lane, x);
+        load_v(a, s, vh, vsh, at_k, slot, lane);
       }
-      scores(a, s, step, span.begin, span.end, pages, lane, x);
+      const uint64_t bits = step_bits<A, PAGED>(at_k, slot);
+      scores(a, s, step, span.begin, span.end, bits, lane, x);
       softmax(s, x);
-      accumulate(s, step, span.begin, span.end, lane, x);
+      accumulate(s, step, span.begin, span.end, bits, lane, x);
     }
 
     // The waves' parts: one maximum, then their rows side by side.

@@ -11,61 +11,91 @@ struct JoinArgs {
   const int32_t* lens;
   uint16_t* out;
   int heads, group, row_groups, part_rows, d, dp;
+  uint32_t count;  // sequences * query heads
 };
 
-// A workgroup per sequence and query head: out = sum_p acc_p 2^(top_p - top) / sum_p sum_p 2^(top_p - top) over the
-// pieces p that the attention's workgroups left, in their order. Items that one workgroup held are done already;
-// sequences without tokens get zeros here.
-template <typename T>
+// Part of a row: its channels y of a lane, in units of 2^top, and the sum l of the probabilities.
+struct Part {
+  float top, l;
+  f4 y;
+};
+
+__device__ __forceinline__ void merge(Part& a, float top, float l, const f4& y) {
+  const float t = __builtin_fmaxf(a.top, top);
+  const float fa = a.top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(a.top - t);
+  const float fb = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - t);
+  a.l = a.l * fa + l * fb;
+  a.y = a.y * fa + y * fb;
+  a.top = t;
+}
+
+// out = sum_p acc_p 2^(top_p - top) / sum_p sum_p 2^(top_p - top) of a sequence's query head over the pieces p that
+// the attention's workgroups left, by one wave (WAVES 1) or a workgroup of 4. dp / 4 lanes take a piece; a wave takes
+// 64 / (dp / 4) side by side, four of each at once, and the parts are merged in an order that depends on the number
+// of pieces alone. Items that one workgroup held are done already; sequences without tokens get zeros here.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
-  __shared__ float acc[4][TF_KV_MAX_HEAD_DIM];
-  __shared__ float sums[4];
+  __shared__ Part parts[WAVES][64];
+  constexpr int kOnce = 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int q_heads = a.heads * a.group;
-  const int b = (int)(blockIdx.x / (uint32_t)q_heads), qh = (int)(blockIdx.x - (uint32_t)b * q_heads);
-  uint16_t* const out = a.out + (int64_t)blockIdx.x * a.d;
-  if (a.lens[b] <= 0) {
-    for (int e = tid * 8; e < a.d; e += 256 * 8) *reinterpret_cast<u4*>(out + e) = u4{0u, 0u, 0u, 0u};
+  const uint32_t q_heads = (uint32_t)(a.heads * a.group);
+  const uint32_t at = WAVES == 1 ? blockIdx.x * 4 + (uint32_t)wave : blockIdx.x;
+  if (at >= a.count) return;
+  const int b = (int)(at / q_heads), qh = (int)(at - (uint32_t)b * q_heads);
+  const int head = qh / a.group, in = qh - head * a.group, rg = in >> 4, row = in & 15;
+  const int n = a.lens[b];
+  const int2 ends = a.ends[((int64_t)b * a.heads + head) * a.row_groups + rg];
+  const int lanes = a.dp >> 2, side = 64 / lanes, part = lane / lanes, e = (lane & (lanes - 1)) * 4;
+  uint16_t* const out = a.out + (int64_t)at * a.d;
+  const bool writes = (WAVES == 1 || wave == 0) && part == 0 && e < a.d;
+  if (n <= 0) {
+    if (writes) *reinterpret_cast<u2*>(out + e) = u2{0u, 0u};
     return;
   }
-  const int head = qh / a.group, in = qh - head * a.group, rg = in >> 4, row = in & 15;
-  const int2 ends = a.ends[((int64_t)b * a.heads + head) * a.row_groups + rg];
   if (ends.x == ends.y) return;
   const int64_t size = (int64_t)a.part_rows * (a.dp + 2);
-  const auto piece = [&](int p) { return a.part + (2 * (int64_t)p + (p == ends.x ? 1 : 0)) * size; };
-  const auto pair = [&](int p) {
-    return *reinterpret_cast<const float2*>(piece(p) + a.part_rows * a.dp + 2 * row);
-  };
-  float top = -__builtin_inff();
-  for (int p = ends.x + lane; p <= ends.y; p += 64) top = __builtin_fmaxf(top, pair(p).x);
+  Part mine{-__builtin_inff(), 0.0f, f4{0.0f, 0.0f, 0.0f, 0.0f}};
+  const int each = WAVES * side;
+  for (int p0 = ends.x + (WAVES == 1 ? 0 : wave) * side + part; p0 <= ends.y; p0 += each * kOnce) {
+    float2 tl[kOnce];
+    f4 y[kOnce];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
-  float l = 0.0f;
-  f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int e = lane * 4;
-  for (int p = ends.x + wave; p <= ends.y; p += 4) {
-    const float2 tl = pair(p);
-    const float f = tl.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(tl.x - top);
-    l += tl.y * f;
-    if (e < a.d) y += *reinterpret_cast<const f4*>(piece(p) + row * a.dp + e) * f;
+    for (int i = 0; i < kOnce; ++i) {
+      const int p = p0 + i * each <= ends.y ? p0 + i * each : p0;
+      const float* const piece = a.part + (2 * (int64_t)p + (p == ends.x ? 1 : 0)) * size;
+      tl[i] = *reinterpret_cast<const float2*>(piece + a.part_rows * a.dp + 2 * row);
+      y[i] = *reinterpret_cast<const f4*>(piece + row * a.dp + e);
+    }
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i)
+      if (p0 + i * each <= ends.y) merge(mine, tl[i].x, tl[i].y, y[i]);
   }
-  if (e < a.d) *reinterpret_cast<f4*>(&acc[wave][e]) = y;
-  if (lane == 0) sums[wave] = l;
-  __syncthreads();
-  if (wave != 0 || e >= a.d) return;
-  l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  const auto at = [&](int w) { return *reinterpret_cast<const f4*>(&acc[w][e]); };
-  y = (at(0) + at(1)) + (at(2) + at(3));
-  store4<T>(out + e, y * (l == 0.0f ? 0.0f : 1.0f / l));
+  for (int o = lanes; o < 64; o <<= 1) {
+    const float t = __shfl_xor(mine.top, o), l = __shfl_xor(mine.l, o);
+    f4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __shfl_xor(mine.y[j], o);
+    merge(mine, t, l, y);
+  }
+  if (WAVES > 1) {
+    parts[wave % WAVES][lane] = mine;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) merge(mine, parts[w][lane].top, parts[w][lane].l, parts[w][lane].y);
+  }
+  if (writes) store4<T>(out + e, mine.y * (mine.l == 0.0f ? 0.0f : 1.0f / mine.l));
 }
+
+constexpr uint32_t kJoinByWave = 1024;  // rows from which a wave each fills the CUs
 
 bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Sizes of a call, and "" or what is wrong with them.
 struct Plan {
   int dp, group, row_groups, part_rows;
-  int64_t items, cap, part_floats;
-  bool fp8;
+  int64_t items, cap, part_floats, bytes;
+  bool fp8, direct;
 };
 
 std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t width, Plan& p) {
@@ -81,7 +111,9 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
   p.cap = width * c.page_size;
   if (m * q_heads > 0x7FFFFF || p.items * cdiv(p.cap, 16) > 0x7FFFFFFF)
     return "more sequences, heads and tokens of block_table than 2^31 steps of 16";
-  p.part_floats = 2 * (int64_t)kAttnGrid * p.part_rows * (p.dp + 2);
+  p.direct = p.cap <= 4 * attention_step(p.fp8, p.dp);
+  p.part_floats = p.direct ? 0 : 2 * (int64_t)kAttnGrid * p.part_rows * (p.dp + 2);
+  p.bytes = p.direct ? 0 : p.part_floats * 4 + p.items * 8;
   return "";
 }
 
@@ -95,7 +127,7 @@ extern "C" int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, 
   Plan p;
   if (!cache || !kv_cache_error(cache, cache->dtype == TF_DTYPE_E4M3 ? TF_DTYPE_FP16 : cache->dtype).empty()) return -1;
   if (!plan_of(*cache, m, q_heads, width, p).empty()) return -1;
-  return p.part_floats * 4 + p.items * 8;
+  return p.bytes;
 }
 
 extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, int64_t q_row, int64_t q_head,
@@ -114,10 +146,9 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
   Plan p;
   const std::string wrong = plan_of(c, m, q_heads, width, p);
   if (!wrong.empty()) return bad(wrong);
-  const int64_t need = p.part_floats * 4 + p.items * 8;
-  if (!workspace || workspace_bytes < need)
-    return bad("workspace too small (" + std::to_string(workspace_bytes) + " < " + std::to_string(need) + ")");
-  if (!multiple(workspace, 16)) return bad("workspace not 16-byte aligned");
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return bad("workspace too small (" + std::to_string(workspace_bytes) + " < " + std::to_string(p.bytes) + ")");
+  if (p.bytes > 0 && !multiple(workspace, 16)) return bad("workspace not 16-byte aligned");
   if (m == 0) return TF_OK;
   const int size = p.fp8 ? 1 : 2;
   AttnArgs a{};
@@ -134,8 +165,13 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
   a.m = (int)m, a.heads = c.heads, a.group = p.group, a.row_groups = p.row_groups, a.part_rows = p.part_rows;
   a.d = c.head_dim, a.cap = (int)p.cap, a.window = window, a.scale_log2 = scale * 1.44269504088896341f;
   a.least = 4;
-  a.direct = p.cap <= 4 * attention_step(p.fp8, p.dp);
-  const bool paged = c.page_size % 16 == 0;
+  a.direct = p.direct;
+  bool paged = c.page_size % 16 == 0;
+  if (p.fp8) {  // a tile's scales go by 16-byte loads
+    paged = paged && multiple(c.k_scale, 16) && multiple(c.v_scale, 16);
+    for (const int64_t* st : {c.k_scale_strides, c.v_scale_strides})
+      paged = paged && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] == 1;
+  }
   bool full = c.head_dim == p.dp;
   if (p.fp8) {  // whole rows go by 16-byte loads
     full = full && multiple(c.k, 16);
@@ -147,10 +183,12 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
   const auto launch = p.dp == 64 ? launch_attention_d64 : p.dp == 128 ? launch_attention_d128 : launch_attention_d256;
   if (int rc = launch(a, bf16, p.fp8, paged, full, grid, s)) return rc;
   if (a.direct) return TF_OK;
-  const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp};
-  if (bf16)
-    join_kernel<BF16><<<(unsigned)(m * q_heads), 256, 0, s>>>(j);
+  const auto count = (uint32_t)(m * q_heads);
+  const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp, count};
+  if (count >= kJoinByWave)
+    bf16 ? join_kernel<BF16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j)
+         : join_kernel<F16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j);
   else
-    join_kernel<F16><<<(unsigned)(m * q_heads), 256, 0, s>>>(j);
+    bf16 ? join_kernel<BF16, 4><<<count, 256, 0, s>>>(j) : join_kernel<F16, 4><<<count, 256, 0, s>>>(j);
   return check_launch("tf_paged_attention");
 }

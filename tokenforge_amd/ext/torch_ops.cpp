@@ -865,12 +865,14 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
                                     block_table, seq_lens, scale, window);
   c10::OptionalDeviceGuard guard(dev);
   at::Tensor out = fresh(q.sizes(), q.scalar_type(), dev);
-  at::Tensor work = fresh({(need + 3) / 4}, at::kFloat, dev);
+  at::Tensor work;
+  if (need > 0) work = fresh({(need + 3) / 4}, at::kFloat, dev);
   check(api().attention(&c, data<const uint16_t>(q), step_of(q, 0), step_of(q, 1), static_cast<int32_t>(q.size(1)),
                         dtype_code(q.scalar_type()), data<const int32_t>(block_table), step_of(block_table, 0),
                         block_table.size(1), data<const int32_t>(seq_lens), q.size(0), static_cast<float>(scale),
                         static_cast<int32_t>(std::min<int64_t>(win, 0x7FFFFFFF)), data<uint16_t>(out),
-                        data<float>(work), need, c10::hip::getCurrentHIPStream(dev.index()).stream()),
+                        work.defined() ? data<float>(work) : nullptr, need,
+                        c10::hip::getCurrentHIPStream(dev.index()).stream()),
         "tf_paged_attention");
   return out;
 }
