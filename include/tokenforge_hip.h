@@ -401,7 +401,8 @@ int tf_kv_cache_read(const tf_kv_cache* cache, const int64_t* slots, uint16_t* k
  * summed in fp32, probabilities carry 16 bits or more into the second product.
  * workspace: fp32, 16-byte aligned, >= tf_paged_attention_workspace_bytes (-1 for sizes the attention refuses).
  * Two calls that may overlap need workspaces of their own. */
-int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads, int64_t width);
+int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads, int64_t width,
+                                           int32_t window);
 int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, int64_t q_row, int64_t q_head, int32_t q_heads,
                        int32_t dtype, const int32_t* block_table, int64_t table_stride, int64_t width,
                        const int32_t* seq_lens, int64_t m, float scale, int32_t window, uint16_t* out,

@@ -21,13 +21,12 @@ def rotate(x: np.ndarray, cos_sin: np.ndarray, positions: np.ndarray, interleave
 def tokens(cache: np.ndarray, scale: np.ndarray | None, table: np.ndarray, begin: int, end: int) -> np.ndarray:
     """Tokens ``[begin, end)`` of a sequence ``[n, heads, d]``, those of a page that is not there left out."""
     pages, _, page, _ = cache.shape
-    rows = []
-    for i in range(begin, end):
-        p = int(table[i // page])
-        if 0 <= p < pages:
-            x = cache[p, :, i % page].astype(np.float64)
-            rows.append(x if scale is None else x * scale[p, :, i % page].astype(np.float64)[:, None])
-    return np.stack(rows) if rows else np.zeros((0, cache.shape[1], cache.shape[3]))
+    i = np.arange(begin, end)
+    at = table[i // page].astype(np.int64)
+    there = (at >= 0) & (at < pages)
+    at, off = at[there], i[there] % page
+    x = cache[at, :, off].astype(np.float64)
+    return x if scale is None else x * scale[at, :, off].astype(np.float64)[..., None]
 
 
 def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, scale: float) -> tuple[np.ndarray, ...]:

@@ -22,6 +22,9 @@ def _queries(m: int, q_heads: int, d: int, dtype: torch.dtype, seed: int = 0) ->
     return q.to(dtype)
 
 
+LINE = 1 << 15  # tokens of a table's row from which items share workgroups, whatever the sequences' lengths
+
+
 def _run(device, lens, heads, group, d, page, dtype, fp8, window=0, width=None, tokens_first=False, scale=None, seed=0):  # type: ignore[no-untyped-def]
     table, pages = kc.tables(lens, page, width, seed)
     c = kc.cache(pages, heads, page, d, dtype, fp8, seed, tokens_first)
@@ -40,8 +43,9 @@ LENS = [[1], [0], [16], [17], [33, 0, 64, 65, 1], [300, 5, 129, 0], [1500], [700
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize("lens", LENS, ids=str)
 @pytest.mark.parametrize("d", [64, 128, 256])
-def test_lengths(d: int, lens: list[int], dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
-    _run(device, lens, 2, 7, d, 16, dtype, fp8)
+@pytest.mark.parametrize("capacity", [0, LINE])
+def test_lengths(capacity: int, d: int, lens: list[int], dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
+    _run(device, lens, 2, 7, d, 16, dtype, fp8, width=capacity // 16)
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
@@ -49,6 +53,7 @@ def test_lengths(d: int, lens: list[int], dtype: torch.dtype, fp8: bool, device:
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_page_sizes(d: int, page: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     _run(device, [200, 1, 77], 2, 4, d, page, dtype, fp8)
+    _run(device, [200, 1, 77], 2, 4, d, page, dtype, fp8, width=LINE // page)
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
@@ -56,12 +61,14 @@ def test_page_sizes(d: int, page: int, dtype: torch.dtype, fp8: bool, device: to
 @pytest.mark.parametrize("page", [16, 24])
 def test_odd_head_lengths(page: int, d: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     _run(device, [150, 31, 400], 3, 2, d, page, dtype, fp8)
+    _run(device, [150, 31, 400], 3, 2, d, page, dtype, fp8, width=LINE // page)
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize(("heads", "group"), [(1, 1), (12, 1), (1, 16), (2, 17), (1, 71), (5, 3)])
 def test_head_layouts(heads: int, group: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     _run(device, [333, 40], heads, group, 128, 16, dtype, fp8)
+    _run(device, [333, 40], heads, group, 128, 16, dtype, fp8, width=LINE // 16)
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
@@ -69,24 +76,36 @@ def test_head_layouts(heads: int, group: int, dtype: torch.dtype, fp8: bool, dev
 @pytest.mark.parametrize("page", [16, 24])
 def test_windows(page: int, window: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     _run(device, [400, 99, 16, 0, 1], 2, 4, 128, page, dtype, fp8, window=window)
+    _run(device, [9000, 99, 16, 0, 1], 2, 4, 128, page, dtype, fp8, window=12 * window)
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize("d", [64, 128])
 def test_long_sequences_and_large_batches(d: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     _run(device, [9001, 3], 2, 7, d, 16, dtype, fp8)
-    # more sequences than threads of a workgroup, empty ones at both ends
+    # more sequences than a workgroup has threads, and than the grid has workgroups; empty ones at both ends
     lens = [0, 0] + [(37 * i) % 91 for i in range(598)] + [0]
     _run(device, lens, 1, 2, d, 16, dtype, fp8, width=40)
+    _run(device, lens, 1, 2, d, 16, dtype, fp8, width=LINE // 16)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lens", [[180000, 0, 90000], [1000] * 100, [5000, 70, 9000, 3, 33, 12000] * 3], ids=["2", "100", "18"])
+def test_every_way_to_share_the_work(lens: list[int], fp8: bool, device: torch.device) -> None:
+    """Parts of 4 to 32 steps an item, and parts that begin and end inside items, of many lengths."""
+    for d in (64, 136):
+        _run(device, lens, 1 if len(lens) < 10 else 3, 3, d, 64, torch.bfloat16, fp8, width=180000 // 64 + 1)
+        _run(device, lens[:1] + lens[-1:], 1, 3, d, 64, torch.bfloat16, fp8)
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize("page", [16, 8])
-def test_layouts(page: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
+@pytest.mark.parametrize("capacity", [0, LINE])
+def test_layouts(capacity: int, page: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     """Caches laid out by token, keys and values in one tensor, strided queries, tables, lengths: the results of
     contiguous copies, bit for bit."""
     lens, heads, group, d = [210, 64, 0, 700], 2, 4, 128
-    table, pages = kc.tables(lens, page)
+    table, pages = kc.tables(lens, page, capacity // page)
     c = kc.cache(pages, heads, page, d, dtype, fp8)
     q = _queries(4, heads * group, d, dtype).to(device)
     n = torch.tensor(lens, dtype=torch.int32, device=device)
@@ -119,12 +138,13 @@ def test_layouts(page: int, dtype: torch.dtype, fp8: bool, device: torch.device)
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize("page", [16, 24])
 @pytest.mark.parametrize("d", [64, 80, 128, 256])
-def test_nothing_outside_a_sequence_takes_part(d: int, page: int, dtype: torch.dtype, fp8: bool,
+@pytest.mark.parametrize("capacity", [0, LINE])
+def test_nothing_outside_a_sequence_takes_part(capacity: int, d: int, page: int, dtype: torch.dtype, fp8: bool,
                                                device: torch.device) -> None:
     """NaN and infinities behind the last token, before the window and in every other page; entries of the table
     behind the last page that lead nowhere; lengths beyond the table and below zero."""
     lens, window = [77, 1, 130, 0, 250], 60
-    table, pages = kc.tables(lens, page)
+    table, pages = kc.tables(lens, page, capacity // page)
     c = kc.cache(pages, 2, page, d, dtype, fp8)
     q = _queries(5, 4, d, dtype)
     used = torch.zeros((pages, page), dtype=torch.bool)
@@ -141,13 +161,15 @@ def test_nothing_outside_a_sequence_takes_part(d: int, page: int, dtype: torch.d
             s.copy_(torch.where(used[:, None], s, float("inf")))
     wild = table.clone()
     for b, n in enumerate(lens):
-        wild[b, -(-n // page):] = torch.tensor([2**31 - 1, -(2**31), pages, -1] * 100)[: wild.shape[1] - -(-n // page)]
+        wild[b, -(-n // page):] = torch.tensor([2**31 - 1, -(2**31), pages, -1] * LINE)[: wild.shape[1] - -(-n // page)]
     out = ops.paged_attention(q.to(device), *c.to(device), wild.to(device),
                               torch.tensor(lens, dtype=torch.int32, device=device), d**-0.5, window)
     for x in (c.k, c.v):  # finite for the oracle, which multiplies them by nothing
         bits = x.view(torch.uint8 if fp8 else torch.int16)
         bits.copy_(torch.where(used[:, None, :, None], bits, torch.zeros_like(bits)))
     kc.check_attention(out, q, c, table, lens, d**-0.5, window)
+    if capacity:
+        return
     # lengths past the table end with it, lengths below zero are none
     far = torch.tensor([2**31 - 1, -5, 130, -(2**31), 250], dtype=torch.int32, device=device)
     c = kc.cache(pages, 2, page, d, dtype, fp8)
@@ -157,11 +179,12 @@ def test_nothing_outside_a_sequence_takes_part(d: int, page: int, dtype: torch.d
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize("page", [16, 24])
-def test_pages_that_are_not_there(page: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
+@pytest.mark.parametrize("capacity", [0, LINE])
+def test_pages_that_are_not_there(capacity: int, page: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
     """Page numbers outside the cache inside a sequence: their tokens take no part; a sequence of such pages alone
     gives zeros."""
     lens = [200, 90, 48]
-    table, pages = kc.tables(lens, page)
+    table, pages = kc.tables(lens, page, capacity // page)
     table[0, 1], table[0, 3], table[1, 0] = -1, pages, 2**31 - 1
     table[2] = -7
     c = kc.cache(pages, 2, page, 128, dtype, fp8)

@@ -303,16 +303,17 @@ def test_c_entries_refuse_before_any_launch() -> None:
         (attend, {"heads": 3}, b"multiple"), (attend, {"heads": 0}, b"multiple"), (attend, {"table": None}, b"null"),
         (attend, {"lens": None}, b"null"), (attend, {"width": -1}, b"size"), (attend, {"m": -1}, b"size"),
         (attend, {"width": 1 << 27}, b"2^31"), (attend, {"width": 1 << 62}, b"2^31"),
-        (attend, {"m": 1 << 22}, b"2^31"), (attend, {"window": -1}, b"window"), (attend, {"ws": None, "width": 40}, b"workspace"),
-        (attend, {"ws": x + 4, "width": 40}, b"16-byte"), (attend, {"size": 64, "width": 40}, b"workspace too small"), (attend, {"stride": -4}, b"negative"),
+        (attend, {"m": 1 << 22}, b"2^31"), (attend, {"window": -1}, b"window"), (attend, {"ws": None, "width": 4000}, b"workspace"),
+        (attend, {"ws": x + 4, "width": 4000}, b"16-byte"), (attend, {"size": 64, "width": 4000}, b"workspace too small"), (attend, {"stride": -4}, b"negative"),
     ]:
         assert call(ok, **changed) == _lib.TF_EINVAL
         assert message in h.tf_last_error(), (call.__name__, changed, h.tf_last_error())
     assert write(ok, t=0) == rope(ok, t=0) == read(ok, t=0) == attend(ok, m=0) == _lib.TF_OK
     assert write(None) == rope(None) == read(None) == attend(None) == _lib.TF_EINVAL
     need = h.tf_paged_attention_workspace_bytes
-    assert need(ok, 2, 4, 40) > 0 and need(ok, 2, 4, 1) == 0 and need(ok, 2, 3, 4) == need(None, 2, 4, 4) == need(ok, 2, 4, 1 << 40) == -1
-    assert need(ok, -1, 4, 4) == need(ok, 1 << 40, 4, 4) == need(_c_cache(head_dim=4), 2, 4, 4) == -1
+    assert need(ok, 2, 4, 4000, 0) > 0 and need(ok, 2, 4, 4000, 100) == need(ok, 2, 4, 1, 0) == need(ok, 0, 4, 40, 0) == 0
+    assert need(ok, 2, 3, 4, 0) == need(None, 2, 4, 4, 0) == need(ok, 2, 4, 1 << 40, 0) == need(ok, 2, 4, 4, -1) == -1
+    assert need(ok, -1, 4, 4, 0) == need(ok, 1 << 40, 4, 4, 0) == need(_c_cache(head_dim=4), 2, 4, 4, 0) == -1
 
 
 def test_page_division_is_exact() -> None:

@@ -148,7 +148,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [ctypes.POINTER(TfKvCache), _p, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i32, _i32,
          _p, _p, _p, _i64, _p]),
     "tf_kv_cache_read": (ctypes.c_int, [ctypes.POINTER(TfKvCache), _p, _p, _p, _i32, _i64, _p]),
-    "tf_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(TfKvCache), _i64, _i32, _i64]),
+    "tf_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(TfKvCache), _i64, _i32, _i64, _i32]),
     "tf_paged_attention": (
         ctypes.c_int,
         [ctypes.POINTER(TfKvCache), _p, _i64, _i64, _i32, _i32, _p, _i64, _i64, _p, _i64, _f32, _i32, _p, _p, _i64,

@@ -257,12 +257,13 @@ def paged_attention(q: torch.Tensor, cache: Cache, block_table: torch.Tensor, se
         block_table = block_table.contiguous()
     c = to_c_cache(cache)
     width = block_table.shape[1]
-    need = int(_lib.lib().tf_paged_attention_workspace_bytes(ctypes.byref(c), m, q.shape[1], width))
+    window = min(window, 0x7FFFFFFF)
+    need = int(_lib.lib().tf_paged_attention_workspace_bytes(ctypes.byref(c), m, q.shape[1], width, window))
     ws = torch.empty((need + 3) // 4, dtype=torch.float32, device=dev) if need > 0 else None
     with on_device(dev):
         rc = _lib.lib().tf_paged_attention(
             ctypes.byref(c), q.data_ptr(), *_two(q), q.shape[1], DTYPES[q.dtype], block_table.data_ptr(),
             block_table.stride(0) if m > 1 else 0, width, seq_lens.data_ptr(), m, float(scale),
-            min(window, 0x7FFFFFFF), out.data_ptr(), ptr(ws), need, stream_of(dev))
+            window, out.data_ptr(), ptr(ws), need, stream_of(dev))
     _lib.check(rc, "tf_paged_attention")
     return out

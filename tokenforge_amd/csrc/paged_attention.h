@@ -48,17 +48,29 @@ struct AttnArgs {
   int cap;     // tokens a row of the table covers
   int window;
   float scale_log2;
-  uint32_t least;  // fewest steps of a workgroup
-  int direct;      // a workgroup an item, whole
+  int direct;  // a workgroup takes a whole item; else the items' steps lie on one line
 };
 
-constexpr int kAttnGrid = 512;
+// Tokens of a step. Two tiles make the second product's k; four where a tile is 2 KB or less (heads up to 64), whose
+// steps would end before the next one's loads are back.
+constexpr int attention_step(int dp) { return dp == 64 ? 64 : 32; }
+
+// Workgroups a CU holds, and the grid of the shared line: two by their 180 to 190 registers, one for heads past 128.
+constexpr int attention_resident(int dp) { return dp > 128 ? 1 : 2; }
+constexpr int attention_grid(int dp) { return 256 * attention_resident(dp); }
+
+// Where a workgroup leaves its part of an item: it has at most two such, of an item that began before it and of one
+// that begins in it and goes on behind it.
+__host__ __device__ __forceinline__ int64_t piece_of(int workgroup, bool begins) {
+  return 2 * (int64_t)workgroup + (begins ? 1 : 0);
+}
 
 // Tokens [begin, end) of sequence b, and its steps of KS tokens.
 template <int KS>
 struct Span {
   int begin, end;
   uint32_t first, count;
+  __device__ __forceinline__ Span(int b, int e, uint32_t f, uint32_t c) : begin(b), end(e), first(f), count(c) {}
   __device__ __forceinline__ Span(const AttnArgs& a, int b) {
     int n = a.lens[b];
     n = n < 0 ? 0 : n > a.cap ? a.cap : n;
@@ -127,7 +139,7 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
 struct Attn {
   static constexpr int kWaves = 4;
-  static constexpr int NT = DP == 64 || (FP8 && DP == 128) ? 4 : 2;  // tiles of 16 tokens a step
+  static constexpr int NT = attention_step(DP) / 16;  // tiles of 16 tokens a step
   static constexpr int KS = 16 * NT;
   static constexpr int NK = DP / 32;                  // MFMAs over the channels
   static constexpr int NSUB = DP > 128 ? DP / 128 : 1;
@@ -295,6 +307,13 @@ __device__ __forceinline__ bool takes_part(uint32_t step, int i, int r, int g, i
   return key >= begin && key < end && ((bits >> (PAGED ? i : 16 * i + 4 * g + r)) & 1u);
 }
 
+// Whether all tokens of the step take part (uniform).
+template <typename A, bool PAGED>
+__device__ __forceinline__ bool all_take_part(uint32_t step, int begin, int end, uint64_t bits) {
+  constexpr uint64_t kAll = PAGED || A::KS < 64 ? (uint64_t(1) << (PAGED ? A::NT : A::KS % 64)) - 1 : ~uint64_t(0);
+  return (int)(step * A::KS) >= begin && (int)(step * A::KS) + A::KS <= end && bits == kAll;
+}
+
 // Scores of the step's tokens, in units of log2, -inf where a token takes no part: x[tile][r] of head c, token
 // 4g + r.
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
@@ -324,9 +343,15 @@ __device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED
     for (int r = 0; r < 4; ++r) {
       float y = t[r] * a.scale_log2;
       if (FP8) y *= PAGED ? s.ks[i][r] : as_f32((uint32_t)from_lane32(as_u32(s.ks1), 16 * i + 4 * g + r));
-      x[i][r] = takes_part<A, PAGED>(step, i, r, g, begin, end, bits) ? y : -__builtin_inff();
+      x[i][r] = y;
     }
   }
+  if (all_take_part<A, PAGED>(step, begin, end, bits)) return;
+#pragma unroll
+  for (int i = 0; i < A::NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (!takes_part<A, PAGED>(step, i, r, g, begin, end, bits)) x[i][r] = -__builtin_inff();
 }
 
 // Scores -> probabilities: the running maximum, the accumulators' rescaling, the sum.
@@ -373,8 +398,7 @@ __device__ __forceinline__ void accumulate(Attn<T, FP8, DP, PAGED, FULL>& s, uin
       for (int r = 0; r < 4; ++r) s.vs[i][r] = as_f32(from_lane32(as_u32(s.vs1), 16 * i + 4 * g + r));
   }
   // Values (and scales) of tokens that take no part may be anything: NaN times a probability of zero is NaN.
-  constexpr uint64_t kAll = PAGED || A::KS < 64 ? (uint64_t(1) << (PAGED ? A::NT : A::KS % 64)) - 1 : ~uint64_t(0);
-  if ((int)(step * A::KS) < begin || (int)(step * A::KS) + A::KS > end || bits != kAll) {
+  if (!all_take_part<A, PAGED>(step, begin, end, bits)) {
 #pragma unroll
     for (int i = 0; i < A::NT; ++i)
 #pragma unroll
@@ -456,118 +480,205 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t wave_total_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(v), 63);
+}
+
 __device__ __forceinline__ uint32_t scalar(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
 
+// (share a constant wherever this is inlined)
+__device__ __forceinline__ uint32_t parts_of(uint32_t count, uint32_t share) { return (count + share - 1) / share; }
+
+// An item's part of a workgroup: steps [at, stop) of sequence b's item `item`.
+struct Item {
+  int b, begin, end, head, row;  // row: first of its query heads in the group
+  uint32_t item, first, count, at, stop;
+};
+
+// The item's steps that `left` allow, from its step `at`.
+template <typename S>
+__device__ __forceinline__ Item item_of(const AttnArgs& a, const S& span, int b, uint32_t item, uint32_t at,
+                                        uint32_t left) {
+  const uint32_t stop = span.count - at < left ? span.count : at + left;
+  const int head = (int)(item / (uint32_t)a.row_groups), row = 16 * (int)(item - (uint32_t)head * a.row_groups);
+  return Item{b, span.begin, span.end, head, row, item, span.first, span.count, at, stop};
+}
+
+// How the line of all items' steps is cut: into parts of `share`, none across two items (`apart`, the line's items
+// rounded up to whole parts) if the grid is enough for parts of s0, s1 or s2, else into as many equal ones as the grid.
+struct Cut {
+  uint32_t total, share;
+  bool apart;
+};
+
+template <typename S>
+__device__ __forceinline__ Cut cut_line(const AttnArgs& a, uint32_t count, int lane, uint32_t per, uint32_t s0,
+                                        uint32_t s1, uint32_t s2) {
+  uint32_t n = count, p0 = parts_of(n, s0), p1 = parts_of(n, s1), p2 = parts_of(n, s2);
+  for (int i = lane + 64; i < a.m; i += 64) {
+    const uint32_t more = S(a, i).count;
+    n += more, p0 += parts_of(more, s0), p1 += parts_of(more, s1), p2 += parts_of(more, s2);
+  }
+  const uint32_t n0 = wave_total_u32(p0) * per, n1 = wave_total_u32(p1) * per, n2 = wave_total_u32(p2) * per;
+  if (n0 <= gridDim.x) return Cut{n0 * s0, s0, true};
+  if (n1 <= gridDim.x) return Cut{n1 * s1, s1, true};
+  if (n2 <= gridDim.x) return Cut{n2 * s2, s2, true};
+  const uint32_t total = wave_total_u32(n) * per;
+  return Cut{total, (total + gridDim.x - 1) / gridDim.x, false};
+}
+
 template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__global__ __launch_bounds__(256, DP > 128 && !(FP8 && FULL) ? 1 : 2) void attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(AttnArgs a) {
   using A = Attn<T, FP8, DP, PAGED, FULL>;
   using S = Span<A::KS>;
-  __shared__ float rows[A::kWaves][16][A::ROW];
-  __shared__ float tops[A::kWaves][16], sums[A::kWaves][16];
+  __shared__ float rows[2][A::kWaves][16][A::ROW];
+  __shared__ float2 ends[2][A::kWaves][16];  // (maximum, sum)
+  int half = 0;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const uint32_t per = (uint32_t)(a.heads * a.row_groups);  // items of a sequence
 
-  int b;
-  uint32_t item, at = 0, left;  // item of sequence b, its next step, steps left of this workgroup
-  uint32_t share = 0;
+  Item it;
+  uint32_t left = ~0u, share = 0;  // steps of this workgroup behind the item, and of every workgroup
   if (a.direct) {
-    b = (int)(blockIdx.x / per);
-    item = blockIdx.x - (uint32_t)b * per;
-    left = ~0u;
+    const int b = (int)(blockIdx.x / per);
+    it = item_of(a, S(a, b), b, blockIdx.x - (uint32_t)b * per, 0, ~0u);
+    left = 0;
   } else {
-    // All steps, then the sequence that holds this workgroup's first: every wave for itself, a sequence a lane.
-    uint32_t own = lane < a.m ? S(a, lane).count : 0u, n = own;
-    for (int i = lane + 64; i < a.m; i += 64) n += S(a, i).count;
-    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(n), 63) * per;
-    share = (total + gridDim.x - 1) / gridDim.x;
-    share = share < a.least ? a.least : share;
+    // Every wave for itself, a sequence a lane: the line's length, then the sequence that holds the workgroup's first
+    // step. Parts of one item where the grid allows it: the end of an item costs a workgroup some us.
+    S own(a, lane < a.m ? lane : a.m - 1);
+    if (lane >= a.m) own.count = 0;
+    Cut line = cut_line<S>(a, own.count, lane, per, 4, 8, 12);
+    if (!line.apart && line.share <= 32) line = cut_line<S>(a, own.count, lane, per, 16, 24, 32);
+    const bool apart = line.apart;
+    const uint32_t total = line.total;
+    share = line.share;
+    const auto room = [&](uint32_t count) { return apart ? (count + share - 1) / share * share : count; };
     const uint64_t start = (uint64_t)blockIdx.x * share;
     if (start >= total) return;
     left = total - (uint32_t)start < share ? total - (uint32_t)start : share;
     const uint32_t want = (uint32_t)start / per;
     uint32_t before = 0;
     for (int i0 = 0;; i0 += 64) {
-      if (i0) own = i0 + lane < a.m ? S(a, i0 + lane).count : 0u;
-      const uint32_t incl = before + wave_scan_u32(own);
-      const int lower = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= want));
-      if (lower < 64) {
-        b = i0 + lower;
-        const uint32_t count = (uint32_t)__builtin_amdgcn_readlane((int)own, lower);
-        const uint32_t rest =
-            (uint32_t)start - ((uint32_t)__builtin_amdgcn_readlane((int)incl, lower) - count) * per;
-        item = rest / count;
-        at = rest - item * count;
+      if (i0) {
+        own = S(a, i0 + lane < a.m ? i0 + lane : a.m - 1);
+        if (i0 + lane >= a.m) own.count = 0;
+      }
+      const uint32_t incl = before + wave_scan_u32(room(own.count));
+      const int at = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= want));
+      if (at < 64) {
+        const auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+        own.begin = (int)of((uint32_t)own.begin), own.end = (int)of((uint32_t)own.end);
+        own.first = of(own.first), own.count = of(own.count);
+        const uint32_t size = room(own.count), rest = (uint32_t)start - (of(incl) - size) * per, item = rest / size;
+        it = item_of(a, own, i0 + at, item, rest - item * size, left);
         break;
       }
       before = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
+    left = apart ? 0 : left - (it.stop - it.at);
   }
-  b = (int)scalar((uint32_t)b), item = scalar(item), at = scalar(at), left = scalar(left);
+  it = Item{(int)scalar(it.b), (int)scalar(it.begin), (int)scalar(it.end), (int)scalar(it.head), (int)scalar(it.row),
+            scalar(it.item), scalar(it.first), scalar(it.count), scalar(it.at), scalar(it.stop)};
+  left = scalar(left), share = scalar(share);
 
-  for (;;) {
-    const int head = (int)(item / (uint32_t)a.row_groups), rg = (int)(item - (uint32_t)head * a.row_groups);
-    const int nrows = a.group - 16 * rg < 16 ? a.group - 16 * rg : 16;
-    const int q0 = head * a.group + 16 * rg;
-    const int32_t* const table = a.table + (int64_t)b * a.table_row;
-    const uint8_t* const kh = a.k + head * a.k_head;
-    const uint8_t* const vh = a.v + head * a.v_head;
-    const float* const ksh = FP8 ? a.ks + head * a.ks_head : nullptr;
-    const float* const vsh = FP8 ? a.vs + head * a.vs_head : nullptr;
-
-    const S span(a, b);
-    const uint32_t stop = span.count - at < left ? span.count : at + left;  // steps [at, stop) of this item
-    uint32_t step = (a.window ? span.first : 0u) + at + (uint32_t)wave;
-    const uint32_t last = span.first + stop;
-    int entry = look_up<A, PAGED>(a, table, step, lane);
-    A s;
-    s.top = -__builtin_inff(), s.sum = 0.0f;
-    const uint16_t* const qp = a.q + (int64_t)b * a.q_row + (int64_t)(q0 + (c < nrows ? c : 0)) * a.q_head;
+  A s;
+  const auto rows_of = [&](const Item& i) { return a.group - i.row < 16 ? a.group - i.row : 16; };
+  const auto table_of = [&](const Item& i) { return a.table + (int64_t)i.b * a.table_row; };
+  const auto load_q = [&](const Item& i) {  // rows past the group's end repeat its first and are not written
+    const int row = i.row + (c < rows_of(i) ? c : 0);
+    const uint16_t* const qp = a.q + (int64_t)i.b * a.q_row + (int64_t)(i.head * a.group + row) * a.q_head;
 #pragma unroll
     for (int j = 0; j < A::NK; ++j) {
       const int d0 = A::k_at(j, g);
       s.q[j] = *reinterpret_cast<const u4*>(qp + (FULL || d0 < a.d ? d0 : 0));
     }
+  };
+  const auto get_k = [&](const Item& i, const Places& at, int slot) {
+    load_k(a, s, a.k + i.head * a.k_head, FP8 ? a.ks + i.head * a.ks_head : nullptr, at, slot, lane);
+  };
+  const auto get_v = [&](const Item& i, const Places& at, int slot) {
+    load_v(a, s, a.v + i.head * a.v_head, FP8 ? a.vs + i.head * a.vs_head : nullptr, at, slot, lane);
+  };
+
+  // The first step's loads; then each item's, while the item before it ends.
+  uint32_t step = (a.window ? it.first : 0u) + it.at + (uint32_t)wave;
+  int entry = look_up<A, PAGED>(a, table_of(it), step, lane), slot = 0;
+  load_q(it);
+  bool has = step < it.first + it.stop;  // whether the wave has a step of the item
+  Places at = places_of<A, PAGED, FP8>(a, entry, step, it.end, lane);
+  if (has) {
+    get_k(it, at, slot);
+    get_v(it, at, slot);
+  }
+  for (;;) {
+    // The item behind this one, and its first entry of the table.
+    const bool more = left != 0;
+    Item next = it;
+    if (more) {
+      uint32_t item = it.item + 1;
+      int b = it.b;
+      S span{it.begin, it.end, it.first, it.count};
+      if (item == per) {
+        item = 0;
+        do span = S(a, ++b);
+        while (span.count == 0);
+      }
+      next = item_of(a, span, b, item, 0, left);
+      left -= next.stop;
+    }
+    const uint32_t next_step = next.first + next.at + (uint32_t)wave;
+    const bool next_has = more && next_step < next.first + next.stop;
+    int next_entry = -1;
+    if (next_has) next_entry = look_up<A, PAGED>(a, table_of(next), next_step, lane);
+
+    s.top = -__builtin_inff(), s.sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < A::NSUB * A::CS; ++j) s.acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (step < last) {
-#pragma unroll
-      for (int j = 0; j < A::NK; ++j)
-        if (c >= nrows || (!FULL && A::k_at(j, g) >= a.d)) s.q[j] = u4{0u, 0u, 0u, 0u};
-      Places at_k = places_of<A, PAGED, FP8>(a, entry, step, span.end, lane);
-      int slot = 0;
-      entry = look_up<A, PAGED>(a, table, step + 4 * A::kAhead, lane);
+    const uint32_t last = it.first + it.stop;
+    if (has) {
       float x[A::NT][4];
-      load_k(a, s, kh, ksh, at_k, slot, lane);
-      load_v(a, s, vh, vsh, at_k, slot, lane);
+      if (!FULL) {
+#pragma unroll
+        for (int j = 0; j < A::NK; ++j)
+          if (A::k_at(j, g) >= a.d) s.q[j] = u4{0u, 0u, 0u, 0u};
+      }
+      if (step + 4 * A::kAhead < last) entry = look_up<A, PAGED>(a, table_of(it), step + 4 * A::kAhead, lane);
       for (; step + 4 < last; step += 4) {
-        const uint64_t bits = step_bits<A, PAGED>(at_k, slot);
-        scores(a, s, step, span.begin, span.end, bits, lane, x);
+        const uint64_t bits = step_bits<A, PAGED>(at, slot);
+        scores(a, s, step, it.begin, it.end, bits, lane, x);
         if (++slot == A::kAhead) {
           slot = 0;
-          at_k = places_of<A, PAGED, FP8>(a, entry, step + 4, span.end, lane);
-          entry = look_up<A, PAGED>(a, table, step + 4 + 4 * A::kAhead, lane);
+          at = places_of<A, PAGED, FP8>(a, entry, step + 4, it.end, lane);
+          entry = look_up<A, PAGED>(a, table_of(it), step + 4 + 4 * A::kAhead, lane);
         }
-        load_k(a, s, kh, ksh, at_k, slot, lane);
+        get_k(it, at, slot);
         softmax(s, x);
-        accumulate(s, step, span.begin, span.end, bits, lane, x);
-        load_v(a, s, vh, vsh, at_k, slot, lane);
+        accumulate(s, step, it.begin, it.end, bits, lane, x);
+        get_v(it, at, slot);
       }
-      const uint64_t bits = step_bits<A, PAGED>(at_k, slot);
-      scores(a, s, step, span.begin, span.end, bits, lane, x);
+      const uint64_t bits = step_bits<A, PAGED>(at, slot);
+      scores(a, s, step, it.begin, it.end, bits, lane, x);
       softmax(s, x);
-      accumulate(s, step, span.begin, span.end, bits, lane, x);
+      accumulate(s, step, it.begin, it.end, bits, lane, x);
+    }
+    if (next_has) {
+      slot = 0;
+      at = places_of<A, PAGED, FP8>(a, next_entry, next_step, next.end, lane);
+      load_q(next);
+      get_k(next, at, slot);
+      get_v(next, at, slot);
     }
 
-    // The waves' parts: one maximum, then their rows side by side.
+    // The waves' parts side by side in one half of the LDS; the next item's go to the other, so that one barrier an
+    // item is enough: past it, every wave has read what it needs of the half before.
+    const int nrows = rows_of(it);
     const float own = sum4(s.sum);
-    if (g == 0) tops[wave][c] = s.top, sums[wave][c] = own;
-    __syncthreads();
-    const float top = __builtin_fmaxf(__builtin_fmaxf(tops[0][c], tops[1][c]), __builtin_fmaxf(tops[2][c], tops[3][c]));
-    const float f = s.top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s.top - top);
     if (c < nrows) {
+      if (g == 0) ends[half][wave][c] = float2{s.top, own};
 #pragma unroll
       for (int n = 0; n < A::NSUB; ++n)
 #pragma unroll
@@ -576,51 +687,48 @@ __global__ __launch_bounds__(256, DP > 128 && !(FP8 && FULL) ? 1 : 2) void atten
           for (int j = 0; j < A::CS; j += 4) {
             f4 y;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) y[x] = s.acc[n * A::CS + j + x][r] * f;
-            *reinterpret_cast<f4*>(&rows[wave][c][128 * n + (4 * g + r) * A::CS + j]) = y;
+            for (int x = 0; x < 4; ++x) y[x] = s.acc[n * A::CS + j + x][r];
+            *reinterpret_cast<f4*>(&rows[half][wave][c][128 * n + (4 * g + r) * A::CS + j]) = y;
           }
     }
     __syncthreads();
-    const bool starts = at == 0, whole = starts && stop == span.count;
+    const bool starts = it.at == 0, whole = starts && it.stop == it.count;
     float* const piece =
-        whole ? nullptr : a.part + (int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * a.part_rows * (DP + 2);
+        whole ? nullptr : a.part + piece_of((int)blockIdx.x, starts) * a.part_rows * (DP + 2);
     for (int e = tid; e < nrows * (DP / 4); e += 256) {
       const int row = e / (DP / 4), d0 = (e - row * (DP / 4)) * 4;
-      const float t = __builtin_fmaxf(__builtin_fmaxf(tops[0][row], tops[1][row]),
-                                      __builtin_fmaxf(tops[2][row], tops[3][row]));
+      float2 tl[A::kWaves];
+      f4 part[A::kWaves];
+#pragma unroll
+      for (int w = 0; w < A::kWaves; ++w) {
+        tl[w] = ends[half][w][row];
+        part[w] = *reinterpret_cast<const f4*>(&rows[half][w][row][d0]);
+      }
+      const float t = __builtin_fmaxf(__builtin_fmaxf(tl[0].x, tl[1].x), __builtin_fmaxf(tl[2].x, tl[3].x));
       float l = 0.0f;
       f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < A::kWaves; ++w) {
-        const float tw = tops[w][row];
-        l += tw == -__builtin_inff() ? 0.0f : sums[w][row] * __builtin_amdgcn_exp2f(tw - t);
-        y += *reinterpret_cast<const f4*>(&rows[w][row][d0]);
+        const float f = tl[w].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(tl[w].x - t);
+        l += tl[w].y * f;
+        y += part[w] * f;
       }
       if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (FULL || d0 < a.d)
-          store4<T>(a.out + ((int64_t)b * a.heads * a.group + q0 + row) * a.d + d0, y * inv);
+          store4<T>(a.out + (((int64_t)it.b * a.heads + it.head) * a.group + it.row + row) * a.d + d0, y * inv);
       } else {
         *reinterpret_cast<f4*>(piece + row * DP + d0) = y;
         if (d0 == 0) *reinterpret_cast<float2*>(piece + a.part_rows * DP + 2 * row) = float2{t, l};
       }
     }
-    if (a.direct) return;
-    if (starts && tid == 0) {
+    if (starts && tid == 0 && !a.direct) {
       // an item's last workgroup: `rest` steps of it lie behind this workgroup's
-      const uint32_t rest = span.count - stop;
-      a.ends[(int64_t)b * per + item] = int2{(int)blockIdx.x, (int)(blockIdx.x + (rest + share - 1) / share)};
+      const uint32_t rest = it.count - it.stop;
+      a.ends[(int64_t)it.b * per + it.item] = int2{(int)blockIdx.x, (int)(blockIdx.x + (rest + share - 1) / share)};
     }
-    left -= stop - at;
-    if (left == 0) return;
-    at = 0;
-    if (++item == per) {
-      item = 0;
-      do ++b;
-      while (b < a.m && S(a, b).count == 0);
-      if (b >= a.m) return;
-    }
-    __syncthreads();
+    if (!more) return;
+    it = next, step = next_step, has = next_has, half ^= 1;
   }
 }
 
@@ -649,8 +757,5 @@ int launch_attention(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool fu
 int launch_attention_d64(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
 int launch_attention_d128(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
 int launch_attention_d256(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
-
-// Tokens of a step, as the kernels above take them.
-constexpr int attention_step(bool fp8, int dp) { return dp == 64 || (fp8 && dp == 128) ? 64 : 32; }
 
 }  // namespace tf

@@ -30,11 +30,11 @@ __device__ __forceinline__ void merge(Part& a, float top, float l, const f4& y) 
 }
 
 // out = sum_p acc_p 2^(top_p - top) / sum_p sum_p 2^(top_p - top) of a sequence's query head over the pieces p that
-// the attention's workgroups left, by one wave (WAVES 1) or a workgroup of 4. dp / 4 lanes take a piece; a wave takes
+// the attention's workgroups left, by one wave (WAVES 1) or a workgroup of 16. dp / 4 lanes take a piece; a wave takes
 // 64 / (dp / 4) side by side, four of each at once, and the parts are merged in an order that depends on the number
 // of pieces alone. Items that one workgroup held are done already; sequences without tokens get zeros here.
 template <typename T, int WAVES>
-__global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(JoinArgs a) {
   __shared__ Part parts[WAVES][64];
   constexpr int kOnce = 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 #pragma unroll
     for (int i = 0; i < kOnce; ++i) {
       const int p = p0 + i * each <= ends.y ? p0 + i * each : p0;
-      const float* const piece = a.part + (2 * (int64_t)p + (p == ends.x ? 1 : 0)) * size;
+      const float* const piece = a.part + piece_of(p, p == ends.x) * size;
       tl[i] = *reinterpret_cast<const float2*>(piece + a.part_rows * a.dp + 2 * row);
       y[i] = *reinterpret_cast<const f4*>(piece + row * a.dp + e);
     }
@@ -87,7 +87,17 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
   if (writes) store4<T>(out + e, mine.y * (mine.l == 0.0f ? 0.0f : 1.0f / mine.l));
 }
 
-constexpr uint32_t kJoinByWave = 1024;  // rows from which a wave each fills the CUs
+// Rows from which a wave each fills the CUs in the join; below, items so few and long that one has some sixty pieces
+// or more get 8 waves a row (MI355X, one sequence of 32749 tokens in e4m3: 16.6 us with it, 17.9 with 4 waves and
+// 16.7 with 16, which cost one of 4096 0.5 and 1.3 us).
+constexpr uint32_t kJoinByWave = 1024;
+constexpr int64_t kFewItems = 8, kLongItems = 8192;
+
+// Bytes of an item up to which a workgroup takes it whole, and with items for every place on the CUs (MI355X: 512
+// items of up to 512 KB in e4m3 25 us against 32, of 1 MB in 16 bits 57 against 49; 1024 of 256 KB 34 against 41;
+// 4 of 256 KB alike).
+constexpr int64_t kDirect = 256 << 10, kDirectMany = 512 << 10, kManyItems = 512;
+
 
 bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
@@ -95,11 +105,13 @@ bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(
 struct Plan {
   int dp, group, row_groups, part_rows;
   int64_t items, cap, part_floats, bytes;
+  uint32_t grid;
   bool fp8, direct;
 };
 
-std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t width, Plan& p) {
+std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t width, int64_t window, Plan& p) {
   if (m < 0 || width < 0 || m > 0x7FFFFFFF) return "bad size";
+  if (window < 0) return "need window >= 0";
   if (q_heads <= 0 || q_heads > 0xFFFF || q_heads % c.heads) return "q_heads must be a multiple of the cache's heads";
   p.fp8 = c.dtype == TF_DTYPE_E4M3;
   p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
@@ -111,8 +123,16 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
   p.cap = width * c.page_size;
   if (m * q_heads > 0x7FFFFF || p.items * cdiv(p.cap, 16) > 0x7FFFFFFF)
     return "more sequences, heads and tokens of block_table than 2^31 steps of 16";
-  p.direct = p.cap <= 4 * attention_step(p.fp8, p.dp);
-  p.part_floats = p.direct ? 0 : 2 * (int64_t)kAttnGrid * p.part_rows * (p.dp + 2);
+  // An item's steps are at most those of its row of the table. Where they are few, or not many and the items enough
+  // to fill the CUs, a workgroup takes a whole item: no second launch, and no search for the workgroup's place. The
+  // longest item then sets the time.
+  const int step = attention_step(p.dp);
+  int64_t most = cdiv(p.cap, step);
+  if (window > 0) most = most < cdiv(window, step) + 1 ? most : cdiv(window, step) + 1;
+  const int64_t bytes = most * step * 2 * p.dp * (p.fp8 ? 1 : 2);
+  p.direct = bytes <= (p.items >= kManyItems ? kDirectMany : kDirect);
+  p.grid = p.direct ? (uint32_t)p.items : (uint32_t)attention_grid(p.dp);
+  p.part_floats = p.direct ? 0 : 2 * (int64_t)p.grid * p.part_rows * (p.dp + 2);
   p.bytes = p.direct ? 0 : p.part_floats * 4 + p.items * 8;
   return "";
 }
@@ -123,10 +143,10 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
 using namespace tf;
 
 extern "C" int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads,
-                                                      int64_t width) {
+                                                      int64_t width, int32_t window) {
   Plan p;
   if (!cache || !kv_cache_error(cache, cache->dtype == TF_DTYPE_E4M3 ? TF_DTYPE_FP16 : cache->dtype).empty()) return -1;
-  if (!plan_of(*cache, m, q_heads, width, p).empty()) return -1;
+  if (!plan_of(*cache, m, q_heads, width, window, p).empty()) return -1;
   return p.bytes;
 }
 
@@ -142,9 +162,8 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
   if (!multiple(q, 16) || q_row % 8 || q_head % 8 || !multiple(out, 16))
     return bad("rows of q and out must be 16-byte aligned");
   if (q_row < 0 || q_head < 0 || table_stride < 0) return bad("negative stride");
-  if (window < 0) return bad("need window >= 0");
   Plan p;
-  const std::string wrong = plan_of(c, m, q_heads, width, p);
+  const std::string wrong = plan_of(c, m, q_heads, width, window, p);
   if (!wrong.empty()) return bad(wrong);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return bad("workspace too small (" + std::to_string(workspace_bytes) + " < " + std::to_string(p.bytes) + ")");
@@ -164,7 +183,6 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
   a.pages = c.pages, a.page = page_div((uint32_t)c.page_size);
   a.m = (int)m, a.heads = c.heads, a.group = p.group, a.row_groups = p.row_groups, a.part_rows = p.part_rows;
   a.d = c.head_dim, a.cap = (int)p.cap, a.window = window, a.scale_log2 = scale * 1.44269504088896341f;
-  a.least = 4;
   a.direct = p.direct;
   bool paged = c.page_size % 16 == 0;
   if (p.fp8) {  // a tile's scales go by 16-byte loads
@@ -177,17 +195,18 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
     full = full && multiple(c.k, 16);
     for (int i = 0; i < 3; ++i) full = full && c.k_strides[i] % 16 == 0;
   }
-  const unsigned grid = a.direct ? (unsigned)p.items : (unsigned)kAttnGrid;
   const bool bf16 = dtype == TF_DTYPE_BF16;
   const auto s = (hipStream_t)stream;
   const auto launch = p.dp == 64 ? launch_attention_d64 : p.dp == 128 ? launch_attention_d128 : launch_attention_d256;
-  if (int rc = launch(a, bf16, p.fp8, paged, full, grid, s)) return rc;
-  if (a.direct) return TF_OK;
+  if (int rc = launch(a, bf16, p.fp8, paged, full, p.grid, s)) return rc;
+  if (p.direct) return TF_OK;
   const auto count = (uint32_t)(m * q_heads);
   const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp, count};
   if (count >= kJoinByWave)
     bf16 ? join_kernel<BF16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j)
          : join_kernel<F16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j);
+  else if (p.items <= kFewItems && p.cap >= kLongItems)
+    bf16 ? join_kernel<BF16, 8><<<count, 512, 0, s>>>(j) : join_kernel<F16, 8><<<count, 512, 0, s>>>(j);
   else
     bf16 ? join_kernel<BF16, 4><<<count, 256, 0, s>>>(j) : join_kernel<F16, 4><<<count, 256, 0, s>>>(j);
   return check_launch("tf_paged_attention");

@@ -849,7 +849,7 @@ std::tuple<at::Tensor, at::Tensor> kv_cache_read(const at::Tensor& k_cache, cons
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                            const OptTensor& k_scale, const OptTensor& v_scale, const at::Tensor& block_table,
                            const at::Tensor& seq_lens, double scale, c10::SymInt window) {
-  const int64_t win = window.guard_int(__FILE__, __LINE__);
+  const int64_t win = std::min<int64_t>(window.guard_int(__FILE__, __LINE__), 0x7FFFFFFF);
   tf_kv_cache c;
   const c10::Device dev = k_cache.device();
   int64_t need = -1;
@@ -859,7 +859,8 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
       index_ok(seq_lens, q.size(0), at::kInt, dev) && block_table.dim() == 2 && block_table.size(0) == q.size(0) &&
       block_table.scalar_type() == at::kInt && on(block_table, dev) &&
       (block_table.size(1) <= 1 || block_table.stride(1) == 1))
-    need = api().attention_bytes(&c, q.size(0), static_cast<int32_t>(q.size(1)), block_table.size(1));
+    need = api().attention_bytes(&c, q.size(0), static_cast<int32_t>(q.size(1)), block_table.size(1),
+                                 static_cast<int32_t>(win));
   if (need < 0)
     return python_body<AttentionFn>("tokenforge::_py_paged_attention", q, k_cache, v_cache, k_scale, v_scale,
                                     block_table, seq_lens, scale, window);
@@ -870,7 +871,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   check(api().attention(&c, data<const uint16_t>(q), step_of(q, 0), step_of(q, 1), static_cast<int32_t>(q.size(1)),
                         dtype_code(q.scalar_type()), data<const int32_t>(block_table), step_of(block_table, 0),
                         block_table.size(1), data<const int32_t>(seq_lens), q.size(0), static_cast<float>(scale),
-                        static_cast<int32_t>(std::min<int64_t>(win, 0x7FFFFFFF)), data<uint16_t>(out),
+                        static_cast<int32_t>(win), data<uint16_t>(out),
                         work.defined() ? data<float>(work) : nullptr, need,
                         c10::hip::getCurrentHIPStream(dev.index()).stream()),
         "tf_paged_attention");
