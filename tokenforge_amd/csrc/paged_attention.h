@@ -183,11 +183,13 @@ __device__ __forceinline__ uint32_t own_key(uint32_t step, int lane) {
   return ((step + 4u * (uint32_t)(lane / A::NT)) * A::NT + (uint32_t)(lane % A::NT)) * 16u;
 }
 
-// Its entry in the table: independent of the sequence's length, so that both can be on their way at once.
+// Its entry in the table, of tokens below `limit`. Where that is the table's own end, the lookup does not depend on
+// the sequence's length, and both are on their way at once.
 template <typename A, bool PAGED>
-__device__ __forceinline__ int look_up(const AttnArgs& a, const int32_t* table, uint32_t step, int lane) {
+__device__ __forceinline__ int look_up(const AttnArgs& a, const int32_t* table, uint32_t step, uint32_t limit,
+                                       int lane) {
   const uint32_t key = own_key<A, PAGED>(step, lane);
-  return key < (uint32_t)a.cap ? table[div_page(key, a.page)] : -1;
+  return key < limit ? table[div_page(key, a.page)] : -1;
 }
 
 template <typename A, bool PAGED, bool FP8>
@@ -588,6 +590,11 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
   A s;
   const auto rows_of = [&](const Item& i) { return a.group - i.row < 16 ? a.group - i.row : 16; };
   const auto table_of = [&](const Item& i) { return a.table + (int64_t)i.b * a.table_row; };
+  // Entries behind the workgroup's part are not fetched where its end is known: 64 of them are 32 lines of memory.
+  const auto limit_of = [&](const Item& i) {
+    const uint32_t end = (i.first + i.stop) * A::KS;
+    return a.direct || end > (uint32_t)a.cap ? (uint32_t)a.cap : end;
+  };
   const auto load_q = [&](const Item& i) {  // rows past the group's end repeat its first and are not written
     const int row = i.row + (c < rows_of(i) ? c : 0);
     const uint16_t* const qp = a.q + (int64_t)i.b * a.q_row + (int64_t)(i.head * a.group + row) * a.q_head;
@@ -606,7 +613,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
 
   // The first step's loads; then each item's, while the item before it ends.
   uint32_t step = (a.window ? it.first : 0u) + it.at + (uint32_t)wave;
-  int entry = look_up<A, PAGED>(a, table_of(it), step, lane), slot = 0;
+  int entry = look_up<A, PAGED>(a, table_of(it), step, limit_of(it), lane), slot = 0;
   load_q(it);
   bool has = step < it.first + it.stop;  // whether the wave has a step of the item
   Places at = places_of<A, PAGED, FP8>(a, entry, step, it.end, lane);
@@ -633,7 +640,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
     const uint32_t next_step = next.first + next.at + (uint32_t)wave;
     const bool next_has = more && next_step < next.first + next.stop;
     int next_entry = -1;
-    if (next_has) next_entry = look_up<A, PAGED>(a, table_of(next), next_step, lane);
+    if (next_has) next_entry = look_up<A, PAGED>(a, table_of(next), next_step, limit_of(next), lane);
 
     s.top = -__builtin_inff(), s.sum = 0.0f;
 #pragma unroll
@@ -646,14 +653,14 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
         for (int j = 0; j < A::NK; ++j)
           if (A::k_at(j, g) >= a.d) s.q[j] = u4{0u, 0u, 0u, 0u};
       }
-      if (step + 4 * A::kAhead < last) entry = look_up<A, PAGED>(a, table_of(it), step + 4 * A::kAhead, lane);
+      if (step + 4 * A::kAhead < last) entry = look_up<A, PAGED>(a, table_of(it), step + 4 * A::kAhead, limit_of(it), lane);
       for (; step + 4 < last; step += 4) {
         const uint64_t bits = step_bits<A, PAGED>(at, slot);
         scores(a, s, step, it.begin, it.end, bits, lane, x);
         if (++slot == A::kAhead) {
           slot = 0;
           at = places_of<A, PAGED, FP8>(a, entry, step + 4, it.end, lane);
-          entry = look_up<A, PAGED>(a, table_of(it), step + 4 + 4 * A::kAhead, lane);
+          entry = look_up<A, PAGED>(a, table_of(it), step + 4 + 4 * A::kAhead, limit_of(it), lane);
         }
         get_k(it, at, slot);
         softmax(s, x);

@@ -709,6 +709,7 @@ void cache_strides(const at::Tensor& t, int64_t (&s)[3]) {
 
 // Whether no two elements of t share memory (dimensions nested by their strides).
 bool elements_apart(const at::Tensor& t) {
+  if (t.is_contiguous()) return true;
   std::array<std::pair<int64_t, int64_t>, 4> d;
   size_t n = 0;
   for (int64_t i = 0; i < t.dim(); ++i)
