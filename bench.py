@@ -92,7 +92,10 @@ Extra objects on the same JSON line:
   addition qkv and
   gate_up take the FP8 codes and scales directly as W4A8 linears ("w4a8", no fp16(q * scale)
   glue; not bit-equal: the scale multiplies each row's sum instead of each element; from M = 128
-  these run on the fp8-MFMA GEMM, which also applies the group scale exactly). A pass
+  these run on the fp8-MFMA GEMM, which also applies the group scale exactly). With
+  ``--stack-context N`` the decode rows also run the fused pass with attention in the place of the
+  identity ("attention", "attention_e4m3"): queries and keys rotated, the token written into a paged
+  cache in 16 or 8 bits, and attention over N cached tokens of each of the M sequences. A pass
   is one HIP graph, tokens/s = M / time per pass, at M in {1, 8, 32} (decode) and 2048
   (prefill).
 * ``cpu_baseline``: reference.py's CPU path (dequantize per call + fp32 matmul), restated in
@@ -988,7 +991,36 @@ HEAD_DIM = 128
 KV_HEADS = 4
 
 
-def stack_bench(dev: torch.device, gpu: str, ms: tuple[int, ...], tune: bool) -> list[dict]:  # type: ignore[type-arg]
+def stack_caches(dev: torch.device, m: int, context: int, fp8: bool) -> dict:  # type: ignore[type-arg]
+    """Caches of the stack's layers with ``context`` tokens of each of ``m`` sequences, the last of which the pass
+    itself writes, and the indices of its calls."""
+    page = 16
+    width = -(-context // page)
+    pages = m * width
+    gen = torch.Generator(device=dev).manual_seed(12)
+    order = torch.randperm(pages, generator=gen, device=dev)
+    ops = torch.ops.tokenforge
+    layers = []
+    for _ in range(STACK_LAYERS):
+        shape = (pages, KV_HEADS, page, HEAD_DIM)
+        kv = [torch.empty(shape, dtype=torch.float8_e4m3fn if fp8 else torch.float16, device=dev) for _ in "kv"]
+        scales = [torch.empty(shape[:3], device=dev) if fp8 else None for _ in "kv"]
+        for part in torch.arange(pages * page, device=dev).split(1 << 18):
+            x = torch.randn((2, part.numel(), KV_HEADS, HEAD_DIM), generator=gen, device=dev, dtype=torch.float16)
+            ops.kv_cache_write(x[0], x[1], *kv, *scales, part)
+        layers.append((*kv, *scales))
+    table = order.view(m, width).to(torch.int32)
+    last = context - 1
+    angle = torch.arange(context, dtype=torch.float64, device=dev)[:, None] * 1e6 ** (
+        -torch.arange(0, HEAD_DIM, 2, dtype=torch.float64, device=dev) / HEAD_DIM)
+    return {"layers": layers, "table": table, "slots": table[:, last // page].long() * page + last % page,
+            "positions": torch.full((m,), last, device=dev), "lens": torch.full((m,), context, dtype=torch.int32, device=dev),
+            "cos_sin": torch.cat([angle.cos(), angle.sin()], 1).float(),
+            "bytes": m * context * 2 * KV_HEADS * (HEAD_DIM + 4 if fp8 else 2 * HEAD_DIM) * STACK_LAYERS}
+
+
+def stack_bench(dev: torch.device, gpu: str, ms: tuple[int, ...], tune: bool,
+                context: int = 0) -> list[dict]:  # type: ignore[type-arg]
     """configs[4]: tokens/s of one pass through 28 decoder layers, per M (module docstring);
     each M timed with the unfused torch glue, with the fused epilogues (residual adds in
     o_proj and down, SiLU*mul in gate_up; same bits) and with W4A8 qkv and gate_up."""
@@ -1012,6 +1044,21 @@ def stack_bench(dev: torch.device, gpu: str, ms: tuple[int, ...], tune: bool) ->
             autotune.tune_layer(n, k, GROUP, device=dev, gpu=gpu, buckets=tuple(sorted(set(ms))))
     ops = torch.ops.tokenforge
     q_width = SHAPES[0][1] - 2 * KV_HEADS * HEAD_DIM  # 3584 query columns, then k and v
+
+    def attention(y: torch.Tensor, cache: tuple) -> torch.Tensor:  # type: ignore[type-arg]
+        kv = KV_HEADS * HEAD_DIM
+        q, k, v = (t.unflatten(1, (-1, HEAD_DIM)) for t in y.split((q_width, kv, kv), 1))
+        q = ops.rope_kv_cache_write(q, k, v, caches["cos_sin"], caches["positions"], *cache, caches["slots"], False)
+        return ops.paged_attention(q, *cache, caches["table"], caches["lens"], HEAD_DIM**-0.5).flatten(1)
+
+    def attention_pass(x: torch.Tensor) -> torch.Tensor:
+        """The fused pass with the rotation, the cache and the attention."""
+        for ((qkv, o, gu, down), bias, g1, g2), cache in zip(layers, caches["layers"]):
+            y = ops.rmsnorm_fp8_w4a16_linear(x, g1, eps, *qkv, bias, GROUP, "hip", "none")
+            x = ops.w4a16_linear_residual(attention(y, cache), *o, None, x, GROUP, "hip")
+            act = ops.rmsnorm_fp8_w4a16_linear(x, g2, eps, *gu, None, GROUP, "hip", "silu_mul")
+            x = ops.w4a16_linear_residual(act, *down, None, x, GROUP, "hip")
+        return x
 
     def layer_pass(x: torch.Tensor, layer: tuple) -> torch.Tensor:  # type: ignore[type-arg]
         (qkv, o, gu, down), bias, g1, g2 = layer
@@ -1079,6 +1126,20 @@ def stack_bench(dev: torch.device, gpu: str, ms: tuple[int, ...], tune: bool) ->
         ref = outs_by_mode["fused"].float()
         row["w4a8_normwise_vs_fp16_input"] = float((outs_by_mode["w4a8"].float() - ref).abs().max() / ref.abs().max())
         row["tokens_per_s"] = row["fused"]["tokens_per_s"]
+        for fp8 in (False, True) if context and m <= 128 else ():
+            key = "attention_e4m3" if fp8 else "attention"
+            caches = stack_caches(dev, m, context, fp8)
+            g, outs = capture([lambda x0=x0: attention_pass(x0)], warm=1)
+            ms_pass = median_replay_ms(g, 1)
+            if not bool(torch.isfinite(outs[0]).all()):
+                raise RuntimeError(f"stack pass with attention at M={m} produced non-finite values")
+            row[key] = {"context": context, "ms_per_pass": ms_pass, "tokens_per_s": m / (ms_pass * 1e-3),
+                        "cache_bytes": caches["bytes"],
+                        "over_fused_ms": ms_pass - row["fused"]["ms_per_pass"]}
+            log(f"  stack M={m:<5d} {key:14s} {ms_pass * 1e3:9.1f} us/pass {m / (ms_pass * 1e-3):9.0f} tok/s over {context} "
+                f"tokens (+{row[key]['over_fused_ms'] * 1e3:.1f} us for {caches['bytes'] / 1e6:.1f} MB of cache)")
+            del g, outs, caches
+            torch.cuda.empty_cache()
         res.append(row)
         del outs_by_mode
     del layers
@@ -1285,6 +1346,8 @@ def main() -> int:
     ap.add_argument("--stack", action="store_true",
                     help="accepted for older command lines: the stack runs at M in {1, 8, 32, 2048} by default")
     ap.add_argument("--no-stack", action="store_true", help="skip the stack (configs[4])")
+    ap.add_argument("--stack-context", type=int, default=0, metavar="TOKENS",
+                    help="also run the stack's decode rows with attention over this many cached tokens a sequence")
     ap.add_argument("--traffic-probe", action="store_true",
                     help="eager gate_up GEMV launches + a calibration kernel, for rocprofv3 --pmc")
     ap.add_argument("--traffic-summary", nargs=3, metavar=("FETCH_DIR", "WRITE_DIR", "PROBE_LOG"),
@@ -1651,7 +1714,7 @@ def main() -> int:
 
     stack = None
     if not args.no_stack:
-        stack = stack_bench(dev, gpu, STACK_M, args.tune)
+        stack = stack_bench(dev, gpu, STACK_M, args.tune, args.stack_context)
 
     gate_n, gate_k = SHAPES[2][1], SHAPES[2][2]
     repack = {"gvalues_per_s": gate_n * gate_k / (rep_ms * 1e-3) / 1e9,
