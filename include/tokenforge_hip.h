@@ -367,14 +367,15 @@ typedef struct {
  * type `dtype` (strides token, head in elements; rows on 16 bytes), the cache's own type or TF_DTYPE_E4M3: then
  *   scale = max(amax / 448, 1/(448*512)) over the head, code = e4m3fn(RNE(value / scale)).
  * slots int64 [t]; a slot outside [0, pages * page_size) is not written (padding). Slots of one call must
- * differ: of two tokens with one slot it is not specified whose values stay.
+ * differ: of two tokens with one slot it is not specified whose values stay. Keys and values (and their scales) are
+ * written to places of their own.
  *
  * tf_rope_kv_cache_write: the same with q [t, q_heads, head_dim] and k rotated first, in fp32 up to the one
  * rounding (or the codes): with i < rot / 2, (a, b) = elements (i, i + rot/2), or (2i, 2i+1) if interleaved,
  *   a' = a cos - b sin, b' = b cos + a sin,  cos = cos_sin[positions[t]][i], sin = cos_sin[..][rot/2 + i];
  * elements from rot on stay. cos_sin fp32 [max_positions, rot] contiguous, 16-byte aligned, rot even and at
  * most head_dim; positions int64 [t]; a position outside the table gives NaN in the rotated elements. q_out
- * [t, q_heads, head_dim] contiguous.
+ * [t, q_heads, head_dim] contiguous, apart from q.
  *
  * tf_kv_cache_read: k_out, v_out [t, heads, head_dim] contiguous, of the 16-bit type `dtype` (the cache's own,
  * or any for e4m3): the tokens in slots int64 [t], code * scale rounded once; zeros for a slot out of range. */

@@ -166,6 +166,11 @@ def test_caches_are_refused() -> None:
         ops.kv_cache_write(x, x, one, f16.as_strided((2, 2, 16, 64), (2048, 1024, 56, 1)), None, None, slots)
     with pytest.raises(ValueError, match="v_scale is written"):
         ops.kv_cache_write(x, x, f8, f8.clone(), s, s[..., :1].expand(2, 2, 16), slots)
+    with pytest.raises(ValueError, match="one tensor"):
+        ops.kv_cache_write(x, x, one, one, None, None, slots)
+    with pytest.raises(ValueError, match="k_scale and v_scale"):
+        ops.kv_cache_write(x, x, f8, f8.clone(), s, s, slots)
+    assert ops.kv_cache_read(one, one, None, None, slots, torch.float16)[0].shape == (3, 2, 64)
     assert ops.kv_cache_read(twice, one, None, None, slots, torch.float16)[0].shape == (3, 2, 64)
 
 
@@ -289,6 +294,9 @@ def test_c_entries_refuse_before_any_launch() -> None:
             assert call(_c_cache(**changed)) == _lib.TF_EINVAL
             assert message in h.tf_last_error(), (changed, h.tf_last_error())
     ok = _c_cache()
+    for bad, message in [({"v": 0x10000}, b"one place"), ({"dtype": 2, "v_scale": 0x30000}, b"scales of keys")]:
+        for call in (write, rope):
+            assert call(_c_cache(**bad)) == _lib.TF_EINVAL and message in h.tf_last_error()
     for call, changed, message in [
         (write, {"k": None}, b"null"), (write, {"k": x + 2}, b"aligned"), (write, {"kt": 129}, b"aligned"),
         (write, {"kh": 4}, b"aligned"), (write, {"dtype": 2}, b"unknown dtype"), (write, {"slots": None}, b"null"),

@@ -71,6 +71,10 @@ def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Ten
                 raise ValueError(f"{name}: a page's tokens must lie less than {MAX_TOKEN_STRIDE} elements apart")
             if written and not _rows_apart(t):
                 raise ValueError(f"{name} is written and must not hold an element twice")
+        if written and k_scale.data_ptr() == v_scale.data_ptr():  # type: ignore[union-attr]
+            raise ValueError("k_scale and v_scale are written and must not be one tensor")
+    if written and k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError("k_cache and v_cache are written and must not be one tensor")
     return pages, heads, page_size, d
 
 

@@ -200,6 +200,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a) {
     const bool kept = mine && r.part < 2 && at.page >= 0;
     const int p = r.part & 1;
     const int64_t to = at.page * a.page_stride[p] + r.head * a.head_stride[p] + at.off * a.token_stride[p];
+    if (ROPE != kNone && r.part == 2) continue;  // (a lane group's rows are of one part, each with all its lanes)
     if (FP8) {
       if (e[0] >= a.d) {
 #pragma unroll
@@ -344,6 +345,12 @@ KvArgs cache_args(const tf_kv_cache& c) {
   return a;
 }
 
+std::string written_error(const tf_kv_cache& c) {
+  if (c.k == c.v) return "keys and values are written to one place";
+  if (c.dtype == TF_DTYPE_E4M3 && c.k_scale == c.v_scale) return "scales of keys and values are written to one place";
+  return "";
+}
+
 std::string rows_error(const void* p, int64_t token, int64_t head, const char* name) {
   if (!p) return std::string(name) + " is a null pointer";
   if (!multiple(p, 16) || token % 8 || head % 8) return std::string("rows of ") + name + " must be 16-byte aligned";
@@ -406,6 +413,7 @@ extern "C" int tf_kv_cache_write(const tf_kv_cache* cache, const uint16_t* k, in
                                  const int64_t* slots, int64_t t, void* stream) {
   const auto bad = [](const std::string& what) { return fail(TF_EINVAL, "tf_kv_cache_write: " + what); };
   std::string e = kv_cache_error(cache, dtype);
+  if (e.empty()) e = written_error(*cache);
   if (e.empty()) e = rows_error(k, k_token, k_head, "k");
   if (e.empty()) e = rows_error(v, v_token, v_head, "v");
   if (!e.empty()) return bad(e);
@@ -428,6 +436,7 @@ extern "C" int tf_rope_kv_cache_write(const tf_kv_cache* cache, const uint16_t* 
                                       void* stream) {
   const auto bad = [](const std::string& what) { return fail(TF_EINVAL, "tf_rope_kv_cache_write: " + what); };
   std::string e = kv_cache_error(cache, dtype);
+  if (e.empty()) e = written_error(*cache);
   if (e.empty()) e = rows_error(q, q_token, q_head, "q");
   if (e.empty()) e = rows_error(k, k_token, k_head, "k");
   if (e.empty()) e = rows_error(v, v_token, v_head, "v");

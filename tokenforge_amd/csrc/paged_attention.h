@@ -1,7 +1,7 @@
 // Attention of one new token per sequence over a paged cache: the kernel template, instantiated by head length
 // in paged_attention_d*.hip, launched and joined by paged_attention.hip.
 //
-// Work. Items are (sequence, key-value head, 16 of its query heads); an item is a run of steps of 16 NT tokens.
+// Work. Items are (sequence, key-value head, 16 or 32 of its query heads); an item is a run of steps of 16 NT tokens.
 // All items' steps form one line, and workgroup w takes the steps [w share, (w + 1) share) of it, so every
 // workgroup gets the same number whatever the sequences' lengths are. Lengths are read on the device; the host
 // knows none. Items that lie in one workgroup are finished by it, the others leave (maximum, sum, accumulator)
@@ -135,8 +135,8 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_
 
 // T: type of q, out and 16-bit caches. DP: head length the tiles hold (d <= DP). PAGED: pages hold whole tiles of
 // 16 tokens (and scales go by 16-byte loads), so a tile's place is one scalar; else every token is looked up. FULL:
-// d == DP.
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+// d == DP. MT: 16s of query heads that share the loads of an item.
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
 struct Attn {
   static constexpr int kWaves = 4;
   static constexpr int NT = attention_step(DP) / 16;  // tiles of 16 tokens a step
@@ -156,9 +156,9 @@ struct Attn {
   f4 ks[NT], vs[NT];  // PAGED: scales of tokens 4g .. 4g + 3
   float ks1, vs1;     // else: of the lane's own token
 
-  f4 acc[NSUB * CS];
-  float top, sum;
-  u4 q[NK];
+  f4 acc[MT][NSUB * CS];
+  float top[MT], sum[MT];
+  u4 q[MT][NK];
 
   // Channels of MFMA j of the first product in lane group g: 8 from
   static __device__ __forceinline__ int k_at(int j, int g) {
@@ -232,10 +232,10 @@ __device__ __forceinline__ uint64_t step_bits(const Places& p, int slot) {
 
 // ------------------------------------------------------------------ loads
 
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, const uint8_t* kh,
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, const uint8_t* kh,
                                        const float* ksh, const Places& at, int slot, int lane) {
-  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
   const int c = lane & 15, g = lane >> 4;
   if (FP8 && !PAGED) s.ks1 = ksh[at.ks];
 #pragma unroll
@@ -263,10 +263,10 @@ __device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, PAGED
   }
 }
 
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, const uint8_t* vh,
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, const uint8_t* vh,
                                        const float* vsh, const Places& at, int slot, int lane) {
-  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
   const int c = lane & 15, g = lane >> 4;
   if (FP8 && !PAGED) s.vs1 = vsh[at.vs];
 #pragma unroll
@@ -318,15 +318,17 @@ __device__ __forceinline__ bool all_take_part(uint32_t step, int begin, int end,
 
 // Scores of the step's tokens, in units of log2, -inf where a token takes no part: x[tile][r] of head c, token
 // 4g + r.
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED, FULL>& s, uint32_t step, int begin,
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, uint32_t step, int begin,
                                        int end, uint64_t bits, int lane,
-                                       float (&x)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
-  using A = Attn<T, FP8, DP, PAGED, FULL>;
+                                       float (&x)[MT][Attn<T, FP8, DP, MT, PAGED, FULL>::NT][4]) {
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
   const int g = lane >> 4;
 #pragma unroll
   for (int i = 0; i < A::NT; ++i) {
-    f4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+    f4 t[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) t[m] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < A::NK; ++j) {
       u4 f;
@@ -339,13 +341,15 @@ __device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED
         f = s.k[i][j];
       }
       if (!FULL && A::k_at(j, g) >= a.d) f = u4{0u, 0u, 0u, 0u};
-      t = mfma16<T::kWide>(f, s.q[j], t);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) t[m] = mfma16<T::kWide>(f, s.q[m][j], t[m]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float y = t[r] * a.scale_log2;
-      if (FP8) y *= PAGED ? s.ks[i][r] : as_f32((uint32_t)from_lane32(as_u32(s.ks1), 16 * i + 4 * g + r));
-      x[i][r] = y;
+      float ks = 1.0f;
+      if (FP8) ks = PAGED ? s.ks[i][r] : as_f32(from_lane32(as_u32(s.ks1), 16 * i + 4 * g + r));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[m][i][r] = FP8 ? t[m][r] * a.scale_log2 * ks : t[m][r] * a.scale_log2;
     }
   }
   if (all_take_part<A, PAGED>(step, begin, end, bits)) return;
@@ -353,45 +357,51 @@ __device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, PAGED
   for (int i = 0; i < A::NT; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (!takes_part<A, PAGED>(step, i, r, g, begin, end, bits)) x[i][r] = -__builtin_inff();
+      if (!takes_part<A, PAGED>(step, i, r, g, begin, end, bits)) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) x[m][i][r] = -__builtin_inff();
+      }
 }
 
 // Scores -> probabilities: the running maximum, the accumulators' rescaling, the sum.
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__device__ __forceinline__ void softmax(Attn<T, FP8, DP, PAGED, FULL>& s,
-                                        float (&x)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
-  using A = Attn<T, FP8, DP, PAGED, FULL>;
-  float m = x[0][0];
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__device__ __forceinline__ void softmax(Attn<T, FP8, DP, MT, PAGED, FULL>& s,
+                                        float (&x)[MT][Attn<T, FP8, DP, MT, PAGED, FULL>::NT][4]) {
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
 #pragma unroll
-  for (int i = 0; i < A::NT; ++i)
+  for (int t = 0; t < MT; ++t) {
+    float m = x[t][0][0];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) m = __builtin_fmaxf(m, x[i][r]);
-  m = __builtin_fmaxf(s.top, max4(m));
-  if (__builtin_amdgcn_ballot_w64(m > s.top)) {
-    // -inf -> anything: nothing is there to rescale
-    const float f = s.top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s.top - m);
-    s.sum *= f;
+    for (int i = 0; i < A::NT; ++i)
 #pragma unroll
-    for (int j = 0; j < A::NSUB * A::CS; ++j)
+      for (int r = 0; r < 4; ++r) m = __builtin_fmaxf(m, x[t][i][r]);
+    m = __builtin_fmaxf(s.top[t], max4(m));
+    if (__builtin_amdgcn_ballot_w64(m > s.top[t])) {
+      // -inf -> anything: nothing is there to rescale
+      const float f = s.top[t] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s.top[t] - m);
+      s.sum[t] *= f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.acc[j][r] *= f;
-    s.top = m;
-  }
-  const float ref = (m == -__builtin_inff() ? 0.0f : m) - (A::PW ? 0.0f : kBias);
+      for (int j = 0; j < A::NSUB * A::CS; ++j)
 #pragma unroll
-  for (int i = 0; i < A::NT; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      x[i][r] = __builtin_amdgcn_exp2f(x[i][r] - ref);
-      s.sum += x[i][r];
+        for (int r = 0; r < 4; ++r) s.acc[t][j][r] *= f;
+      s.top[t] = m;
     }
+    const float ref = (m == -__builtin_inff() ? 0.0f : m) - (A::PW ? 0.0f : kBias);
+#pragma unroll
+    for (int i = 0; i < A::NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[t][i][r] = __builtin_amdgcn_exp2f(x[t][i][r] - ref);
+        s.sum[t] += x[t][i][r];
+      }
+  }
 }
 
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
-__device__ __forceinline__ void accumulate(Attn<T, FP8, DP, PAGED, FULL>& s, uint32_t step, int begin, int end,
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__device__ __forceinline__ void accumulate(Attn<T, FP8, DP, MT, PAGED, FULL>& s, uint32_t step, int begin, int end,
                                            uint64_t bits, int lane,
-                                           float (&p)[Attn<T, FP8, DP, PAGED, FULL>::NT][4]) {
-  using A = Attn<T, FP8, DP, PAGED, FULL>;
+                                           float (&p)[MT][Attn<T, FP8, DP, MT, PAGED, FULL>::NT][4]) {
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
   const int g = lane >> 4;
   if (FP8 && !PAGED) {
 #pragma unroll
@@ -415,16 +425,18 @@ __device__ __forceinline__ void accumulate(Attn<T, FP8, DP, PAGED, FULL>& s, uin
   }
 #pragma unroll
   for (int u = 0; u < A::NT; u += 2) {
-    u4 hi, lo;
+    u4 hi[MT], lo[MT];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = u + (x >> 1), r = 2 * (x & 1);
-      const float p0 = FP8 ? p[i][r] * s.vs[i][r] : p[i][r];
-      const float p1 = FP8 ? p[i][r + 1] * s.vs[i][r + 1] : p[i][r + 1];
-      uint32_t h, l;
-      split2<A::PW>(p0, p1, h, l);
-      hi[x] = h, lo[x] = l;
-    }
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int i = u + (x >> 1), r = 2 * (x & 1);
+        const float p0 = FP8 ? p[m][i][r] * s.vs[i][r] : p[m][i][r];
+        const float p1 = FP8 ? p[m][i][r + 1] * s.vs[i][r + 1] : p[m][i][r + 1];
+        uint32_t h, l;
+        split2<A::PW>(p0, p1, h, l);
+        hi[m][x] = h, lo[m][x] = l;
+      }
 #pragma unroll
     for (int n = 0; n < A::NSUB; ++n)
 #pragma unroll
@@ -446,11 +458,13 @@ __device__ __forceinline__ void accumulate(Attn<T, FP8, DP, PAGED, FULL>& s, uin
           }
         }
 #pragma unroll
-        for (int y = 0; y < (FP8 ? 4 : 2); ++y) {
-          f4& t = s.acc[n * A::CS + (FP8 ? 4 : 2) * w + y];
-          t = mfma16<A::PW>(f[y], hi, t);
-          t = mfma16<A::PW>(f[y], lo, t);
-        }
+        for (int y = 0; y < (FP8 ? 4 : 2); ++y)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            f4& t = s.acc[m][n * A::CS + (FP8 ? 4 : 2) * w + y];
+            t = mfma16<A::PW>(f[y], hi[m], t);
+            t = mfma16<A::PW>(f[y], lo[m], t);
+          }
       }
   }
 }
@@ -500,11 +514,11 @@ struct Item {
 };
 
 // The item's steps that `left` allow, from its step `at`.
-template <typename S>
+template <int MT, typename S>
 __device__ __forceinline__ Item item_of(const AttnArgs& a, const S& span, int b, uint32_t item, uint32_t at,
                                         uint32_t left) {
   const uint32_t stop = span.count - at < left ? span.count : at + left;
-  const int head = (int)(item / (uint32_t)a.row_groups), row = 16 * (int)(item - (uint32_t)head * a.row_groups);
+  const int head = (int)(item / (uint32_t)a.row_groups), row = 16 * MT * (int)(item - (uint32_t)head * a.row_groups);
   return Item{b, span.begin, span.end, head, row, item, span.first, span.count, at, stop};
 }
 
@@ -531,9 +545,9 @@ __device__ __forceinline__ Cut cut_line(const AttnArgs& a, uint32_t count, int l
   return Cut{total, (total + gridDim.x - 1) / gridDim.x, false};
 }
 
-template <typename T, bool FP8, int DP, bool PAGED, bool FULL>
+template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
 __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(AttnArgs a) {
-  using A = Attn<T, FP8, DP, PAGED, FULL>;
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
   using S = Span<A::KS>;
   __shared__ float rows[2][A::kWaves][16][A::ROW];
   __shared__ float2 ends[2][A::kWaves][16];  // (maximum, sum)
@@ -546,7 +560,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
   uint32_t left = ~0u, share = 0;  // steps of this workgroup behind the item, and of every workgroup
   if (a.direct) {
     const int b = (int)(blockIdx.x / per);
-    it = item_of(a, S(a, b), b, blockIdx.x - (uint32_t)b * per, 0, ~0u);
+    it = item_of<MT>(a, S(a, b), b, blockIdx.x - (uint32_t)b * per, 0, ~0u);
     left = 0;
   } else {
     // Every wave for itself, a sequence a lane: the line's length, then the sequence that holds the workgroup's first
@@ -576,7 +590,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
         own.begin = (int)of((uint32_t)own.begin), own.end = (int)of((uint32_t)own.end);
         own.first = of(own.first), own.count = of(own.count);
         const uint32_t size = room(own.count), rest = (uint32_t)start - (of(incl) - size) * per, item = rest / size;
-        it = item_of(a, own, i0 + at, item, rest - item * size, left);
+        it = item_of<MT>(a, own, i0 + at, item, rest - item * size, left);
         break;
       }
       before = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
@@ -588,7 +602,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
   left = scalar(left), share = scalar(share);
 
   A s;
-  const auto rows_of = [&](const Item& i) { return a.group - i.row < 16 ? a.group - i.row : 16; };
+  const auto rows_of = [&](const Item& i) { return a.group - i.row < 16 * MT ? a.group - i.row : 16 * MT; };
   const auto table_of = [&](const Item& i) { return a.table + (int64_t)i.b * a.table_row; };
   // Entries behind the workgroup's part are not fetched where its end is known: 64 of them are 32 lines of memory.
   const auto limit_of = [&](const Item& i) {
@@ -596,12 +610,15 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
     return a.direct || end > (uint32_t)a.cap ? (uint32_t)a.cap : end;
   };
   const auto load_q = [&](const Item& i) {  // rows past the group's end repeat its first and are not written
-    const int row = i.row + (c < rows_of(i) ? c : 0);
-    const uint16_t* const qp = a.q + (int64_t)i.b * a.q_row + (int64_t)(i.head * a.group + row) * a.q_head;
 #pragma unroll
-    for (int j = 0; j < A::NK; ++j) {
-      const int d0 = A::k_at(j, g);
-      s.q[j] = *reinterpret_cast<const u4*>(qp + (FULL || d0 < a.d ? d0 : 0));
+    for (int m = 0; m < MT; ++m) {
+      const int row = i.row + (16 * m + c < rows_of(i) ? 16 * m + c : 0);
+      const uint16_t* const qp = a.q + (int64_t)i.b * a.q_row + (int64_t)(i.head * a.group + row) * a.q_head;
+#pragma unroll
+      for (int j = 0; j < A::NK; ++j) {
+        const int d0 = A::k_at(j, g);
+        s.q[m][j] = *reinterpret_cast<const u4*>(qp + (FULL || d0 < a.d ? d0 : 0));
+      }
     }
   };
   const auto get_k = [&](const Item& i, const Places& at, int slot) {
@@ -634,7 +651,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
         do span = S(a, ++b);
         while (span.count == 0);
       }
-      next = item_of(a, span, b, item, 0, left);
+      next = item_of<MT>(a, span, b, item, 0, left);
       left -= next.stop;
     }
     const uint32_t next_step = next.first + next.at + (uint32_t)wave;
@@ -642,16 +659,22 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
     int next_entry = -1;
     if (next_has) next_entry = look_up<A, PAGED>(a, table_of(next), next_step, limit_of(next), lane);
 
-    s.top = -__builtin_inff(), s.sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < A::NSUB * A::CS; ++j) s.acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int m = 0; m < MT; ++m) {
+      s.top[m] = -__builtin_inff(), s.sum[m] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < A::NSUB * A::CS; ++j) s.acc[m][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     const uint32_t last = it.first + it.stop;
     if (has) {
-      float x[A::NT][4];
+      float x[MT][A::NT][4];
       if (!FULL) {
 #pragma unroll
         for (int j = 0; j < A::NK; ++j)
-          if (A::k_at(j, g) >= a.d) s.q[j] = u4{0u, 0u, 0u, 0u};
+          if (A::k_at(j, g) >= a.d) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) s.q[m][j] = u4{0u, 0u, 0u, 0u};
+          }
       }
       if (step + 4 * A::kAhead < last) entry = look_up<A, PAGED>(a, table_of(it), step + 4 * A::kAhead, limit_of(it), lane);
       for (; step + 4 < last; step += 4) {
@@ -680,54 +703,58 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
       get_v(next, at, slot);
     }
 
-    // The waves' parts side by side in one half of the LDS; the next item's go to the other, so that one barrier an
-    // item is enough: past it, every wave has read what it needs of the half before.
-    const int nrows = rows_of(it);
-    const float own = sum4(s.sum);
-    if (c < nrows) {
-      if (g == 0) ends[half][wave][c] = float2{s.top, own};
-#pragma unroll
-      for (int n = 0; n < A::NSUB; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int j = 0; j < A::CS; j += 4) {
-            f4 y;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) y[x] = s.acc[n * A::CS + j + x][r];
-            *reinterpret_cast<f4*>(&rows[half][wave][c][128 * n + (4 * g + r) * A::CS + j]) = y;
-          }
-    }
-    __syncthreads();
+    // The waves' parts of 16 heads side by side in one half of the LDS; the next 16's go to the other, so that one
+    // barrier each is enough: past it, every wave has read what it needs of the half before.
     const bool starts = it.at == 0, whole = starts && it.stop == it.count;
-    float* const piece =
-        whole ? nullptr : a.part + piece_of((int)blockIdx.x, starts) * a.part_rows * (DP + 2);
-    for (int e = tid; e < nrows * (DP / 4); e += 256) {
-      const int row = e / (DP / 4), d0 = (e - row * (DP / 4)) * 4;
-      float2 tl[A::kWaves];
-      f4 part[A::kWaves];
+    float* const piece = whole ? nullptr : a.part + piece_of((int)blockIdx.x, starts) * a.part_rows * (DP + 2);
 #pragma unroll
-      for (int w = 0; w < A::kWaves; ++w) {
-        tl[w] = ends[half][w][row];
-        part[w] = *reinterpret_cast<const f4*>(&rows[half][w][row][d0]);
-      }
-      const float t = __builtin_fmaxf(__builtin_fmaxf(tl[0].x, tl[1].x), __builtin_fmaxf(tl[2].x, tl[3].x));
-      float l = 0.0f;
-      f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int m = 0; m < MT; ++m) {
+      const int nrows = rows_of(it) - 16 * m < 16 ? rows_of(it) - 16 * m : 16;  // none of the last 16, maybe
+      const float own = sum4(s.sum[m]);
+      if (c < nrows) {
+        if (g == 0) ends[half][wave][c] = float2{s.top[m], own};
 #pragma unroll
-      for (int w = 0; w < A::kWaves; ++w) {
-        const float f = tl[w].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(tl[w].x - t);
-        l += tl[w].y * f;
-        y += part[w] * f;
+        for (int n = 0; n < A::NSUB; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < A::CS; j += 4) {
+              f4 y;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) y[x] = s.acc[m][n * A::CS + j + x][r];
+              *reinterpret_cast<f4*>(&rows[half][wave][c][128 * n + (4 * g + r) * A::CS + j]) = y;
+            }
       }
-      if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (FULL || d0 < a.d)
-          store4<T>(a.out + (((int64_t)it.b * a.heads + it.head) * a.group + it.row + row) * a.d + d0, y * inv);
-      } else {
-        *reinterpret_cast<f4*>(piece + row * DP + d0) = y;
-        if (d0 == 0) *reinterpret_cast<float2*>(piece + a.part_rows * DP + 2 * row) = float2{t, l};
+      __syncthreads();
+      for (int e = tid; e < nrows * (DP / 4); e += 256) {
+        const int row = e / (DP / 4), d0 = (e - row * (DP / 4)) * 4;
+        float2 tl[A::kWaves];
+        f4 part[A::kWaves];
+#pragma unroll
+        for (int w = 0; w < A::kWaves; ++w) {
+          tl[w] = ends[half][w][row];
+          part[w] = *reinterpret_cast<const f4*>(&rows[half][w][row][d0]);
+        }
+        const float t = __builtin_fmaxf(__builtin_fmaxf(tl[0].x, tl[1].x), __builtin_fmaxf(tl[2].x, tl[3].x));
+        float l = 0.0f;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < A::kWaves; ++w) {
+          const float f = tl[w].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(tl[w].x - t);
+          l += tl[w].y * f;
+          y += part[w] * f;
+        }
+        if (whole) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          if (FULL || d0 < a.d)
+            store4<T>(a.out + (((int64_t)it.b * a.heads + it.head) * a.group + it.row + 16 * m + row) * a.d + d0,
+                      y * inv);
+        } else {
+          *reinterpret_cast<f4*>(piece + (16 * m + row) * DP + d0) = y;
+          if (d0 == 0) *reinterpret_cast<float2*>(piece + a.part_rows * DP + 2 * (16 * m + row)) = float2{t, l};
+        }
       }
+      half ^= 1;
     }
     if (starts && tid == 0 && !a.direct) {
       // an item's last workgroup: `rest` steps of it lie behind this workgroup's
@@ -735,34 +762,37 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
       a.ends[(int64_t)it.b * per + it.item] = int2{(int)blockIdx.x, (int)(blockIdx.x + (rest + share - 1) / share)};
     }
     if (!more) return;
-    it = next, step = next_step, has = next_has, half ^= 1;
+    it = next, step = next_step, has = next_has;
   }
 }
 
-template <typename T, bool FP8, int DP>
+template <typename T, bool FP8, int DP, int MT>
 int launch_attention_as(const AttnArgs& a, bool paged, bool full, unsigned grid, hipStream_t stream) {
   if (paged && full)
-    attention_kernel<T, FP8, DP, true, true><<<grid, 256, 0, stream>>>(a);
+    attention_kernel<T, FP8, DP, MT, true, true><<<grid, 256, 0, stream>>>(a);
   else if (paged)
-    attention_kernel<T, FP8, DP, true, false><<<grid, 256, 0, stream>>>(a);
+    attention_kernel<T, FP8, DP, MT, true, false><<<grid, 256, 0, stream>>>(a);
   else
-    attention_kernel<T, FP8, DP, false, false><<<grid, 256, 0, stream>>>(a);
+    attention_kernel<T, FP8, DP, MT, false, false><<<grid, 256, 0, stream>>>(a);
   return check_launch("tf_paged_attention");
 }
 
-template <int DP>
-int launch_attention(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid,
-                     hipStream_t stream) {
-  if (bf16)
-    return fp8 ? launch_attention_as<BF16, true, DP>(a, paged, full, grid, stream)
-               : launch_attention_as<BF16, false, DP>(a, paged, full, grid, stream);
-  return fp8 ? launch_attention_as<F16, true, DP>(a, paged, full, grid, stream)
-             : launch_attention_as<F16, false, DP>(a, paged, full, grid, stream);
+struct AttnKind {
+  bool bf16, fp8, paged, full;
+};
+
+template <int DP, int MT>
+int launch_attention(const AttnArgs& a, const AttnKind& k, unsigned grid, hipStream_t stream) {
+  if (k.bf16)
+    return k.fp8 ? launch_attention_as<BF16, true, DP, MT>(a, k.paged, k.full, grid, stream)
+                 : launch_attention_as<BF16, false, DP, MT>(a, k.paged, k.full, grid, stream);
+  return k.fp8 ? launch_attention_as<F16, true, DP, MT>(a, k.paged, k.full, grid, stream)
+               : launch_attention_as<F16, false, DP, MT>(a, k.paged, k.full, grid, stream);
 }
 
-// One per head length, each in a file of its own.
-int launch_attention_d64(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
-int launch_attention_d128(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
-int launch_attention_d256(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid, hipStream_t s);
+// By head length and 16s of query heads, each head length in a file of its own.
+int launch_attention_d64(const AttnArgs& a, const AttnKind& k, int tiles, unsigned grid, hipStream_t stream);
+int launch_attention_d128(const AttnArgs& a, const AttnKind& k, int tiles, unsigned grid, hipStream_t stream);
+int launch_attention_d256(const AttnArgs& a, const AttnKind& k, unsigned grid, hipStream_t stream);
 
 }  // namespace tf

@@ -10,7 +10,7 @@ struct JoinArgs {
   const int2* ends;
   const int32_t* lens;
   uint16_t* out;
-  int heads, group, row_groups, part_rows, d, dp;
+  int heads, group, row_groups, part_rows, d, dp, tiles;
   uint32_t count;  // sequences * query heads
 };
 
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(Joi
   const uint32_t at = WAVES == 1 ? blockIdx.x * 4 + (uint32_t)wave : blockIdx.x;
   if (at >= a.count) return;
   const int b = (int)(at / q_heads), qh = (int)(at - (uint32_t)b * q_heads);
-  const int head = qh / a.group, in = qh - head * a.group, rg = in >> 4, row = in & 15;
+  const int head = qh / a.group, in = qh - head * a.group, rg = in / (16 * a.tiles), row = in - rg * 16 * a.tiles;
   const int n = a.lens[b];
   const int2 ends = a.ends[((int64_t)b * a.heads + head) * a.row_groups + rg];
   const int lanes = a.dp >> 2, side = 64 / lanes, part = lane / lanes, e = (lane & (lanes - 1)) * 4;
@@ -103,7 +103,7 @@ bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(
 
 // Sizes of a call, and "" or what is wrong with them.
 struct Plan {
-  int dp, group, row_groups, part_rows;
+  int dp, group, tiles, row_groups, part_rows;
   int64_t items, cap, part_floats, bytes;
   uint32_t grid;
   bool fp8, direct;
@@ -116,8 +116,10 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
   p.fp8 = c.dtype == TF_DTYPE_E4M3;
   p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   p.group = q_heads / c.heads;
-  p.row_groups = (int)cdiv(p.group, 16);
-  p.part_rows = p.group < 16 ? p.group : 16;
+  // Past 16 query heads a key-value head, 32 share its loads where the registers hold both.
+  p.tiles = p.group > 16 && p.dp <= 128 ? 2 : 1;
+  p.row_groups = (int)cdiv(p.group, 16 * p.tiles);
+  p.part_rows = p.group < 16 * p.tiles ? p.group : 16 * p.tiles;
   p.items = m * c.heads * p.row_groups;
   if (width > 0x7FFFFF00 / c.page_size) return "block_table covers 2^31 - 256 tokens or more";
   p.cap = width * c.page_size;
@@ -196,12 +198,15 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
     for (int i = 0; i < 3; ++i) full = full && c.k_strides[i] % 16 == 0;
   }
   const bool bf16 = dtype == TF_DTYPE_BF16;
+  const AttnKind kind{bf16, p.fp8, paged, full};
   const auto s = (hipStream_t)stream;
-  const auto launch = p.dp == 64 ? launch_attention_d64 : p.dp == 128 ? launch_attention_d128 : launch_attention_d256;
-  if (int rc = launch(a, bf16, p.fp8, paged, full, p.grid, s)) return rc;
+  const int rc = p.dp == 64    ? launch_attention_d64(a, kind, p.tiles, p.grid, s)
+                 : p.dp == 128 ? launch_attention_d128(a, kind, p.tiles, p.grid, s)
+                               : launch_attention_d256(a, kind, p.grid, s);
+  if (rc) return rc;
   if (p.direct) return TF_OK;
   const auto count = (uint32_t)(m * q_heads);
-  const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp, count};
+  const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp, p.tiles, count};
   if (count >= kJoinByWave)
     bf16 ? join_kernel<BF16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j)
          : join_kernel<F16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j);

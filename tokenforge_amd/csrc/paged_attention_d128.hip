@@ -3,9 +3,8 @@
 
 namespace tf {
 
-int launch_attention_d128(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid,
-                         hipStream_t stream) {
-  return launch_attention<128>(a, bf16, fp8, paged, full, grid, stream);
+int launch_attention_d128(const AttnArgs& a, const AttnKind& k, int tiles, unsigned grid, hipStream_t stream) {
+  return tiles == 1 ? launch_attention<128, 1>(a, k, grid, stream) : launch_attention<128, 2>(a, k, grid, stream);
 }
 
 }  // namespace tf

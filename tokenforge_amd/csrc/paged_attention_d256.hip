@@ -3,9 +3,8 @@
 
 namespace tf {
 
-int launch_attention_d256(const AttnArgs& a, bool bf16, bool fp8, bool paged, bool full, unsigned grid,
-                         hipStream_t stream) {
-  return launch_attention<256>(a, bf16, fp8, paged, full, grid, stream);
+int launch_attention_d256(const AttnArgs& a, const AttnKind& k, unsigned grid, hipStream_t stream) {
+  return launch_attention<256, 1>(a, k, grid, stream);
 }
 
 }  // namespace tf

@@ -738,6 +738,7 @@ bool cache_ok(const at::Tensor& k, const at::Tensor& v, const OptTensor& ks, con
   if (d == 0 || d % 8 != 0 || d > TF_KV_MAX_HEAD_DIM) return false;
   c = tf_kv_cache{};
   c.k = k.data_ptr(), c.v = v.data_ptr();
+  if (written && c.k == c.v) return false;
   c.pages = pages, c.heads = static_cast<int32_t>(heads), c.page_size = static_cast<int32_t>(page);
   c.head_dim = static_cast<int32_t>(d), c.dtype = dtype;
   cache_strides(k, c.k_strides);
@@ -755,6 +756,7 @@ bool cache_ok(const at::Tensor& k, const at::Tensor& v, const OptTensor& ks, con
     if (written && !elements_apart(*t)) return false;
   }
   c.k_scale = data<float>(*ks), c.v_scale = data<float>(*vs);
+  if (written && c.k_scale == c.v_scale) return false;
   cache_strides(*ks, c.k_scale_strides);
   cache_strides(*vs, c.v_scale_strides);
   return true;
