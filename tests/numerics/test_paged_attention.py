@@ -3,6 +3,8 @@ where it can go wrong. Bounds: ``kv_cases.check_attention``."""
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 from torch.library import opcheck
@@ -248,6 +250,8 @@ def test_scales_far_apart(device: torch.device) -> None:
         c = kc.cache(pages, 2, 16, 128, dtype, True)
         c.vs *= torch.exp2(torch.randint(-40, 3, c.vs.shape, generator=kc.gen("far")).float())
         c.ks *= torch.exp2(torch.randint(-40, 1, c.ks.shape, generator=kc.gen("far2")).float())
+        c.vs[:, 1] *= -1.0  # no quantizer writes such; they multiply all the same
+        c.ks[:, 1] *= -1.0
         q = _queries(2, 4, 128, dtype)
         out = ops.paged_attention(q.to(device), *c.to(device), table.to(device),
                                   torch.tensor(lens, dtype=torch.int32, device=device), 0.1, 0)
@@ -343,3 +347,18 @@ def test_opcheck_and_compile(device: torch.device) -> None:
     assert torch.equal(got, ops.paged_attention(*args) * 2)
     assert ops.paged_attention(q[:0], *c, table[:0].to(device), args[6][:0], 0.125, 0).shape == (0, 4, 64)
     assert not ops.paged_attention(q, *c, table[:, :0].to(device), args[6], 0.125, 0).any()
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_calls(seed: int, device: torch.device) -> None:
+    """Calls of no pattern: every combination of sizes, layouts and types that the operator takes can come up."""
+    rng = random.Random(seed)
+    dtype, fp8 = rng.choice(TYPES)
+    page = rng.choice((16, 16, 32, 64, rng.randint(1, 70)))
+    heads, group = rng.choice((1, 2, 3, 8)), rng.choice((1, 2, 7, 15, 16, 17, 31, 33, 40))
+    d = rng.choice((64, 128, 256, 8 * rng.randint(1, 32)))
+    longest = rng.choice((20, 100, 700, 4000))
+    lens = [rng.choice((0, 1, rng.randint(1, longest), rng.randint(1, longest))) for _ in range(rng.choice((1, 3, 20, 70)))]
+    width = rng.choice((0, 0, LINE // page, rng.randint(1, 2 * longest) // page))
+    _run(device, lens, heads, group, d, page, dtype, fp8, window=rng.choice((0, 0, rng.randint(1, longest))), width=width,
+         tokens_first=rng.random() < 0.3, scale=rng.choice((None, None, rng.uniform(-0.5, 0.5))), seed=seed)

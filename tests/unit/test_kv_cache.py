@@ -342,3 +342,20 @@ def test_kernel_limits_match_the_library() -> None:
     header = (_lib.LIB_PATH.parents[2] / "include" / "tokenforge_hip.h").read_text()
     assert f"#define TF_KV_MAX_HEAD_DIM {kv.MAX_HEAD_DIM}" in header
     assert f"#define TF_DTYPE_E4M3 {_lib.DTYPE_E4M3}" in header
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_the_attentions_bound_sees_a_token(dtype: torch.dtype) -> None:
+    """What the bound is held to: an oracle that misses one token, reads another page, has the window off by one or the
+    scale by 2% is outside it."""
+    lens = [60]
+    table, pages = kc.tables(lens, 16)
+    c = kc.cache(pages, 1, 16, 64, dtype, False)
+    q = _rows(1, 2, 64, dtype, 0)
+    out = ops.paged_attention(q, *c.to("cpu"), table, torch.tensor(lens, dtype=torch.int32), 0.05, 20)
+    kc.check_attention(out, q, c, table, lens, 0.05, 20)
+    swapped = table.clone()
+    swapped[0, 3] = table[0, 2]
+    for t, n, scale, window in ((table, 59, 0.05, 20), (swapped, 60, 0.05, 20), (table, 60, 0.05, 21), (table, 60, 0.051, 20)):
+        with pytest.raises(AssertionError):
+            kc.check_attention(out, q, c, t, [n], scale, window)

@@ -126,9 +126,8 @@ template <bool WIDE>
 __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   if (WIDE) {
     hi = __builtin_amdgcn_perm(as_u32(p1), as_u32(p0), 0x07060302u);
-    const float r0 = __builtin_fmaxf(p0 - as_f32(as_u32(p0) & 0xFFFF0000u), p0 * 0x1p-20f);
-    const float r1 = __builtin_fmaxf(p1 - as_f32(as_u32(p1) & 0xFFFF0000u), p1 * 0x1p-20f);
-    lo = round_pair<BF16>(r0, r1);
+    const float r0 = p0 - as_f32(as_u32(p0) & 0xFFFF0000u), r1 = p1 - as_f32(as_u32(p1) & 0xFFFF0000u);
+    lo = round_pair<BF16>(r0 != 0.0f ? r0 : p0 * 0x1p-20f, r1 != 0.0f ? r1 : p1 * 0x1p-20f);
   } else {
     const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
     hi = __builtin_bit_cast(uint32_t, h);
