@@ -46,7 +46,7 @@ struct AttnArgs {
   int64_t table_row;
   const int32_t* lens;
   uint16_t* out;
-  float* part;  // [2 grid] pieces of part_rows rows: accumulators [part_rows][DP], then (maximum, sum) [part_rows]
+  float* part;  // [2 grid] pieces of part_rows rows
   int2* ends;   // [items] first and last workgroup of an item
   int64_t pages;
   PageDiv page;
@@ -64,6 +64,9 @@ constexpr int attention_step(int dp) { return dp == 64 ? 64 : 32; }
 // Workgroups a CU holds, and the grid of the shared line: two by their 180 to 190 registers, one for heads past 128.
 constexpr int attention_resident(int dp) { return dp > 128 ? 1 : 2; }
 constexpr int attention_grid(int dp) { return 256 * attention_resident(dp); }
+
+// Floats of a piece: the rows' accumulators, then their (maximum, sum), up to 16 bytes.
+__host__ __device__ constexpr int64_t piece_floats(int rows, int dp) { return rows * dp + (2 * rows + 3) / 4 * 4; }
 
 // Where a workgroup leaves its part of an item: it has at most two such, of an item that began before it and of one
 // that begins in it and goes on behind it.
@@ -584,6 +587,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
     const uint32_t want = (uint32_t)start / per;
     uint32_t before = 0;
     for (int i0 = 0;; i0 += 64) {
+      if (i0 >= a.m) return;  // (only where lengths change under the call)
       if (i0) {
         own = S(a, i0 + lane < a.m ? i0 + lane : a.m - 1);
         if (i0 + lane >= a.m) own.count = 0;
@@ -645,7 +649,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
   }
   for (;;) {
     // The item behind this one, and its first entry of the table.
-    const bool more = left != 0;
+    bool more = left != 0;
     Item next = it;
     if (more) {
       uint32_t item = it.item + 1;
@@ -653,11 +657,13 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
       S span{it.begin, it.end, it.first, it.count};
       if (item == per) {
         item = 0;
-        do span = S(a, ++b);
-        while (span.count == 0);
+        do
+          if (++b < a.m) span = S(a, b);
+        while (b < a.m && span.count == 0);
       }
-      next = item_of<MT>(a, span, b, item, 0, left);
-      left -= next.stop;
+      more = b < a.m;  // (always, but where lengths change under the call)
+      next = more ? item_of<MT>(a, span, b, item, 0, left) : it;
+      left -= more ? next.stop : 0;
     }
     const uint32_t next_step = next.first + next.at + (uint32_t)wave;
     const bool next_has = more && next_step < next.first + next.stop;
@@ -711,7 +717,7 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
     // The waves' parts of 16 heads side by side in one half of the LDS; the next 16's go to the other, so that one
     // barrier each is enough: past it, every wave has read what it needs of the half before.
     const bool starts = it.at == 0, whole = starts && it.stop == it.count;
-    float* const piece = whole ? nullptr : a.part + piece_of((int)blockIdx.x, starts) * a.part_rows * (DP + 2);
+    float* const piece = whole ? nullptr : a.part + piece_of((int)blockIdx.x, starts) * piece_floats(a.part_rows, DP);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int nrows = rows_of(it) - 16 * m < 16 ? rows_of(it) - 16 * m : 16;  // none of the last 16, maybe

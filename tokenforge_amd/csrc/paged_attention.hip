@@ -53,7 +53,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(Joi
     return;
   }
   if (ends.x == ends.y) return;
-  const int64_t size = (int64_t)a.part_rows * (a.dp + 2);
+  const int64_t size = piece_floats(a.part_rows, a.dp);
   Part mine{-__builtin_inff(), 0.0f, f4{0.0f, 0.0f, 0.0f, 0.0f}};
   const int each = WAVES * side;
   for (int p0 = ends.x + (WAVES == 1 ? 0 : wave) * side + part; p0 <= ends.y; p0 += each * kOnce) {
@@ -134,7 +134,7 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
   const int64_t bytes = most * step * 2 * p.dp * (p.fp8 ? 1 : 2);
   p.direct = bytes <= (p.items >= kManyItems ? kDirectMany : kDirect);
   p.grid = p.direct ? (uint32_t)p.items : (uint32_t)attention_grid(p.dp);
-  p.part_floats = p.direct ? 0 : 2 * (int64_t)p.grid * p.part_rows * (p.dp + 2);
+  p.part_floats = p.direct ? 0 : 2 * (int64_t)p.grid * piece_floats(p.part_rows, p.dp);
   p.bytes = p.direct ? 0 : p.part_floats * 4 + p.items * 8;
   return "";
 }
