@@ -267,18 +267,46 @@ def test_offsets_past_32_bits(fp8: bool, device: torch.device) -> None:
           host.kv_cache_read(c.k, c.v, c.ks, c.vs, slots, dtype))
 
 
+@pytest.mark.parametrize("page", [32, 24])
+def test_slots_past_31_bits(page: int, device: torch.device) -> None:
+    """Slot numbers up to 2^33 (a page repeated 2^28 times)."""
+    one = torch.randn((1, 2, page, 64), generator=kc.gen("repeated")).half()
+    pages = 1 << 28
+    cache = one.to(device).expand(pages, -1, -1, -1)
+    slots = torch.tensor([0, 2**31 - 1, 2**31, 2**31 + 7, 2**32 + 5, pages * page - 1, pages * page, 2**31 - page, 5 * page])
+    k, v = ops.kv_cache_read(cache, cache, None, None, slots.to(device), torch.float16)
+    want = one[0, :, slots % page].transpose(0, 1).clone()
+    want[6] = 0
+    assert torch.equal(k.cpu(), want) and torch.equal(v, k)
+
+
 def test_many_tokens(device: torch.device) -> None:
-    """More rows than a launch takes at once are written in parts."""
+    """Tens of thousands of tokens; and more rows than a launch takes (2^26), written, rotated and read in parts."""
     t, heads, d, page = 20000, 12, 64, 128
     pages = t // page + 1
-    k, v = torch.randn((2, 1, heads, d), device=device).half().expand(2, t, heads, d).unbind(0)
-    k = k + torch.arange(t, device=device).half()[:, None, None] / 64
+    k = torch.randn((1, heads, d), device=device).half().expand(t, heads, d)
+    v = k + torch.arange(t, device=device).half()[:, None, None] / 64
     dev = kc.cache(pages, heads, page, d, torch.float16, True).to(device)
     slots = torch.arange(t, device=device)
     ops.kv_cache_write(k, v, *dev, slots)
-    k2, _ = ops.kv_cache_read(*dev, slots, torch.float16)
-    top = k.float().abs().amax(-1, keepdim=True)
-    assert ((k2.float() - k.float()).abs() <= top * (2.0**-4 + 2.0**-8)).all()
+    for x, got in zip((k, v), ops.kv_cache_read(*dev, slots, torch.float16)):
+        top = x.float().abs().amax(-1, keepdim=True)
+        assert ((got.float() - x.float()).abs() <= top * (2.0**-4 + 2.0**-8)).all()
+    del dev
+    t, heads, d, page = 2500, 16384, 8, 50  # 2048 tokens a launch; with as many queries 1365
+    x = torch.randn((t, 1, d), device=device).bfloat16()
+    k, slots = x.expand(t, heads, d), torch.arange(t, device=device).flip(0)
+    cache = [torch.zeros((t // page, heads, page, d), dtype=torch.bfloat16, device=device) for _ in "kv"]
+    ops.kv_cache_write(k, -k, *cache, None, None, slots)
+    got = ops.kv_cache_read(*cache, None, None, slots, torch.bfloat16)
+    assert torch.equal(got[0], k) and torch.equal(got[1], -k)
+    quarter = torch.tensor([[0.0] * 4 + [1.0] * 4], device=device)  # a quarter turn: (a, b) -> (-b, a)
+    q = ops.rope_kv_cache_write(-k, k, k, quarter, torch.zeros_like(slots), *cache, None, None, slots)
+    turned = torch.cat([-x[..., 4:], x[..., :4]], -1).expand(t, heads, d)
+    assert torch.equal(q, -turned)
+    del q, got
+    got = ops.kv_cache_read(*cache, None, None, slots, torch.bfloat16)
+    assert torch.equal(got[0], turned) and torch.equal(got[1], k)
 
 
 def test_graphs_streams_and_opcheck(device: torch.device) -> None:
