@@ -101,6 +101,26 @@ def test_every_way_to_share_the_work(lens: list[int], fp8: bool, device: torch.d
 
 
 @pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
+@pytest.mark.parametrize(("d", "group"), [(64, 4), (64, 20), (128, 4), (128, 20), (256, 4)])
+@pytest.mark.parametrize("whole", [False, True], ids=["shared", "whole"])
+def test_calls_of_many_bytes(whole: bool, d: int, group: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:
+    """Below and past 100 MiB of keys and values on the line, and 384 MiB in the table of items that a workgroup takes
+    whole: the same four sequences again and again, over the same pages."""
+    row = 2 * d * (1 if fp8 else 2)
+    capacity = (512 << 10) // row if whole else LINE
+    lens = [min(2049, capacity), capacity // 2 + 1 if whole else 1777, 1, 300]
+    past = 101 if whole else (60 << 20) // (sum(lens) * row) + 1  # 808 items of 512 KB; 120 MiB of 2 heads
+    table, pages = kc.tables(lens, 16, capacity // 16)
+    c = kc.cache(pages, 2, 16, d, dtype, fp8)
+    q = _queries(len(lens), 2 * group, d, dtype)
+    for n in (80 if whole else past // 4, past):
+        out = ops.paged_attention(q.repeat(n, 1, 1).to(device), *c.to(device), table.repeat(n, 1).to(device),
+                                  torch.tensor(lens * n, dtype=torch.int32, device=device), d**-0.5, 0)
+        for at in (0, n // 2, n - 1):
+            kc.check_attention(out[4 * at:4 * at + 4], q, c, table, lens, d**-0.5)
+
+
+@pytest.mark.parametrize(("dtype", "fp8"), TYPES, ids=IDS)
 @pytest.mark.parametrize("page", [16, 8])
 @pytest.mark.parametrize("capacity", [0, LINE])
 def test_layouts(capacity: int, page: int, dtype: torch.dtype, fp8: bool, device: torch.device) -> None:

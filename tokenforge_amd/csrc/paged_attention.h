@@ -7,9 +7,9 @@
 // knows none. Items that lie in one workgroup are finished by it, the others leave (maximum, sum, accumulator)
 // in the workspace for the join.
 //
-// Memory bound: every cached byte is read once (counters: 1.004 times the cache's bytes), 4 q_heads d flops a token are
+// Memory bound: every cached byte is read once (counters: 1.004 to 1.02 times the cache's bytes), 4 q_heads d flops a token are
 // 3% of the matrix rate at that speed. On MI355X (copy of 1 GiB 5.14 TB/s), head length 128, 28 query on 4 key-value
-// heads, us: 64 sequences of 2000 to 16384 tokens in bf16 (929 MB) 164 and 5 for the join, 32 of up to 4096 (69 MB) 15.2
+// heads, us: 64 sequences of 2000 to 16384 tokens in bf16 (929 MB) 147 and 5 for the join, 32 of up to 4096 (69 MB) 15.6
 // and 4.0, 128 of up to 2048 in e4m3 (90 MB) 24.4 in one launch, one of 32749 in e4m3 (35 MB) 11.5 and 4.9. Beside
 // the bytes a call takes some 5.5 (a launch; lengths, table and keys wait for each other; the last join in LDS).
 //
@@ -67,6 +67,14 @@ constexpr int attention_grid(int dp) { return 256 * attention_resident(dp); }
 
 // Floats of a piece: the rows' accumulators, then their (maximum, sum), up to 16 bytes.
 __host__ __device__ constexpr int64_t piece_floats(int rows, int dp) { return rows * dp + (2 * rows + 3) / 4 * 4; }
+
+// Bytes of keys and values from which a call's loads are nontemporal, by what its line holds or, where a workgroup takes
+// a whole item and none knows the others' lengths, by what the table covers. Each byte is read once; a call that fills
+// a good part of the 256 MB last-level cache only pushes out of it what other kernels left. MI355X, three caches in
+// turn, us without and with: 64 sequences of 2000 to 16384 tokens (929 MB) 169 and 150, 8 of 8192 (134 MB) 31.7 and
+// 28.5; 32 of up to 4096 (69 MB), where three caches stay in it, 19.2 and 21.4. Whole items: 512 of up to 512 tokens (table
+// 537 MB) 97.4 and 92.1, 128 of up to 2048 in e4m3 (table 268 MB) 24.1 and 26.3.
+constexpr int64_t kStreamLine = 100 << 20, kStreamTable = 384 << 20;
 
 // Where a workgroup leaves its part of an item: it has at most two such, of an item that began before it and of one
 // that begins in it and goes on behind it.
@@ -240,7 +248,12 @@ __device__ __forceinline__ uint64_t step_bits(const Places& p, int slot) {
 
 // ------------------------------------------------------------------ loads
 
-template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load_as(const uint8_t* p) {
+  return STREAM ? __builtin_nontemporal_load(reinterpret_cast<const V*>(p)) : *reinterpret_cast<const V*>(p);
+}
+
+template <bool STREAM, typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
 __device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, const uint8_t* kh,
                                        const float* ksh, const Places& at, int slot, int lane) {
   using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
@@ -259,19 +272,19 @@ __device__ __forceinline__ void load_k(const AttnArgs& a, Attn<T, FP8, DP, MT, P
     for (int w = 0; w < A::KW; ++w) {
       const int d0 = FP8 ? 64 * w + 16 * g : 32 * w + 8 * g;
       if (FULL) {
-        s.k[i][w] = *reinterpret_cast<const u4*>(base + d0 * A::E);
+        s.k[i][w] = load_as<STREAM, u4>(base + d0 * A::E);
       } else if (FP8) {  // rows of 8-byte alignment; channels past d from the row's start, cleared in scores()
-        const u2 lo = *reinterpret_cast<const u2*>(base + (d0 < a.d ? d0 : 0));
-        const u2 hi = *reinterpret_cast<const u2*>(base + (d0 + 8 < a.d ? d0 + 8 : 0));
+        const u2 lo = load_as<STREAM, u2>(base + (d0 < a.d ? d0 : 0));
+        const u2 hi = load_as<STREAM, u2>(base + (d0 + 8 < a.d ? d0 + 8 : 0));
         s.k[i][w] = u4{lo[0], lo[1], hi[0], hi[1]};
       } else {
-        s.k[i][w] = *reinterpret_cast<const u4*>(base + (d0 < a.d ? d0 : 0) * A::E);
+        s.k[i][w] = load_as<STREAM, u4>(base + (d0 < a.d ? d0 : 0) * A::E);
       }
     }
   }
 }
 
-template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+template <bool STREAM, typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
 __device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, const uint8_t* vh,
                                        const float* vsh, const Places& at, int slot, int lane) {
   using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
@@ -293,15 +306,15 @@ __device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, MT, P
         const int d0 = 128 * n + A::CS * c;
         const uint8_t* const p = base + (FULL || d0 < a.d ? d0 : 0) * A::E;
         if (A::VW == 4) {
-          const u4 w = *reinterpret_cast<const u4*>(p);
+          const u4 w = load_as<STREAM, u4>(p);
 #pragma unroll
           for (int x = 0; x < A::VW; ++x) s.v[i][r][n][x] = w[x & 3];
         } else if (A::VW == 2) {
-          const u2 w = *reinterpret_cast<const u2*>(p);
+          const u2 w = load_as<STREAM, u2>(p);
 #pragma unroll
           for (int x = 0; x < A::VW; ++x) s.v[i][r][n][x] = w[x & 1];
         } else {
-          s.v[i][r][n][0] = *reinterpret_cast<const uint32_t*>(p);
+          s.v[i][r][n][0] = load_as<STREAM, uint32_t>(p);
         }
       }
     }
@@ -553,64 +566,17 @@ __device__ __forceinline__ Cut cut_line(const AttnArgs& a, uint32_t count, int l
   return Cut{total, (total + gridDim.x - 1) / gridDim.x, false};
 }
 
-template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
-__global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(AttnArgs a) {
-  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
+// A workgroup's items from `it` on, `left` steps behind it.
+template <typename A, bool STREAM, typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t left, uint32_t share,
+                                          float (&rows)[2][A::kWaves][16][A::ROW],
+                                          float2 (&ends)[2][A::kWaves][16]) {
   using S = Span<A::KS>;
-  __shared__ float rows[2][A::kWaves][16][A::ROW];
-  __shared__ float2 ends[2][A::kWaves][16];  // (maximum, sum)
   int half = 0;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const uint32_t per = (uint32_t)(a.heads * a.row_groups);  // items of a sequence
-
-  Item it;
-  uint32_t left = ~0u, share = 0;  // steps of this workgroup behind the item, and of every workgroup
-  if (a.direct) {
-    const int b = (int)(blockIdx.x / per);
-    it = item_of<MT>(a, S(a, b), b, blockIdx.x - (uint32_t)b * per, 0, ~0u);
-    left = 0;
-  } else {
-    // Every wave for itself, a sequence a lane: the line's length, then the sequence that holds the workgroup's first
-    // step. Parts of one item where the grid allows it: the end of an item costs a workgroup some us.
-    S own(a, lane < a.m ? lane : a.m - 1);
-    if (lane >= a.m) own.count = 0;
-    Cut line = cut_line<S>(a, own.count, lane, per, 4, 8, 12);
-    if (!line.apart && line.share <= 32) line = cut_line<S>(a, own.count, lane, per, 16, 24, 32);
-    const bool apart = line.apart;
-    const uint32_t total = line.total;
-    share = line.share;
-    const auto room = [&](uint32_t count) { return apart ? (count + share - 1) / share * share : count; };
-    const uint64_t start = (uint64_t)blockIdx.x * share;
-    if (start >= total) return;
-    left = total - (uint32_t)start < share ? total - (uint32_t)start : share;
-    const uint32_t want = (uint32_t)start / per;
-    uint32_t before = 0;
-    for (int i0 = 0;; i0 += 64) {
-      if (i0 >= a.m) return;  // (only where lengths change under the call)
-      if (i0) {
-        own = S(a, i0 + lane < a.m ? i0 + lane : a.m - 1);
-        if (i0 + lane >= a.m) own.count = 0;
-      }
-      const uint32_t incl = before + wave_scan_u32(room(own.count));
-      const int at = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= want));
-      if (at < 64) {
-        const auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
-        own.begin = (int)of((uint32_t)own.begin), own.end = (int)of((uint32_t)own.end);
-        own.first = of(own.first), own.count = of(own.count);
-        const uint32_t size = room(own.count), rest = (uint32_t)start - (of(incl) - size) * per, item = rest / size;
-        it = item_of<MT>(a, own, i0 + at, item, rest - item * size, left);
-        break;
-      }
-      before = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-    }
-    left = apart ? 0 : left - (it.stop - it.at);
-  }
-  it = Item{(int)scalar(it.b), (int)scalar(it.begin), (int)scalar(it.end), (int)scalar(it.head), (int)scalar(it.row),
-            scalar(it.item), scalar(it.first), scalar(it.count), scalar(it.at), scalar(it.stop)};
-  left = scalar(left), share = scalar(share);
-
-  A s;
+  Attn<T, FP8, DP, MT, PAGED, FULL> s;
   const auto rows_of = [&](const Item& i) { return a.group - i.row < 16 * MT ? a.group - i.row : 16 * MT; };
   const auto table_of = [&](const Item& i) { return a.table + (int64_t)i.b * a.table_row; };
   // Entries behind the workgroup's part are not fetched where its end is known: 64 of them are 32 lines of memory.
@@ -631,10 +597,10 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
     }
   };
   const auto get_k = [&](const Item& i, const Places& at, int slot) {
-    load_k(a, s, a.k + i.head * a.k_head, FP8 ? a.ks + i.head * a.ks_head : nullptr, at, slot, lane);
+    load_k<STREAM>(a, s, a.k + i.head * a.k_head, FP8 ? a.ks + i.head * a.ks_head : nullptr, at, slot, lane);
   };
   const auto get_v = [&](const Item& i, const Places& at, int slot) {
-    load_v(a, s, a.v + i.head * a.v_head, FP8 ? a.vs + i.head * a.vs_head : nullptr, at, slot, lane);
+    load_v<STREAM>(a, s, a.v + i.head * a.v_head, FP8 ? a.vs + i.head * a.vs_head : nullptr, at, slot, lane);
   };
 
   // The first step's loads; then each item's, while the item before it ends.
@@ -777,28 +743,95 @@ __global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(
   }
 }
 
-template <typename T, bool FP8, int DP, int MT>
-int launch_attention_as(const AttnArgs& a, bool paged, bool full, unsigned grid, hipStream_t stream) {
-  if (paged && full)
-    attention_kernel<T, FP8, DP, MT, true, true><<<grid, 256, 0, stream>>>(a);
-  else if (paged)
-    attention_kernel<T, FP8, DP, MT, true, false><<<grid, 256, 0, stream>>>(a);
+// STREAM: the call may be one for nontemporal loads. (Of two loops where one is run, the other's code costs the small
+// calls some 0.3 us.)
+template <bool STREAM, typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
+__global__ __launch_bounds__(256, attention_resident(DP)) void attention_kernel(AttnArgs a) {
+  using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
+  using S = Span<A::KS>;
+  __shared__ float rows[2][A::kWaves][16][A::ROW];
+  __shared__ float2 ends[2][A::kWaves][16];  // (maximum, sum)
+  const int lane = threadIdx.x & 63;
+  const uint32_t per = (uint32_t)(a.heads * a.row_groups);  // items of a sequence
+
+  Item it;
+  bool stream = STREAM;
+  uint32_t left = ~0u, share = 0;  // steps of this workgroup behind the item, and of every workgroup
+  if (a.direct) {
+    const int b = (int)(blockIdx.x / per);
+    it = item_of<MT>(a, S(a, b), b, blockIdx.x - (uint32_t)b * per, 0, ~0u);
+    left = 0;
+  } else {
+    // Every wave for itself, a sequence a lane: the line's length, then the sequence that holds the workgroup's first
+    // step. Parts of one item where the grid allows it: the end of an item costs a workgroup some us.
+    S own(a, lane < a.m ? lane : a.m - 1);
+    if (lane >= a.m) own.count = 0;
+    Cut line = cut_line<S>(a, own.count, lane, per, 4, 8, 12);
+    if (!line.apart && line.share <= 32) line = cut_line<S>(a, own.count, lane, per, 16, 24, 32);
+    const bool apart = line.apart;
+    const uint32_t total = line.total;
+    share = line.share;
+    stream = STREAM && (uint64_t)total * (A::KS * 2 * DP * A::E) >= (uint64_t)kStreamLine * (uint32_t)a.row_groups;
+    const auto room = [&](uint32_t count) { return apart ? (count + share - 1) / share * share : count; };
+    const uint64_t start = (uint64_t)blockIdx.x * share;
+    if (start >= total) return;
+    left = total - (uint32_t)start < share ? total - (uint32_t)start : share;
+    const uint32_t want = (uint32_t)start / per;
+    uint32_t before = 0;
+    for (int i0 = 0;; i0 += 64) {
+      if (i0 >= a.m) return;  // (only where lengths change under the call)
+      if (i0) {
+        own = S(a, i0 + lane < a.m ? i0 + lane : a.m - 1);
+        if (i0 + lane >= a.m) own.count = 0;
+      }
+      const uint32_t incl = before + wave_scan_u32(room(own.count));
+      const int at = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(incl <= want));
+      if (at < 64) {
+        const auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+        own.begin = (int)of((uint32_t)own.begin), own.end = (int)of((uint32_t)own.end);
+        own.first = of(own.first), own.count = of(own.count);
+        const uint32_t size = room(own.count), rest = (uint32_t)start - (of(incl) - size) * per, item = rest / size;
+        it = item_of<MT>(a, own, i0 + at, item, rest - item * size, left);
+        break;
+      }
+      before = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    }
+    left = apart ? 0 : left - (it.stop - it.at);
+  }
+  it = Item{(int)scalar(it.b), (int)scalar(it.begin), (int)scalar(it.end), (int)scalar(it.head), (int)scalar(it.row),
+            scalar(it.item), scalar(it.first), scalar(it.count), scalar(it.at), scalar(it.stop)};
+  left = scalar(left), share = scalar(share);
+
+  if (STREAM && stream)
+    run_items<A, true, T, FP8, DP, MT, PAGED, FULL>(a, it, left, share, rows, ends);
   else
-    attention_kernel<T, FP8, DP, MT, false, false><<<grid, 256, 0, stream>>>(a);
-  return check_launch("tf_paged_attention");
+    run_items<A, false, T, FP8, DP, MT, PAGED, FULL>(a, it, left, share, rows, ends);
 }
 
 struct AttnKind {
-  bool bf16, fp8, paged, full;
+  bool bf16, fp8, paged, full, stream;
 };
+
+template <typename T, bool FP8, int DP, int MT>
+int launch_attention_as(const AttnArgs& a, const AttnKind& k, unsigned grid, hipStream_t stream) {
+  if (k.paged && k.full && k.stream)
+    attention_kernel<true, T, FP8, DP, MT, true, true><<<grid, 256, 0, stream>>>(a);
+  else if (k.paged && k.full)
+    attention_kernel<false, T, FP8, DP, MT, true, true><<<grid, 256, 0, stream>>>(a);
+  else if (k.paged)
+    attention_kernel<false, T, FP8, DP, MT, true, false><<<grid, 256, 0, stream>>>(a);
+  else
+    attention_kernel<false, T, FP8, DP, MT, false, false><<<grid, 256, 0, stream>>>(a);
+  return check_launch("tf_paged_attention");
+}
 
 template <int DP, int MT>
 int launch_attention(const AttnArgs& a, const AttnKind& k, unsigned grid, hipStream_t stream) {
   if (k.bf16)
-    return k.fp8 ? launch_attention_as<BF16, true, DP, MT>(a, k.paged, k.full, grid, stream)
-                 : launch_attention_as<BF16, false, DP, MT>(a, k.paged, k.full, grid, stream);
-  return k.fp8 ? launch_attention_as<F16, true, DP, MT>(a, k.paged, k.full, grid, stream)
-               : launch_attention_as<F16, false, DP, MT>(a, k.paged, k.full, grid, stream);
+    return k.fp8 ? launch_attention_as<BF16, true, DP, MT>(a, k, grid, stream)
+                 : launch_attention_as<BF16, false, DP, MT>(a, k, grid, stream);
+  return k.fp8 ? launch_attention_as<F16, true, DP, MT>(a, k, grid, stream)
+               : launch_attention_as<F16, false, DP, MT>(a, k, grid, stream);
 }
 
 // By head length and 16s of query heads, each head length in a file of its own.

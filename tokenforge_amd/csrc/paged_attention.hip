@@ -106,7 +106,7 @@ struct Plan {
   int dp, group, tiles, row_groups, part_rows;
   int64_t items, cap, part_floats, bytes;
   uint32_t grid;
-  bool fp8, direct;
+  bool fp8, direct, stream;
 };
 
 std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t width, int64_t window, Plan& p) {
@@ -133,6 +133,7 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
   if (window > 0) most = most < cdiv(window, step) + 1 ? most : cdiv(window, step) + 1;
   const int64_t bytes = most * step * 2 * p.dp * (p.fp8 ? 1 : 2);
   p.direct = bytes <= (p.items >= kManyItems ? kDirectMany : kDirect);
+  p.stream = m * c.heads * bytes >= (p.direct ? kStreamTable : kStreamLine);
   p.grid = p.direct ? (uint32_t)p.items : (uint32_t)attention_grid(p.dp);
   p.part_floats = p.direct ? 0 : 2 * (int64_t)p.grid * piece_floats(p.part_rows, p.dp);
   p.bytes = p.direct ? 0 : p.part_floats * 4 + p.items * 8;
@@ -198,7 +199,7 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
     for (int i = 0; i < 3; ++i) full = full && c.k_strides[i] % 16 == 0;
   }
   const bool bf16 = dtype == TF_DTYPE_BF16;
-  const AttnKind kind{bf16, p.fp8, paged, full};
+  const AttnKind kind{bf16, p.fp8, paged, full, p.stream};
   const auto s = (hipStream_t)stream;
   const int rc = p.dp == 64    ? launch_attention_d64(a, kind, p.tiles, p.grid, s)
                  : p.dp == 128 ? launch_attention_d128(a, kind, p.tiles, p.grid, s)
