@@ -7,11 +7,12 @@
 // knows none. Items that lie in one workgroup are finished by it, the others leave (maximum, sum, accumulator)
 // in the workspace for the join.
 //
-// Memory bound: every cached byte is read once (counters: 1.004 to 1.02 times the cache's bytes), 4 q_heads d flops a token are
-// 3% of the matrix rate at that speed. On MI355X (copy of 1 GiB 5.14 TB/s), head length 128, 28 query on 4 key-value
-// heads, us: 64 sequences of 2000 to 16384 tokens in bf16 (929 MB) 147 and 5 for the join, 32 of up to 4096 (69 MB) 15.6
-// and 4.0, 128 of up to 2048 in e4m3 (90 MB) 24.4 in one launch, one of 32749 in e4m3 (35 MB) 11.5 and 4.9. Beside
-// the bytes a call takes some 5.5 (a launch; lengths, table and keys wait for each other; the last join in LDS).
+// Memory bound: every cached byte is read once (counters: 1.004 to 1.02 times the cache's bytes), 4 q_heads d flops a
+// token are 3% of the matrix rate at that speed. On MI355X (copy of 1 GiB 5.14 TB/s), head length 128, 28 query on 4
+// key-value heads, us: 64 sequences of 2000 to 16384 tokens in bf16 (929 MB) 147 and 5 for the join, 32 of up to 4096
+// (69 MB) 15.6 and 4.0, 128 of up to 2048 in e4m3 (90 MB) 24.4 in one launch, one of 32749 in e4m3 (35 MB) 11.5 and
+// 4.9. Beside the bytes a call takes some 5.5 (a launch; lengths, table and keys wait for each other; the
+// last join in LDS).
 //
 // A wave takes every fourth step. S^T = K Q^T by v_mfma_f32_16x16x32 with 16 tokens as rows and 16 query heads as
 // columns: lane 16g + c then holds head c's scores of tokens 4g .. 4g + 3 of each tile, which is, for the second
@@ -72,8 +73,8 @@ __host__ __device__ constexpr int64_t piece_floats(int rows, int dp) { return ro
 // a whole item and none knows the others' lengths, by what the table covers. Each byte is read once; a call that fills
 // a good part of the 256 MB last-level cache only pushes out of it what other kernels left. MI355X, three caches in
 // turn, us without and with: 64 sequences of 2000 to 16384 tokens (929 MB) 169 and 150, 8 of 8192 (134 MB) 31.7 and
-// 28.5; 32 of up to 4096 (69 MB), where three caches stay in it, 19.2 and 21.4. Whole items: 512 of up to 512 tokens (table
-// 537 MB) 97.4 and 92.1, 128 of up to 2048 in e4m3 (table 268 MB) 24.1 and 26.3.
+// 28.5; 32 of up to 4096 (69 MB), where three caches stay in it, 19.2 and 21.4. Whole items: 512 sequences of up to 512
+// tokens (table 537 MB) 97.4 and 92.1, 128 of up to 2048 in e4m3 (table 268 MB) 24.1 and 26.3.
 constexpr int64_t kStreamLine = 100 << 20, kStreamTable = 384 << 20;
 
 // Where a workgroup leaves its part of an item: it has at most two such, of an item that began before it and of one
