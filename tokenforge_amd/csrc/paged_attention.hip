@@ -12,6 +12,7 @@ struct JoinArgs {
   uint16_t* out;
   int heads, group, row_groups, part_rows, d, dp, tiles;
   uint32_t count;  // sequences * query heads
+  int grid;        // workgroups of the attention
 };
 
 // Part of a row: its channels y of a lane, in units of 2^top, and the sum l of the probabilities.
@@ -44,7 +45,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(Joi
   const int b = (int)(at / q_heads), qh = (int)(at - (uint32_t)b * q_heads);
   const int head = qh / a.group, in = qh - head * a.group, rg = in / (16 * a.tiles), row = in - rg * 16 * a.tiles;
   const int n = a.lens[b];
-  const int2 ends = a.ends[((int64_t)b * a.heads + head) * a.row_groups + rg];
+  const int2 found = a.ends[((int64_t)b * a.heads + head) * a.row_groups + rg];
+  // (within the pieces, also where lengths change under the call and an item was left out)
+  const int2 ends{found.x > 0 ? found.x : 0, found.y < a.grid ? found.y : a.grid - 1};
   const int lanes = a.dp >> 2, side = 64 / lanes, part = lane / lanes, e = (lane & (lanes - 1)) * 4;
   uint16_t* const out = a.out + (int64_t)at * a.d;
   const bool writes = (WAVES == 1 || wave == 0) && part == 0 && e < a.d;
@@ -52,7 +55,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(Joi
     if (writes) *reinterpret_cast<u2*>(out + e) = u2{0u, 0u};
     return;
   }
-  if (ends.x == ends.y) return;
+  if (ends.x >= ends.y) return;
   const int64_t size = piece_floats(a.part_rows, a.dp);
   Part mine{-__builtin_inff(), 0.0f, f4{0.0f, 0.0f, 0.0f, 0.0f}};
   const int each = WAVES * side;
@@ -207,7 +210,8 @@ extern "C" int tf_paged_attention(const tf_kv_cache* cache, const uint16_t* q, i
   if (rc) return rc;
   if (p.direct) return TF_OK;
   const auto count = (uint32_t)(m * q_heads);
-  const JoinArgs j{a.part, a.ends, seq_lens, out, c.heads, p.group, p.row_groups, p.part_rows, a.d, p.dp, p.tiles, count};
+  const JoinArgs j{a.part,       a.ends,      seq_lens, out,  c.heads, p.group,
+                   p.row_groups, p.part_rows, a.d,      p.dp, p.tiles, count,   (int)p.grid};
   if (count >= kJoinByWave)
     bf16 ? join_kernel<BF16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j)
          : join_kernel<F16, 1><<<(unsigned)cdiv(count, 4), 256, 0, s>>>(j);
