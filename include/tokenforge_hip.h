@@ -399,7 +399,8 @@ int tf_kv_cache_read(const tf_kv_cache* cache, const int64_t* slots, uint16_t* k
  * elements, rows on 16 bytes) and out [m, q_heads, head_dim] contiguous of the 16-bit type `dtype`, the cache's own
  * or any for e4m3; block_table int32 [m, width], row stride table_stride; seq_lens int32 [m]; width *
  * page_size < 2^31 - 256 and the steps of 16 tokens of all heads' table rows below 2^31. Products are exact and
- * summed in fp32, probabilities carry 16 bits or more into the second product.
+ * summed in fp32; probabilities carry 16 bits or more into the second product, with 16-bit fp16 values those from
+ * 2^-24 of the row's largest on (smaller ones are off by up to 2^-40 of it).
  * workspace: fp32, 16-byte aligned, >= tf_paged_attention_workspace_bytes (-1 for sizes the attention refuses).
  * Two calls that may overlap need workspaces of their own. */
 int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads, int64_t width,

@@ -22,10 +22,10 @@
 // for 4 bytes. No step goes through LDS. Running maximum, sum and accumulator are fp32; the waves' are joined in
 // LDS when an item ends.
 //
-// Probabilities go into the second product as two 16-bit halves (p truncated, and the rest), 16 to 22 bits
-// together: the product is memory bound, and with one half alone a bf16 result is off by 1.4 times its own
-// rounding. The lower half is never zero where the upper is not, so that an infinite value times it is infinite
-// and not NaN. Scales of e4m3 values go into the probabilities before the split, e4m3 codes into bf16 (exact).
+// Probabilities go into the second product as two 16-bit halves, 16 bits together in bf16, 21 in fp16 (fewer below 2^-19
+// of the row's largest, split2): the product is memory bound, and with one half alone a bf16 result is off by 1.4 times
+// its own rounding. The lower half is not zero where the upper is not, so that an infinite value times it is infinite and
+// not NaN. Scales of e4m3 values go into the probabilities before the split, e4m3 codes into bf16 (exact).
 #pragma once
 
 #include "kv_cache.h"
@@ -130,9 +130,16 @@ __device__ __forceinline__ float sum4(float v) {
   return as_f32(s[0]) + as_f32(s[1]);
 }
 
-// Probabilities p0, p1 as two pairs: truncated, and what is left (see the top). fp16 ones come multiplied by
-// 2^kBias, which keeps them normal down to 2^-24 of the row's largest; the factor cancels in the quotient.
-constexpr float kBias = 10.0f;
+// Probabilities p0, p1 as two pairs that add up to them (see the top). bf16: truncated, and what is left. fp16, of
+// probabilities times kUp: a little less than truncated, and what is left, rounded.
+//
+// fp16 pairs end on the subnormals' step of 2^-24, 2^-39 of the row's largest: a probability is off by half of that,
+// or by 2^-21 of itself if that is more, to either side, so 16 bits hold down to 2^-24 of the largest (16.6 in the
+// scores), 12 at 2^-28. kUp is the most that the largest may be multiplied by. What is left is 2^-24 or more wherever
+// the upper half is not 0 (the product with 1 - 2^-12 and the 2^-24 taken off see to it for values that fp16 holds
+// exactly), so that an infinite value stays one for probabilities from 2^-37 of the largest on; far below, and in bf16
+// below 2^-106, it gives NaN, as in fp32 below 2^-149.
+constexpr float kUp = 0x1p15f;
 
 template <bool WIDE>
 __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
@@ -141,12 +148,11 @@ __device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_
     const float r0 = p0 - as_f32(as_u32(p0) & 0xFFFF0000u), r1 = p1 - as_f32(as_u32(p1) & 0xFFFF0000u);
     lo = round_pair<BF16>(r0 != 0.0f ? r0 : p0 * 0x1p-20f, r1 != 0.0f ? r1 : p1 * 0x1p-20f);
   } else {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+    constexpr float kLess = kUp * (1.0f - 0x1p-12f);
+    const auto h = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaxf(__builtin_fmaf(p0, kLess, -0x1p-24f), 0.0f),
+                                              __builtin_fmaxf(__builtin_fmaf(p1, kLess, -0x1p-24f), 0.0f));
     hi = __builtin_bit_cast(uint32_t, h);
-    const float h0 = (float)h[0], h1 = (float)h[1];
-    const float r0 = __builtin_fmaxf(p0 - h0, h0 > 0.0f ? 0x1p-24f : 0.0f);
-    const float r1 = __builtin_fmaxf(p1 - h1, h1 > 0.0f ? 0x1p-24f : 0.0f);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+    lo = round_pair<F16>(__builtin_fmaf(p0, kUp, -(float)h[0]), __builtin_fmaf(p1, kUp, -(float)h[1]));
   }
 }
 
@@ -408,7 +414,7 @@ __device__ __forceinline__ void softmax(Attn<T, FP8, DP, MT, PAGED, FULL>& s,
         for (int r = 0; r < 4; ++r) s.acc[t][j][r] *= f;
       s.top[t] = m;
     }
-    const float ref = (m == -__builtin_inff() ? 0.0f : m) - (A::PW ? 0.0f : kBias);
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < A::NT; ++i)
 #pragma unroll
@@ -688,7 +694,7 @@ __device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t l
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int nrows = rows_of(it) - 16 * m < 16 ? rows_of(it) - 16 * m : 16;  // none of the last 16, maybe
-      const float own = sum4(s.sum[m]);
+      const float own = sum4(s.sum[m]) * (A::PW ? 1.0f : kUp);  // as the products are
       if (c < nrows) {
         if (g == 0) ends[half][wave][c] = float2{s.top[m], own};
 #pragma unroll
