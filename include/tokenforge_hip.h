@@ -395,7 +395,7 @@ int tf_kv_cache_read(const tf_kv_cache* cache, const int64_t* slots, uint16_t* k
  *   out[b][j] = sum_i p_i v_i / sum_i p_i,  p_i = exp(scale * q[b][j] . k_i - max)
  * over i in [max(0, n - window), n) (window 0: [0, n)), n = seq_lens[b] clamped to [0, width * page_size], head
  * j reading key-value head j / (q_heads / heads). Token i lies in page block_table[b][i / page_size]; the tokens
- * of a page index outside [0, pages) take no part. No token left: zeros. q [m, q_heads, head_dim] (strides in
+ * of a page index outside [0, pages) take no part. No token left: zeros; all of those left scoring -infinity: NaN. q [m, q_heads, head_dim] (strides in
  * elements, rows on 16 bytes) and out [m, q_heads, head_dim] contiguous of the 16-bit type `dtype`, the cache's own
  * or any for e4m3; block_table int32 [m, width], row stride table_stride; seq_lens int32 [m]; width *
  * page_size < 2^31 - 256 and the steps of 16 tokens of all heads' table rows below 2^31. Products are exact and

@@ -330,6 +330,10 @@ __device__ __forceinline__ void load_v(const AttnArgs& a, Attn<T, FP8, DP, MT, P
 
 // ------------------------------------------------------------------ one step
 
+// The maximum of a part whose tokens all score -infinity: 0 / 0 in the end, NaN, if the others' do too, where a maximum
+// of -infinity says that no token takes part, and gives zeros.
+constexpr float kLeast = -3.402823466e38f;
+
 // Whether token 4g + r of tile i of the step takes part.
 template <typename A, bool PAGED>
 __device__ __forceinline__ bool takes_part(uint32_t step, int i, int r, int g, int begin, int end, uint64_t bits) {
@@ -345,9 +349,9 @@ __device__ __forceinline__ bool all_take_part(uint32_t step, int begin, int end,
 }
 
 // Scores of the step's tokens, in units of log2, -inf where a token takes no part: x[tile][r] of head c, token
-// 4g + r.
+// 4g + r. Returns whether any takes part (uniform).
 template <typename T, bool FP8, int DP, int MT, bool PAGED, bool FULL>
-__device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, uint32_t step, int begin,
+__device__ __forceinline__ bool scores(const AttnArgs& a, Attn<T, FP8, DP, MT, PAGED, FULL>& s, uint32_t step, int begin,
                                        int end, uint64_t bits, int lane,
                                        float (&x)[MT][Attn<T, FP8, DP, MT, PAGED, FULL>::NT][4]) {
   using A = Attn<T, FP8, DP, MT, PAGED, FULL>;
@@ -380,15 +384,18 @@ __device__ __forceinline__ void scores(const AttnArgs& a, Attn<T, FP8, DP, MT, P
       for (int m = 0; m < MT; ++m) x[m][i][r] = FP8 ? t[m][r] * a.scale_log2 * ks : t[m][r] * a.scale_log2;
     }
   }
-  if (all_take_part<A, PAGED>(step, begin, end, bits)) return;
+  if (all_take_part<A, PAGED>(step, begin, end, bits)) return true;
+  bool some = false;
 #pragma unroll
   for (int i = 0; i < A::NT; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (!takes_part<A, PAGED>(step, i, r, g, begin, end, bits)) {
+    for (int r = 0; r < 4; ++r) {
+      const bool in = takes_part<A, PAGED>(step, i, r, g, begin, end, bits);
+      some |= in;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) x[m][i][r] = -__builtin_inff();
-      }
+      for (int m = 0; m < MT; ++m) x[m][i][r] = in ? x[m][i][r] : -__builtin_inff();
+    }
+  return __builtin_amdgcn_ballot_w64(some) != 0;
 }
 
 // Scores -> probabilities: the running maximum, the accumulators' rescaling, the sum.
@@ -650,6 +657,7 @@ __device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t l
       for (int j = 0; j < A::NSUB * A::CS; ++j) s.acc[m][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const uint32_t last = it.first + it.stop;
+    bool any = false;  // whether a token of the wave's steps takes part
     if (has) {
       float x[MT][A::NT][4];
       if (!FULL) {
@@ -663,7 +671,7 @@ __device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t l
       if (step + 4 * A::kAhead < last) entry = look_up<A, PAGED>(a, table_of(it), step + 4 * A::kAhead, limit_of(it), lane);
       for (; step + 4 < last; step += 4) {
         const uint64_t bits = step_bits<A, PAGED>(at, slot);
-        scores(a, s, step, it.begin, it.end, bits, lane, x);
+        any |= scores(a, s, step, it.begin, it.end, bits, lane, x);
         if (++slot == A::kAhead) {
           slot = 0;
           at = places_of<A, PAGED, FP8>(a, entry, step + 4, it.end, lane);
@@ -675,7 +683,7 @@ __device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t l
         get_v(it, at, slot);
       }
       const uint64_t bits = step_bits<A, PAGED>(at, slot);
-      scores(a, s, step, it.begin, it.end, bits, lane, x);
+      any |= scores(a, s, step, it.begin, it.end, bits, lane, x);
       softmax(s, x);
       accumulate(s, step, it.begin, it.end, bits, lane, x);
     }
@@ -696,7 +704,7 @@ __device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t l
       const int nrows = rows_of(it) - 16 * m < 16 ? rows_of(it) - 16 * m : 16;  // none of the last 16, maybe
       const float own = sum4(s.sum[m]) * (A::PW ? 1.0f : kUp);  // as the products are
       if (c < nrows) {
-        if (g == 0) ends[half][wave][c] = float2{s.top[m], own};
+        if (g == 0) ends[half][wave][c] = float2{any ? __builtin_fmaxf(s.top[m], kLeast) : s.top[m], own};
 #pragma unroll
         for (int n = 0; n < A::NSUB; ++n)
 #pragma unroll
@@ -729,7 +737,7 @@ __device__ __forceinline__ void run_items(const AttnArgs& a, Item it, uint32_t l
           y += part[w] * f;
         }
         if (whole) {
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          const float inv = t == -__builtin_inff() ? 0.0f : 1.0f / l;
           if (FULL || d0 < a.d)
             store4<T>(a.out + (((int64_t)it.b * a.heads + it.head) * a.group + it.row + 16 * m + row) * a.d + d0,
                       y * inv);

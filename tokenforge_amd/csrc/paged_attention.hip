@@ -87,7 +87,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(Joi
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) merge(mine, parts[w][lane].top, parts[w][lane].l, parts[w][lane].y);
   }
-  if (writes) store4<T>(out + e, mine.y * (mine.l == 0.0f ? 0.0f : 1.0f / mine.l));
+  if (writes) store4<T>(out + e, mine.y * (mine.top == -__builtin_inff() ? 0.0f : 1.0f / mine.l));
 }
 
 // Rows from which a wave each fills the CUs in the join; below, items so few and long that one has some sixty pieces
