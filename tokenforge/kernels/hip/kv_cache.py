@@ -37,6 +37,35 @@ def _rows_apart(t: torch.Tensor) -> bool:
     return True
 
 
+def _runs(t: torch.Tensor) -> tuple[list[tuple[int, int]], int]:
+    """``t`` as runs of bytes: its dimensions of two or more as (stride in bytes, size), the largest stride first, and the
+    bytes of a run (a cache's row, a scale)."""
+    e = t.element_size()
+    dims = [(st * e, sz) for st, sz in zip(t.stride()[:3], t.shape) if sz > 1]
+    return sorted(dims, reverse=True), e * (t.shape[3] if t.dim() == 4 else 1)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether tensors of nested dimensions (:func:`_rows_apart`) share memory. A dimension of one stride in both is settled
+    by the one or two differences of its indices that bring what lies within it together; from one on where the
+    strides differ, ranges that meet count as overlap."""
+    (da, ra), (db, rb) = _runs(a), _runs(b)
+
+    def meet(far: int, i: int) -> bool:
+        ea, eb = (r + sum(st * (sz - 1) for st, sz in d[i:]) for d, r in ((da, ra), (db, rb)))
+        if far >= ea or far <= -eb:
+            return False
+        if i >= len(da) or i >= len(db) or da[i][0] != db[i][0]:
+            return True
+        s, na = da[i]
+        nb = db[i][1]
+        ia, ib = ea - s * (na - 1), eb - s * (nb - 1)
+        first, last = (-ib - far) // s + 1, (ia - 1 - far) // s
+        return any(meet(far + s * t, i + 1) for t in range(max(first, 1 - na), min(last, nb - 1) + 1))
+
+    return meet(b.data_ptr() - a.data_ptr(), 0)
+
+
 def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor | None,
                 v_scale: torch.Tensor | None, *, written: bool = False) -> tuple[int, int, int, int]:
     """Checks of a cache, on any device; returns ``(pages, heads, page_size, head_dim)``."""
@@ -75,6 +104,13 @@ def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Ten
             raise ValueError("k_scale and v_scale are written and must not be one tensor")
     if written and k_cache.data_ptr() == v_cache.data_ptr():
         raise ValueError("k_cache and v_cache are written and must not be one tensor")
+    if written:
+        held = [(n, t) for n, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale),
+                                    ("v_scale", v_scale)) if t is not None]
+        for j, (name, t) in enumerate(held):
+            for other, u in held[:j]:
+                if _overlap(u, t):
+                    raise ValueError(f"{other} and {name} are written and must not overlap")
     return pages, heads, page_size, d
 
 

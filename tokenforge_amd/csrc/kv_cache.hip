@@ -9,6 +9,7 @@
 // 8191 tokens of 36 rows rotated into bf16 (155 MB) 32.4, 4095 of 8 rows written in e4m3 (13 MB) 5.7, 32767 read from
 // e4m3 slots in no order (102 MB, and a line of memory for each of 262136 scales) 21.5; one token 3.1.
 #include "kv_cache.h"
+#include "overlap.h"
 
 namespace tf {
 namespace {
@@ -350,6 +351,20 @@ KvArgs cache_args(const tf_kv_cache& c) {
 std::string written_error(const tf_kv_cache& c) {
   if (c.k == c.v) return "keys and values are written to one place";
   if (c.dtype == TF_DTYPE_E4M3 && c.k_scale == c.v_scale) return "scales of keys and values are written to one place";
+  const bool fp8 = c.dtype == TF_DTYPE_E4M3;
+  const int64_t size[3] = {c.pages, c.heads, c.page_size};
+  const auto placed = [&](const void* p, const int64_t (&stride)[3], int64_t bytes, int64_t run) {
+    Runs r(p, run);
+    for (int i = 0; i < 3; ++i) r.add(stride[i] * bytes, size[i]);
+    return r;
+  };
+  const int e = fp8 ? 1 : 2;
+  const Runs all[4] = {placed(c.k, c.k_strides, e, e * c.head_dim), placed(c.v, c.v_strides, e, e * c.head_dim),
+                       placed(c.k_scale, c.k_scale_strides, 4, 4), placed(c.v_scale, c.v_scale_strides, 4, 4)};
+  const char* const names[4] = {"k", "v", "k_scale", "v_scale"};
+  for (int i = 0; i < (fp8 ? 4 : 2); ++i)
+    for (int j = 0; j < i; ++j)
+      if (overlap(all[j], all[i])) return std::string(names[j]) + " and " + names[i] + " of the cache overlap";
   return "";
 }
 
