@@ -23,6 +23,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/library.h>
@@ -787,6 +788,14 @@ bool write_ok(const at::Tensor& k, const at::Tensor& v, const tf_kv_cache& c, at
          index_ok(slots, t, at::kLong, dev);
 }
 
+// Advances the written tensors' version counters, as torch's own writes do, so that a gradient's saved copy of one is
+// known to be stale. Inference tensors have none; where torch's writes leave them alone (below its own layer), so does this.
+void count_writes(const at::Tensor& k, const at::Tensor& v, const OptTensor& ks, const OptTensor& vs) {
+  if (c10::impl::tls_is_dispatch_key_excluded(c10::DispatchKey::ADInplaceOrView)) return;
+  for (const at::Tensor* t : {&k, &v, ks.has_value() ? &*ks : nullptr, vs.has_value() ? &*vs : nullptr})
+    if (t != nullptr && t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void kv_cache_write(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache, at::Tensor& v_cache,
                     const OptTensor& k_scale, const OptTensor& v_scale, const at::Tensor& slots) {
   tf_kv_cache c;
@@ -794,6 +803,7 @@ void kv_cache_write(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cach
   if (!cache_ok(k_cache, v_cache, k_scale, v_scale, true, c) ||
       !write_ok(k, v, c, k_cache.scalar_type(), slots, dev)) {
     python_body<KvWriteFn>("tokenforge::_py_kv_cache_write", k, v, k_cache, v_cache, k_scale, v_scale, slots);
+    count_writes(k_cache, v_cache, k_scale, v_scale);
     return;
   }
   c10::OptionalDeviceGuard guard(dev);
@@ -801,6 +811,7 @@ void kv_cache_write(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cach
                        step_of(v, 0), step_of(v, 1), dtype_code(k.scalar_type()), data<const int64_t>(slots),
                        k.size(0), c10::hip::getCurrentHIPStream(dev.index()).stream()),
         "tf_kv_cache_write");
+  count_writes(k_cache, v_cache, k_scale, v_scale);
 }
 
 at::Tensor rope_kv_cache_write(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -816,9 +827,12 @@ at::Tensor rope_kv_cache_write(const at::Tensor& q, const at::Tensor& k, const a
       !index_ok(positions, k.size(0), at::kLong, dev) || cos_sin.dim() != 2 || cos_sin.scalar_type() != at::kFloat ||
       !on(cos_sin, dev) || !cos_sin.is_contiguous() || cos_sin.size(0) == 0 || cos_sin.size(1) == 0 ||
       cos_sin.size(1) % 2 != 0 || cos_sin.size(1) > c.head_dim ||
-      reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 != 0)
-    return python_body<RopeKvWriteFn>("tokenforge::_py_rope_kv_cache_write", q, k, v, cos_sin, positions, k_cache,
-                                      v_cache, k_scale, v_scale, slots, interleaved);
+      reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 != 0) {
+    at::Tensor out = python_body<RopeKvWriteFn>("tokenforge::_py_rope_kv_cache_write", q, k, v, cos_sin, positions,
+                                                k_cache, v_cache, k_scale, v_scale, slots, interleaved);
+    count_writes(k_cache, v_cache, k_scale, v_scale);
+    return out;
+  }
   c10::OptionalDeviceGuard guard(dev);
   at::Tensor out = fresh(q.sizes(), q.scalar_type(), dev);
   check(api().rope_kv_write(&c, data<const uint16_t>(q), step_of(q, 0), step_of(q, 1), static_cast<int32_t>(q_heads),
@@ -828,6 +842,7 @@ at::Tensor rope_kv_cache_write(const at::Tensor& q, const at::Tensor& k, const a
                             data<const int64_t>(positions), data<const int64_t>(slots), data<uint16_t>(out),
                             k.size(0), c10::hip::getCurrentHIPStream(dev.index()).stream()),
         "tf_rope_kv_cache_write");
+  count_writes(k_cache, v_cache, k_scale, v_scale);
   return out;
 }
 
