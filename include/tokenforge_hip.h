@@ -396,12 +396,13 @@ int tf_kv_cache_read(const tf_kv_cache* cache, const int64_t* slots, uint16_t* k
  *   out[b][j] = sum_i p_i v_i / sum_i p_i,  p_i = exp(scale * q[b][j] . k_i - max)
  * over i in [max(0, n - window), n) (window 0: [0, n)), n = seq_lens[b] clamped to [0, width * page_size], head
  * j reading key-value head j / (q_heads / heads). Token i lies in page block_table[b][i / page_size]; the tokens
- * of a page index outside [0, pages) take no part. No token left: zeros; all of those left scoring -infinity: NaN. q [m, q_heads, head_dim] (strides in
- * elements, rows on 16 bytes) and out [m, q_heads, head_dim] contiguous of the 16-bit type `dtype`, the cache's own
- * or any for e4m3; block_table int32 [m, width], row stride table_stride; seq_lens int32 [m]; width *
- * page_size < 2^31 - 256 and the steps of 16 tokens of all heads' table rows below 2^31. Products are exact and
- * summed in fp32; probabilities carry 16 bits or more into the second product, with 16-bit fp16 values those from
- * 2^-24 of the row's largest on (smaller ones are off by up to 2^-40 of it).
+ * of a page index outside [0, pages) take no part. No token left: zeros; all of those left scoring -infinity: NaN.
+ * q [m, q_heads, head_dim] (strides in elements, rows on 16 bytes) and out [m, q_heads, head_dim] contiguous of the
+ * 16-bit type `dtype`, the cache's own or any for e4m3; block_table int32 [m, width], row stride table_stride;
+ * seq_lens int32 [m]. width * page_size < 2^31 - 256, and the steps of 16 tokens of all table rows, times the heads,
+ * times the 16s (past 16 and up to head_dim 128: 32s) of a head's query heads, below 2^31. Products are exact and summed
+ * in fp32; probabilities carry 16 bits or more into the second product, with 16-bit fp16 values those from 2^-24 of
+ * the row's largest on (smaller ones are off by up to 2^-40 of it).
  * workspace: fp32, 16-byte aligned, >= tf_paged_attention_workspace_bytes (-1 for sizes the attention refuses).
  * Two calls that may overlap need workspaces of their own. */
 int64_t tf_paged_attention_workspace_bytes(const tf_kv_cache* cache, int64_t m, int32_t q_heads, int64_t width,

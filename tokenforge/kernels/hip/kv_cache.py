@@ -195,7 +195,8 @@ def check_attention(q: torch.Tensor, cache: Cache, block_table: torch.Tensor, se
     if window < 0:
         raise ValueError(f"window must be 0 (none) or more, got {window}")
     width = block_table.shape[1]
-    items = m * heads * -(-(q.shape[1] // heads) // 16)
+    group = q.shape[1] // heads
+    items = m * heads * -(-group // (32 if group > 16 and d <= 128 else 16))  # query heads that share a pass, as the C entry
     if width > 0x7FFFFF00 // page_size or m * q.shape[1] > 0x7FFFFF or items * -(-width * page_size // 16) > 0x7FFFFFFF:
         raise ValueError(f"{m} sequences of {width} pages of {page_size} with {q.shape[1]} heads are too large")
     return m
