@@ -6,8 +6,8 @@
 // values, then the queries): their loads are on their way together, and the token's slot, position and angles are
 // read once. In the rotation by halves a lane's two chunks are each other's partners. Every byte is read and written
 // once; memory bound from some thousand tokens on, latency below. On MI355X (copy of 1 GiB 5.14 TB/s), heads of 128, us:
-// 8191 tokens of 36 rows rotated into bf16 (155 MB) 32.4, 4095 of 8 rows written in e4m3 (13 MB) 5.7, 32767 read from
-// e4m3 slots in no order (102 MB, and a line of memory for each of 262136 scales) 21.5; one token 3.1.
+// 8191 tokens of 36 rows rotated into bf16 (155 MB) 32.2, 4095 of 8 rows written in e4m3 (13 MB) 5.5, 32767 read from
+// e4m3 slots in no order (102 MB, and a line of memory for each of 262136 scales) 21.5; one token 2.8.
 #include "kv_cache.h"
 #include "overlap.h"
 

@@ -2,15 +2,16 @@
 // in paged_attention_d*.hip, launched and joined by paged_attention.hip.
 //
 // Work. Items are (sequence, key-value head, 16 or 32 of its query heads); an item is a run of steps of 16 NT tokens.
-// All items' steps form one line, and workgroup w takes the steps [w share, (w + 1) share) of it, so every
-// workgroup gets the same number whatever the sequences' lengths are. Lengths are read on the device; the host
-// knows none. Items that lie in one workgroup are finished by it, the others leave (maximum, sum, accumulator)
-// in the workspace for the join.
+// All items' steps form one line, and workgroup w takes the steps [w share, (w + 1) share) of it: parts that end with
+// their item where the grid is enough for those, else equal ones across items, whatever the sequences' lengths are.
+// Lengths are read on the device; the host knows none. Items that lie in one workgroup are finished by it, the others
+// leave (maximum, sum, accumulator) in the workspace for the join. Where the table's rows are short, a workgroup takes an
+// item and there is no line.
 //
 // Memory bound: every cached byte is read once (counters: 1.004 to 1.02 times the cache's bytes), 4 q_heads d flops a
 // token are 3% of the matrix rate at that speed. On MI355X (copy of 1 GiB 5.14 TB/s), head length 128, 28 query on 4
 // key-value heads, us: 64 sequences of 2000 to 16384 tokens in bf16 (929 MB) 147 and 5 for the join, 32 of up to 4096
-// (69 MB) 15.6 and 4.0, 128 of up to 2048 in e4m3 (90 MB) 24.4 in one launch, one of 32749 in e4m3 (35 MB) 11.5 and
+// (69 MB) 15.6 and 3.9, 128 of up to 2048 in e4m3 (90 MB) 24.8 in one launch, one of 32749 in e4m3 (35 MB) 11.8 and
 // 4.9. Beside the bytes a call takes some 5.5 (a launch; lengths, table and keys wait for each other; the
 // last join in LDS).
 //
@@ -62,7 +63,8 @@ struct AttnArgs {
 // steps would end before the next one's loads are back.
 constexpr int attention_step(int dp) { return dp == 64 ? 64 : 32; }
 
-// Workgroups a CU holds, and the grid of the shared line: two by their 180 to 190 registers, one for heads past 128.
+// Workgroups a CU holds, and the grid of the shared line: two by their 167 to 256 registers, one for heads past 128
+// (320 to 420, and 134 KB of LDS).
 constexpr int attention_resident(int dp) { return dp > 128 ? 1 : 2; }
 constexpr int attention_grid(int dp) { return 256 * attention_resident(dp); }
 
@@ -74,7 +76,8 @@ __host__ __device__ constexpr int64_t piece_floats(int rows, int dp) { return ro
 // a good part of the 256 MB last-level cache only pushes out of it what other kernels left. MI355X, three caches in
 // turn, us without and with: 64 sequences of 2000 to 16384 tokens (929 MB) 169 and 150, 8 of 8192 (134 MB) 31.7 and
 // 28.5; 32 of up to 4096 (69 MB), where three caches stay in it, 19.2 and 21.4. Whole items: 512 sequences of up to 512
-// tokens (table 537 MB) 97.4 and 92.1, 128 of up to 2048 in e4m3 (table 268 MB) 24.1 and 26.3.
+// tokens (table 537 MB) 97.4 and 92.1, 128 of up to 2048 in e4m3 (table 268 MB) 24.1 and 26.3. Only the form of whole
+// tiles and exact head lengths has such a loop.
 constexpr int64_t kStreamLine = 100 << 20, kStreamTable = 384 << 20;
 
 // Where a workgroup leaves its part of an item: it has at most two such, of an item that began before it and of one

@@ -31,7 +31,7 @@ __device__ __forceinline__ void merge(Part& a, float top, float l, const f4& y) 
 }
 
 // out = sum_p acc_p 2^(top_p - top) / sum_p sum_p 2^(top_p - top) of a sequence's query head over the pieces p that
-// the attention's workgroups left, by one wave (WAVES 1) or a workgroup of 16. dp / 4 lanes take a piece; a wave takes
+// the attention's workgroups left, by one wave (WAVES 1) or a workgroup of 4 or 8. dp / 4 lanes take a piece; a wave takes
 // 64 / (dp / 4) side by side, four of each at once, and the parts are merged in an order that depends on the number
 // of pieces alone. Items that one workgroup held are done already; sequences without tokens get zeros here.
 template <typename T, int WAVES>
@@ -90,17 +90,26 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void join_kernel(Joi
   if (writes) store4<T>(out + e, mine.y * (mine.top == -__builtin_inff() ? 0.0f : 1.0f / mine.l));
 }
 
-// Rows from which a wave each fills the CUs in the join; below, items so few and long that one has some sixty pieces
-// or more get 8 waves a row (MI355X, one sequence of 32749 tokens in e4m3: 16.6 us with it, 17.9 with 4 waves and
-// 16.7 with 16, which cost one of 4096 0.5 and 1.3 us).
+// Rows from which a wave each fills the CUs in the join; below, few items get 8 waves a row where the table has room for
+// long ones (the host knows no lengths): of 8 items that fill the line one has 64 pieces, past heads of 128 32 (MI355X,
+// one sequence of 32749 tokens in e4m3: 16.6 us with 8 waves, 17.9 with 4 and 16.7 with 16, which cost one of
+// 4096 0.5 and 1.3 us).
 constexpr uint32_t kJoinByWave = 1024;
 constexpr int64_t kFewItems = 8, kLongItems = 8192;
 
-// Bytes of an item up to which a workgroup takes it whole, and with items for every place on the CUs (MI355X: 512
-// items of up to 512 KB in e4m3 25 us against 32, of 1 MB in 16 bits 57 against 49; 1024 of 256 KB 34 against 41;
-// 4 of 256 KB alike).
+// Bytes of an item up to which a workgroup takes it whole, by what the table's row holds, and the same from kManyItems
+// items on. MI355X, heads of 128 in e4m3, us whole and on the line; lengths that fill the row, then lengths spread over
+// the logarithm from a twentieth of it:
+//   items     256 KB                     384 KB                     512 KB                     1 MB
+//     400   24.3  28.0   13.6  18.1   35.7  38.4   17.4  21.4   45.6  46.8   21.5  27.4    84.3  82.2   47.8  39.4
+//     512   28.0  29.9   14.1  19.5   40.0  40.2   18.3  28.3   51.8  51.0   24.2  33.5    91.3  94.6   49.8  47.1
+//     520   35.3  36.0   14.8  28.4   50.3  47.6   18.4  28.7   65.3  59.0   24.6  35.2   120.1 103.9   49.8  47.9
+//     768   40.9  46.0   22.7  32.8   63.5  70.8   31.7  39.1   70.0  80.0   44.6  46.4   134.7 144.5   78.0  63.9
+//    1024   53.0  66.4   27.0  40.3   73.4  87.6   38.9  46.8   92.9 110.4   48.4  56.2   177.7 238.8   91.5  82.6
+// In bf16 512 items of 512 KB take 48.2, 47.5, 20.4 and 28.5, of 1 MB 88.8, 92.1, 44.7 and 42.6; 4 items of 256 KB 10.7 and
+// 8.1 in e4m3, 8.0 and 8.1 in bf16. So whole items gain up to the limits, but for a few items in e4m3 and just past a round of
+// the grid's places (520 equal ones); from 400 items on they would gain past 256 KB as well.
 constexpr int64_t kDirect = 256 << 10, kDirectMany = 512 << 10, kManyItems = 512;
-
 
 bool multiple(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
@@ -119,7 +128,11 @@ std::string plan_of(const tf_kv_cache& c, int64_t m, int32_t q_heads, int64_t wi
   p.fp8 = c.dtype == TF_DTYPE_E4M3;
   p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   p.group = q_heads / c.heads;
-  // Past 16 query heads a key-value head, 32 share its loads where the registers hold both.
+  // Past 16 query heads a key-value head, 32 share its loads; past heads of 128 the registers hold no second tile. With
+  // whole tiles of exact lengths they hold both, and 161 sequences of up to 4096 with 20 query heads on each of 2 take
+  // 54 us against 82 in 16 bits, 44 against 57 in e4m3 (32 sequences: 19.5 against 21.9, 18.1 against 17.7). The forms that
+  // look each token up keep 10 to 42 registers a lane in scratch, the 16-bit one of odd lengths 2 or 3: 161 sequences with
+  // pages of 24 73.8 against 77.0 in bf16 and 52.6 against 59.3 in e4m3, 32 of them 23.1 against 21.5 and alike.
   p.tiles = p.group > 16 && p.dp <= 128 ? 2 : 1;
   p.row_groups = (int)cdiv(p.group, 16 * p.tiles);
   p.part_rows = p.group < 16 * p.tiles ? p.group : 16 * p.tiles;
