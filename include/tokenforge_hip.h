@@ -368,8 +368,8 @@ typedef struct {
  *   scale = max(amax / 448, 1/(448*512)) over the head, code = e4m3fn(RNE(value / scale)).
  * slots int64 [t]; a slot outside [0, pages * page_size) is not written (padding). Slots of one call must
  * differ: of two tokens with one slot it is not specified whose values stay. Keys and values (and their scales) are
- * written to places of their own, which may lie between each other's but must not overlap (refused), and none of
- * which the call reads as k, v or q.
+ * written to places of their own, which may lie between each other's but must not overlap (refused, and so are ranges
+ * that meet under different strides), and none of which the call reads as k, v or q.
  *
  * tf_rope_kv_cache_write: the same with q [t, q_heads, head_dim] and k rotated first, in fp32 up to the one
  * rounding (or the codes): with i < rot / 2, (a, b) = elements (i, i + rot/2), or (2i, 2i+1) if interleaved,
