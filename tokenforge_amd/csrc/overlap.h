@@ -29,10 +29,10 @@ struct Runs {
   }
 };
 
-// Runs a and, `far` bytes behind where a's lie, runs b, both within their dimension i on. A dimension of one stride in both
-// is settled by the (one or two) differences of its indices that bring what lies within it together; from one on where
-// the strides differ, ranges that meet count as overlap. So do not dimensions that are not nested (what lies within
-// one reaches over its stride), whose rows no caller here has.
+// Whether runs a and, `far` bytes behind where they begin, runs b share a byte, both from their dimension i on. A dimension
+// of one stride in both is settled by the (one or two) differences of its indices that bring what lies within it
+// together; where the strides differ, ranges that meet count as overlap. Dimensions that are not nested (what lies
+// within one reaches over its stride) are not looked into: the operators refuse them before.
 inline bool runs_meet(const Runs& a, const Runs& b, int64_t far, int i) {
   const int64_t ea = a.extent(i), eb = b.extent(i);
   if (far >= ea || far <= -eb) return false;
